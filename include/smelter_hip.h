@@ -346,6 +346,43 @@ int sm_nhwc_f16_to_float_array(const void* x, float* y, int32_t N, int32_t C, in
                                int32_t x_ld, sm_stream_t stream);
 size_t sm_float_array_count(int32_t N, int32_t C, int32_t H, int32_t W);
 
+/* ---- linear layers with 4-bit weights, and expert layers (csrc/kernels/mx4.hip, linear.hip, moe.hip) ----
+ * Where an MPSCNNFullyConnectedNode (Converters.swift:297) holds fp16 weights [N][K], these hold fp16, bf16 or MX4 ones, for one layer or for E experts of the same shape.
+ * No call allocates, synchronises or keeps anything between calls; every one can be captured into a graph. */
+enum { SM_F16 = 0, SM_BF16 = 1, SM_F32 = 2,
+       SM_MX4 = 3 /* blocks of 32 e2m1 elements along the row (16 bytes, even column in the low nibble; columns behind the end hold code 0) + one e8m0 scale byte per block, 2^(b - 127), 255 = NaN:
+                     codes [rows][ceil(K / 32)][16], 16-byte aligned, scales [rows][ceil(K / 32)], both dense */ };
+/* x [rows][K] of x_type (row stride x_ld elements) -> MX4.  Scale 2^(floor(log2 amax) - 2) (not below 2^-127), elements rounded to the nearest, ties to even, values above 6 scales become 6.
+ * A block with a NaN or an infinity becomes NaN (scale 255, codes 0). */
+int sm_mx4_quantize(const void* x, int32_t x_type, int64_t rows, int32_t K, int64_t x_ld, void* codes, void* scales, sm_stream_t stream);
+/* ... and the values it stands for, rounded once to y_type (exact in bf16 and fp32 wherever the value is in range) */
+int sm_mx4_dequantize(const void* codes, const void* scales, int64_t rows, int32_t K, void* y, int32_t y_type, int64_t y_ld, sm_stream_t stream);
+
+/* y[s][n] = act(bias[e][n] + sum_k x[r(s)][k] * w[e][n][k]) for the slots s of group e: offsets[e] <= s < offsets[e + 1], r(s) = rows ? rows[s] : s.
+ * gated: y[s][n] = silu(z[s][n]) * z[s][N + n], z = product + bias over the 2 N weight rows (gate rows first).
+ * `offsets` (device, E + 1 ascending values) may be NULL when E = 1: all M slots then.  Slots that no group covers are left as they were.  Offsets are read as clamped to 0 .. M; a row index
+ * outside 0 .. T - 1 reads as a row of zeros.  fp32 accumulation, one rounding to y_type. */
+typedef struct sm_linear_desc {
+    int64_t M, T;                   /* slots (rows of y); rows of x */
+    int32_t N, K, E;                /* columns of y, inner size, groups (1 = an ordinary layer) */
+    int32_t x_type, w_type, y_type; /* fp16 | bf16 x on weights of the same type or MX4, y of x's type or fp32; MX4 x on MX4 weights, any y */
+    int32_t act; float slope;       /* SM_ACT_* behind the bias (not with gated) */
+    int32_t gated;
+    int64_t x_ld, y_ld;             /* row strides in elements, 0 = dense (an MX4 x is dense) */
+} sm_linear_desc;
+int sm_linear_fwd(const sm_linear_desc* d, const void* x, const void* x_scales, const void* w, const void* w_scales, const float* bias /* [E][N or 2 N] or NULL */, const int32_t* offsets,
+                  const int32_t* rows, void* y, sm_stream_t stream);
+
+/* Routing: for each of T tokens the k <= 32 largest of its E <= 1024 scores (ties: the lower index first) and their softmax weights (over the chosen ones, or over all E when !renormalize),
+ * and the assignments in the order of their expert (stable): offsets [E + 1], rows [T k] = token of each slot, slots [T][k] = slot of each assignment.  A score of -inf or NaN is never
+ * chosen: what is missing to k gets expert -1, weight 0, slot -1, and rows behind offsets[E] hold -1.  Workspace: sm_moe_route_workspace_bytes. */
+size_t sm_moe_route_workspace_bytes(int64_t T, int32_t E, int32_t k);
+int sm_moe_route(const void* scores, int32_t type, int64_t T, int32_t E, int32_t k, int64_t ld, int32_t renormalize, float* weights /* [T][k] */, int32_t* experts /* [T][k] */,
+                 int32_t* offsets, int32_t* rows, int32_t* slots, void* workspace, size_t workspace_bytes, sm_stream_t stream);
+/* out[t] = sum_j weights[t][j] * y[slots[t][j]] over [M][N] rows of y (fp16 | bf16), added in the order of j in fp32; a slot outside 0 .. M - 1 adds nothing */
+int sm_moe_combine(const void* y, int32_t type, int64_t M, int32_t N, int64_t y_ld, const float* weights, const int32_t* slots, int64_t T, int32_t k, void* out, int64_t out_ld,
+                   sm_stream_t stream);
+
 /* Host-side weight preparation Smelter does on the CPU at load time */
 /* Float16.swift:17-77 (IEEE, RNE) */
 void sm_half_to_float(const uint16_t* src, float* dst, size_t n);

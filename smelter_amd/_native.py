@@ -77,6 +77,12 @@ class RunInfo(C.Structure):
                 ("err_bits", C.c_int32), ("why_off", C.c_int32), ("t_run_us", C.c_float), ("t_layers_us", C.c_float)]
 
 
+class LinearDesc(C.Structure):
+    """sm_linear_desc (include/smelter_hip.h): a linear layer, dense or grouped by expert (sm_linear_fwd)"""
+    _fields_ = [("M", C.c_int64), ("T", C.c_int64)] + [(n, C.c_int32) for n in ("N", "K", "E", "x_type", "w_type", "y_type", "act")] + \
+               [("slope", C.c_float), ("gated", C.c_int32), ("x_ld", C.c_int64), ("y_ld", C.c_int64)]
+
+
 SYMBOLS = {
     "smelter_last_error_string": (C.c_char_p, []),
     "smelter_version": (C.c_char_p, []),
@@ -143,6 +149,12 @@ SYMBOLS = {
     "sm_nhwc_f16_to_nchw_f32": (_i32, [_vp, _vp] + [_i32] * 5 + [_vp]),
     "sm_nhwc_f16_to_float_array": (_i32, [_vp, _vp] + [_i32] * 5 + [_vp]),
     "sm_float_array_count": (_sz, [_i32] * 4),
+    "sm_mx4_quantize": (_i32, [_vp, _i32, _i64, _i32, _i64, _vp, _vp, _vp]),
+    "sm_mx4_dequantize": (_i32, [_vp, _vp, _i64, _i32, _vp, _i32, _i64, _vp]),
+    "sm_linear_fwd": (_i32, [C.POINTER(LinearDesc)] + [_vp] * 9),
+    "sm_moe_route_workspace_bytes": (_sz, [_i64, _i32, _i32]),
+    "sm_moe_route": (_i32, [_vp, _i32, _i64, _i32, _i32, _i64, _i32] + [_vp] * 6 + [_sz, _vp]),
+    "sm_moe_combine": (_i32, [_vp, _i32, _i64, _i32, _i64, _vp, _vp, _i64, _i32, _vp, _i64, _vp]),
     "sm_half_to_float": (None, [_vp, _vp, _sz]),
     "sm_float_to_half": (None, [_vp, _vp, _sz]),
     "sm_reformat_conv_weight": (_i32, [_vp, _vp] + [_i32] * 6),

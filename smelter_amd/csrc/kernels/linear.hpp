@@ -1,0 +1,122 @@
+// smelter_amd/csrc/kernels/linear.hpp — what the linear-layer kernels (linear.hip) share: element types, the MX4 block format, group lookup, epilogue.
+//
+//     y[s, n] = act(bias[e, n] + sum_k x[r(s), k] * w[e, n, k])          e = the group slot s lies in: offsets[e] <= s < offsets[e + 1];  r(s) = rows ? rows[s] : s
+//     gated:  y[s, n] = silu(z[s, n]) * z[s, N + n],  z = the product (with bias) over 2 N weight rows
+//
+// Operand kinds: fp16 / bf16 (2 bytes), MX4 = blocks of 32 e2m1 elements along K (16 bytes, even element in the low nibble) with one e8m0 scale byte 2^(b - 127) each (255 = NaN).
+#pragma once
+#include "common.hpp"
+
+typedef __bf16 bf16_t;
+typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
+typedef int intx4_t __attribute__((ext_vector_type(4)));
+typedef int intx8_t __attribute__((ext_vector_type(8)));
+typedef float floatx2_t __attribute__((ext_vector_type(2)));
+
+struct LinearParams {
+    const char* x; const unsigned char* xs;         // x rows; scales of an MX4 x
+    const char* w; const unsigned char* ws;
+    const float* bias; void* y;
+    const int* offsets; const int* rows;
+    long long x_ld, xs_ld;                          // BYTES per x row / per scale row
+    long long w_ld, ws_ld, w_es, ws_es;             // BYTES per weight row, scale row, expert
+    long long y_ld, M, T;                           // y row stride in elements; slots; x rows
+    int N, K, E, act; float slope;
+    int gated, y_type, y_vec, w_rows;               // y_vec: four consecutive outputs may be stored as one 8 / 16-byte word;  w_rows = N or 2 N
+    long long m_tiles; int n_tiles;                 // launch grid: a bound on the row tiles (the real number is known on the device only) x column tiles
+};
+
+__device__ __forceinline__ float lin_act(float v, int act, float slope) {
+    if (act == SM_ACT_NONE) return v;
+    if (act == SM_ACT_RELU) return v < 0.f ? 0.f : v;
+    if (act == SM_ACT_PRELU) return v < 0.f ? v * slope : v;
+    return sm_act_other(v, act, slope);
+}
+__device__ __forceinline__ float lin_silu(float v) { return v / (1.f + __expf(-v)); }
+
+// one rounding to the output type (nearest even)
+__device__ __forceinline__ void lin_store1(void* y, long long i, float v, int type) {
+    if (type == SM_F16) ((half_t*)y)[i] = (half_t)v;
+    else if (type == SM_BF16) ((bf16_t*)y)[i] = (bf16_t)v;
+    else ((float*)y)[i] = v;
+}
+__device__ __forceinline__ void lin_store4(void* y, long long i, floatx4 v, int type) {
+    if (type == SM_F16) *(half4_t*)((half_t*)y + i) = __builtin_convertvector(v, half4_t);
+    else if (type == SM_BF16) { typedef __bf16 b4 __attribute__((ext_vector_type(4))); *(b4*)((bf16_t*)y + i) = __builtin_convertvector(v, b4); }
+    else *(floatx4*)((float*)y + i) = v;
+}
+
+struct LinTile { int e; long long row0; int rows; long long index, total; };   // group, first slot, rows of the tile (<= BM); index of the row tile and number of row tiles
+
+// Row tile `t` of the group list.  Every group is cut into tiles of BM slots; the offsets live on the device, so each wave counts the tiles of 64 groups at a time (prefix sum over the
+// lanes) until it has passed `t`.  Offsets are clamped to 0 .. M, a group that ends before it begins is empty: nothing outside the M slots is ever addressed, whatever they hold.
+// rows = 0: there is no such tile.  Wave-uniform.
+__device__ __forceinline__ long long lin_clamp(long long v, long long hi) { return v < 0 ? 0 : (v > hi ? hi : v); }
+__device__ __forceinline__ LinTile lin_find_tile(const LinearParams& p, int BM, long long t, bool want_total) {
+    LinTile r; r.e = 0; r.row0 = 0; r.rows = 0; r.index = t; r.total = 0;
+    if (!p.offsets) {
+        r.total = (p.M + BM - 1) / BM;
+        if (t < r.total) { r.row0 = t * BM; long long left = p.M - r.row0; r.rows = (int)(left < BM ? left : BM); }
+        return r;
+    }
+    const int lane = threadIdx.x & 63;
+    for (int base = 0; base < p.E; base += 64) {
+        int e = base + lane;
+        long long lo = 0, hi = 0;
+        if (e < p.E) { lo = lin_clamp(p.offsets[e], p.M); hi = lin_clamp(p.offsets[e + 1], p.M); }
+        int n = hi > lo ? (int)((hi - lo + BM - 1) / BM) : 0;
+        int sum = n;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) { int up = __shfl_up(sum, d); if (lane >= d) sum += up; }
+        const int all = __shfl(sum, 63);
+        if (r.rows == 0 && t < r.total + all) {
+            const unsigned long long past = __ballot(r.total + sum > t);
+            const int at = __builtin_ctzll(past);
+            const long long tl = t - r.total - (__shfl(sum, at) - __shfl(n, at));
+            const long long l = __shfl(lo, at), h = __shfl(hi, at);
+            r.e = base + at; r.row0 = l + tl * BM; r.rows = (int)((h - r.row0) < BM ? (h - r.row0) : BM);
+            if (!want_total) return r;
+        }
+        r.total += all;
+    }
+    return r;
+}
+
+// eight consecutive 16-bit elements k .. k + 7 of a row of K, zero behind its end (any alignment: the compiler's unaligned 16-byte load)
+__device__ __forceinline__ intx4_t lin_load8(const char* row, int k, int K) {
+    intx4_t v = {0, 0, 0, 0};
+    if (k + 8 <= K) __builtin_memcpy(&v, row + 2ll * k, 16);
+    else if (k < K) {
+        unsigned h[4] = {0, 0, 0, 0};
+#pragma unroll
+        for (int i = 0; i < 8; i++) if (k + i < K) { unsigned short q; __builtin_memcpy(&q, row + 2ll * (k + i), 2); h[i >> 1] |= (unsigned)q << (16 * (i & 1)); }
+        v = intx4_t{(int)h[0], (int)h[1], (int)h[2], (int)h[3]};
+    }
+    return v;
+}
+
+// eight MX4 elements (one dword of codes) as 16-bit values times the power of two `scale` (exact while the result is in the type's range; a NaN scale gives NaN)
+template <int KIND> __device__ __forceinline__ intx4_t mx4_to16(int codes, float scale) {
+    intx4_t r;
+    if constexpr (KIND == SM_F16) {
+        r[0] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, scale, 0)); r[1] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, scale, 1));
+        r[2] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, scale, 2)); r[3] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, scale, 3));
+    } else {
+        r[0] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 0)); r[1] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 1));
+        r[2] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 2)); r[3] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 3));
+    }
+    return r;
+}
+__device__ __forceinline__ float mx4_scale(int byte) { return __builtin_bit_cast(float, byte << 23); }   // as an operand of the MX4 conversions, which read the exponent field alone (0 = 2^-127)
+
+// 16 x 16 x 32 product of 16-bit fragments: lane l holds row l & 15, k = 8 (l >> 4) .. + 7 of either operand; result rows (first operand) 4 (l >> 4) + i, column l & 15
+template <int KIND> __device__ __forceinline__ floatx4 lin_mma16(intx4_t a, intx4_t b, floatx4 c) {
+    if constexpr (KIND == SM_F16) return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, a), __builtin_bit_cast(half8_t, b), c, 0, 0, 0);
+    else return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
+}
+// 16 x 16 x 128 product of MX4 fragments: lane l holds row l & 15 and one block of 32, with its scale byte in the low byte of sa / sb
+__device__ __forceinline__ floatx4 lin_mma4(intx4_t a, int sa, intx4_t b, int sb, floatx4 c) {
+    const intx8_t va = {a[0], a[1], a[2], a[3], 0, 0, 0, 0}, vb = {b[0], b[1], b[2], b[3], 0, 0, 0, 0};
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(va, vb, c, 4, 4, 0, sa, 0, sb);
+}

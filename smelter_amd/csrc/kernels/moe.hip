@@ -1,0 +1,255 @@
+// smelter_amd/csrc/kernels/moe.hip — routing of tokens to experts, and the weighted sum of the experts' answers.
+//
+// Route: per token the k largest of E scores (ties: the lower index first), their softmax weights, and the order of all T k assignments by expert (stable: by token, then by rank), which is what
+// the grouped products take:  offsets[e] .. offsets[e + 1] = the slots of expert e,  rows[slot] = token,  slots[token][rank] = slot.  A score of -inf or NaN is never chosen: a token with fewer
+// than k others gets expert -1, weight 0 and slot -1 for the rest, a padded token (all -inf) no slot at all.  Weights: exp(z_i - z_max) over the sum of the chosen ones (renormalised) or of all
+// E; a score that equals the maximum counts as 1, so +inf scores share the weight.  Statistics in fp32.
+//
+// The order is a counting sort in which every place is computed, none handed out by an atomic's order.  Up to SMALL assignments one block does everything in one launch; above, one launch selects
+// and counts per block, a second adds the counts of the blocks before it and places.  Bound by latency below some thousand tokens, by the reading of the scores above.
+#include "linear.hpp"
+
+#define MOE_MAX_E 1024
+#define MOE_MAX_K 32
+#define MOE_WAVES 8
+
+struct RouteParams {
+    const char* z; int type; long long T; int E, k; long long ld; int renorm;       // ld in elements
+    float* weights; int* experts; int* offsets; int* rows; int* slots; int* counts;
+    int per_block;                                                                    // tokens of a block
+};
+
+// scores as unsigned keys in their order; 0 = never chosen
+__device__ __forceinline__ unsigned route_key(float z) {
+    if (!(z > -__builtin_inff())) return 0;
+    const unsigned b = __builtin_bit_cast(unsigned, z);
+    return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float route_value(unsigned key) { return __builtin_bit_cast(float, key & 0x80000000u ? key & 0x7fffffffu : ~key); }
+__device__ __forceinline__ float route_load(const RouteParams& p, long long t, int e) {
+    const long long i = t * p.ld + e;
+    return p.type == SM_F32 ? ((const float*)p.z)[i] : p.type == SM_F16 ? (float)((const half_t*)p.z)[i] : (float)((const bf16_t*)p.z)[i];
+}
+
+// one token by one wave: lane l holds the scores of experts l, 64 + l, ...
+template <int EPL> __device__ __forceinline__ void route_token(const RouteParams& p, long long t, int* hist) {
+    const int lane = threadIdx.x & 63;
+    unsigned key[EPL];
+#pragma unroll
+    for (int j = 0; j < EPL; j++) { const int e = j * 64 + lane; float z = e < p.E ? route_load(p, t, e) : -__builtin_inff(); if (z == 0.f) z = 0.f; key[j] = route_key(z); }
+    unsigned all[EPL];
+#pragma unroll
+    for (int j = 0; j < EPL; j++) all[j] = key[j];
+    unsigned first = 0; float chosen = 0.f, mine = 0.f; int expert = -1;      // lane i < k keeps the i-th choice
+    for (int i = 0; i < p.k; i++) {
+        unsigned m = 0;
+#pragma unroll
+        for (int j = 0; j < EPL; j++) m = m > key[j] ? m : key[j];
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) { const unsigned o = __shfl_xor(m, d); m = m > o ? m : o; }
+        if (m == 0) break;
+        if (i == 0) first = m;
+        const float e1 = m == first ? 1.f : expf(route_value(m) - route_value(first));
+        chosen += e1;
+        int at = -1;
+#pragma unroll
+        for (int j = 0; j < EPL; j++) {
+            const unsigned long long hit = __ballot(at < 0 && key[j] == m);
+            if (hit) { const int l = __builtin_ctzll(hit); at = j * 64 + l; if (lane == l) key[j] = 0; }
+        }
+        if (lane == i) { mine = e1; expert = at; }
+    }
+    if (!p.renorm) {
+        float s = 0.f;
+#pragma unroll
+        for (int j = 0; j < EPL; j++) s += all[j] == 0 ? 0.f : all[j] == first ? 1.f : expf(route_value(all[j]) - route_value(first));
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) s += __shfl_xor(s, d);
+        chosen = s;
+    }
+    if (lane < p.k) {
+        p.experts[t * p.k + lane] = expert;
+        p.weights[t * p.k + lane] = expert < 0 ? 0.f : mine / chosen;
+        if (expert >= 0) atomicAdd(&hist[expert], 1);                          // a count: the same in any order
+    }
+}
+
+// Places the assignments a0 .. a1 of this block: `start[e]` = slot of the first one of expert e.  Each wave takes a run of them in order; waves before it are counted first.
+__device__ __forceinline__ void route_place(const RouteParams& p, const int* experts, long long a0, int n, int* start, int* wcount) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+    const int per = ((n + waves - 1) / waves + 63) & ~63;
+    const int lo = wave * per < n ? wave * per : n, hi = lo + per < n ? lo + per : n;
+    for (int i = threadIdx.x; i < waves * p.E; i += blockDim.x) wcount[i] = 0;
+    __syncthreads();
+    for (int i = lo + lane; i < hi; i += 64) { const int e = experts[a0 + i]; if (e >= 0) atomicAdd(&wcount[wave * p.E + e], 1); }
+    __syncthreads();
+    for (int e = threadIdx.x; e < p.E; e += blockDim.x) { int s = start[e]; for (int w = 0; w < waves; w++) { const int c = wcount[w * p.E + e]; wcount[w * p.E + e] = s; s += c; } }
+    __syncthreads();
+    const int bits = 32 - __builtin_clz(p.E);
+    for (int i0 = lo; i0 < hi; i0 += 64) {
+        const int i = i0 + lane;
+        const int e = i < hi ? experts[a0 + i] : -1;
+        unsigned long long same = __ballot(e >= 0);
+        if (e < 0) same = 0;
+        for (int b = 0; b < bits; b++) { const unsigned long long v = __ballot(e >= 0 && (e >> b & 1)); same &= (e >> b & 1) ? v : ~v; }
+        const int before = __popcll(same & ((1ull << lane) - 1));
+        int slot = -1;
+        if (e >= 0) slot = wcount[wave * p.E + e] + before;
+        __builtin_amdgcn_wave_barrier();
+        if (e >= 0 && (same >> lane) == 1ull) wcount[wave * p.E + e] = slot + 1;       // the last lane of its expert
+        __builtin_amdgcn_wave_barrier();
+        if (i < hi) { p.slots[a0 + i] = slot; if (e >= 0) p.rows[slot] = (int)((a0 + i) / p.k); }
+    }
+}
+
+// exclusive prefix sum of total[0 .. E) into offs[0 .. E] by the first wave of the block
+__device__ __forceinline__ void route_scan(const int* total, int* offs, int E) {
+    if (threadIdx.x >= 64) return;
+    int run = 0;
+    for (int base = 0; base < E; base += 64) {
+        const int e = base + threadIdx.x, v = e < E ? total[e] : 0;
+        int s = v;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) { const int up = __shfl_up(s, d); if ((int)threadIdx.x >= d) s += up; }
+        if (e < E) offs[e] = run + s - v;
+        run += __shfl(s, 63);
+    }
+    if (threadIdx.x == 0) offs[E] = run;
+}
+
+// ONE = true: the whole of a small routing in one block
+template <int EPL, bool ONE> __global__ void route_select_kernel(RouteParams p) {
+    extern __shared__ int lds[];
+    int* hist = lds;                                                             // [E]
+    const int wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+    for (int e = threadIdx.x; e < p.E; e += blockDim.x) hist[e] = 0;
+    __syncthreads();
+    const long long t0 = (long long)blockIdx.x * p.per_block, t1 = t0 + p.per_block < p.T ? t0 + p.per_block : p.T;
+    for (long long t = t0 + wave; t < t1; t += waves) route_token<EPL>(p, t, hist);
+    __syncthreads();
+    if constexpr (!ONE) { for (int e = threadIdx.x; e < p.E; e += blockDim.x) p.counts[(long long)blockIdx.x * p.E + e] = hist[e]; }
+    else {
+        int* offs = lds + p.E; int* wcount = offs + p.E + 1;
+        route_scan(hist, offs, p.E);
+        __threadfence_block();
+        __syncthreads();
+        for (int e = threadIdx.x; e <= p.E; e += blockDim.x) p.offsets[e] = offs[e];
+        const int used = offs[p.E], n = (int)(p.T * p.k);
+        for (int i = used + threadIdx.x; i < n; i += blockDim.x) p.rows[i] = -1;
+        route_place(p, p.experts, 0, n, offs, wcount);
+    }
+}
+
+__global__ void route_place_kernel(RouteParams p, int blocks) {
+    extern __shared__ int lds[];
+    int* total = lds; int* before = total + p.E; int* offs = before + p.E; int* wcount = offs + p.E + 1;
+    for (int e = threadIdx.x; e < 2 * p.E; e += blockDim.x) lds[e] = 0;
+    __syncthreads();
+    // counts of all blocks and of the blocks before this one; integer sums, the same in any order
+    for (long long i = threadIdx.x; i < (long long)blocks * p.E; i += blockDim.x) {
+        const int b = (int)(i / p.E), e = (int)(i - (long long)b * p.E), c = p.counts[i];
+        if (c) { atomicAdd(&total[e], c); if (b < (int)blockIdx.x) atomicAdd(&before[e], c); }
+    }
+    __syncthreads();
+    route_scan(total, offs, p.E);
+    __syncthreads();
+    const int used = offs[p.E];
+    if (blockIdx.x == 0) for (int e = threadIdx.x; e <= p.E; e += blockDim.x) p.offsets[e] = offs[e];
+    for (long long i = used + (long long)blockIdx.x * blockDim.x + threadIdx.x; i < p.T * p.k; i += (long long)gridDim.x * blockDim.x) p.rows[i] = -1;
+    __syncthreads();
+    for (int e = threadIdx.x; e < p.E; e += blockDim.x) before[e] += offs[e];
+    __syncthreads();
+    const long long t0 = (long long)blockIdx.x * p.per_block, t1 = t0 + p.per_block < p.T ? t0 + p.per_block : p.T;
+    route_place(p, p.experts, t0 * p.k, (int)((t1 - t0) * p.k), before, wcount);
+}
+
+#define ROUTE_SMALL 64                                                            // tokens
+
+static long long route_blocks(long long T, int* per) {
+    long long b = (T + 63) / 64; if (b > 512) b = 512;
+    *per = (int)((T + b - 1) / b);
+    return (T + *per - 1) / *per;
+}
+
+extern "C" size_t sm_moe_route_workspace_bytes(int64_t T, int32_t E, int32_t k) {
+    if (T <= ROUTE_SMALL || E < 1) return 0;
+    int per; return (size_t)route_blocks(T, &per) * E * sizeof(int);
+}
+
+template <int EPL> static int route_launch(RouteParams p, hipStream_t s) {
+    const size_t place = (size_t)(MOE_WAVES * p.E + p.E + 1) * sizeof(int);
+    if (p.T <= ROUTE_SMALL) {
+        p.per_block = (int)p.T;
+        route_select_kernel<EPL, true><<<1, 64 * MOE_WAVES, p.E * sizeof(int) + place, s>>>(p);
+    } else {
+        const long long blocks = route_blocks(p.T, &p.per_block);
+        route_select_kernel<EPL, false><<<dim3((unsigned)blocks), 64 * MOE_WAVES, p.E * sizeof(int), s>>>(p);
+        SM_LAUNCH_CHECK();
+        route_place_kernel<<<dim3((unsigned)blocks), 64 * MOE_WAVES, 2 * p.E * sizeof(int) + place, s>>>(p, (int)blocks);
+    }
+    SM_LAUNCH_CHECK();
+    return SM_OK;
+}
+
+extern "C" int sm_moe_route(const void* scores, int32_t type, int64_t T, int32_t E, int32_t k, int64_t ld, int32_t renormalize, float* weights, int32_t* experts, int32_t* offsets,
+                            int32_t* rows, int32_t* slots, void* workspace, size_t workspace_bytes, sm_stream_t stream) {
+    SM_REQUIRE(type == SM_F16 || type == SM_BF16 || type == SM_F32, "moe_route: type %d is not fp16, bf16 or fp32", type);
+    SM_REQUIRE(E >= 1 && E <= MOE_MAX_E, "moe_route: %d experts (taken: 1 .. %d)", E, MOE_MAX_E);
+    SM_REQUIRE(k >= 1 && k <= MOE_MAX_K && k <= E, "moe_route: %d of %d experts (taken: 1 .. min(%d, E))", k, E, MOE_MAX_K);
+    SM_REQUIRE(T >= 0 && T * k < (1ll << 31), "moe_route: %lld tokens x %d", (long long)T, k);
+    SM_REQUIRE(offsets && (T == 0 || (scores && weights && experts && rows && slots)), "moe_route: null operand");
+    SM_REQUIRE(T <= 1 || ld >= E, "moe_route: row stride %lld below the %d scores", (long long)ld, E);
+    SM_REQUIRE((size_t)scores % (type == SM_F32 ? 4 : 2) == 0, "moe_route: scores are not aligned to their element");
+    SM_REQUIRE(workspace_bytes >= sm_moe_route_workspace_bytes(T, E, k) && (workspace || T <= ROUTE_SMALL) && (size_t)workspace % 4 == 0, "moe_route: workspace of %zu bytes, %zu wanted",
+               workspace_bytes, sm_moe_route_workspace_bytes(T, E, k));
+    RouteParams p = {};
+    p.z = (const char*)scores; p.type = type; p.T = T; p.E = E; p.k = k; p.ld = ld; p.renorm = renormalize;
+    p.weights = weights; p.experts = experts; p.offsets = offsets; p.rows = rows; p.slots = slots; p.counts = (int*)workspace;
+    hipStream_t s = sm_s(stream);
+    if (E <= 64) return route_launch<1>(p, s);
+    if (E <= 128) return route_launch<2>(p, s);
+    if (E <= 256) return route_launch<4>(p, s);
+    return route_launch<16>(p, s);
+}
+
+// out[t, n] = sum_j weights[t, j] * y[slots[t, j], n]: one thread per eight columns of a token, terms added in the order of j in fp32, one rounding; a slot outside 0 .. M - 1 adds nothing.
+// Bound by the reading of the k rows.
+template <int KIND> __global__ void combine_kernel(const char* y, long long M, int N, long long y_ld, const float* weights, const int* slots, long long T, int k, void* out, long long out_ld, int vec) {
+    const int chunks = (N + 7) / 8;
+    const long long units = T * chunks;
+    for (long long u = (long long)blockIdx.x * blockDim.x + threadIdx.x; u < units; u += (long long)gridDim.x * blockDim.x) {
+        const long long t = u < 0x7fffffffll ? (long long)((unsigned)u / (unsigned)chunks) : u / chunks;
+        const int c = (int)(u - t * chunks) * 8;
+        float s[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+        for (int j = 0; j < k; j++) {
+            const int at = slots[t * k + j];
+            if (at < 0 || at >= M) continue;
+            const float w = weights[t * k + j];
+            const intx4_t v = lin_load8(y + 2ll * at * y_ld, c, N);
+            if constexpr (KIND == SM_F16) { const half8_t h = __builtin_bit_cast(half8_t, v); for (int i = 0; i < 8; i++) s[i] += w * (float)h[i]; }
+            else { const bf16x8_t h = __builtin_bit_cast(bf16x8_t, v); for (int i = 0; i < 8; i++) s[i] += w * (float)h[i]; }
+        }
+        const long long o = t * out_ld + c;
+        if (vec && c + 8 <= N) {
+            if constexpr (KIND == SM_F16) { half8_t h; for (int i = 0; i < 8; i++) h[i] = (half_t)s[i]; *(half8_t*)((half_t*)out + o) = h; }
+            else { bf16x8_t h; for (int i = 0; i < 8; i++) h[i] = (bf16_t)s[i]; *(bf16x8_t*)((bf16_t*)out + o) = h; }
+        } else for (int i = 0; i < 8; i++) if (c + i < N) lin_store1(out, o + i, s[i], KIND);
+    }
+}
+
+extern "C" int sm_moe_combine(const void* y, int32_t type, int64_t M, int32_t N, int64_t y_ld, const float* weights, const int32_t* slots, int64_t T, int32_t k, void* out, int64_t out_ld,
+                              sm_stream_t stream) {
+    SM_REQUIRE(type == SM_F16 || type == SM_BF16, "moe_combine: type %d is not fp16 or bf16", type);
+    SM_REQUIRE(M >= 0 && N >= 0 && T >= 0 && k >= 0 && M < (1ll << 31) && T < (1ll << 31) && N <= (1 << 29), "moe_combine: sizes M %lld, N %d, T %lld, k %d", (long long)M, N, (long long)T, k);
+    if (T == 0 || N == 0) return SM_OK;
+    SM_REQUIRE(out && (k == 0 || (weights && slots)) && (k == 0 || M == 0 || y), "moe_combine: null operand");
+    SM_REQUIRE((M <= 1 || y_ld >= N) && (T == 1 || out_ld >= N), "moe_combine: row strides %lld, %lld below the %d columns", (long long)y_ld, (long long)out_ld, N);
+    SM_REQUIRE((size_t)y % 2 == 0 && (size_t)out % 2 == 0, "moe_combine: an operand is not aligned to its element");
+    const int vec = (size_t)out % 16 == 0 && (T == 1 || out_ld % 8 == 0);
+    const long long units = T * ((N + 7) / 8), want = (units + 255) / 256, cap = (long long)SM_NUM_CU * 32;
+    const dim3 grid((unsigned)(want < cap ? want : cap));
+    if (type == SM_F16) combine_kernel<SM_F16><<<grid, 256, 0, sm_s(stream)>>>((const char*)y, M, N, y_ld, weights, slots, T, k, out, out_ld, vec);
+    else combine_kernel<SM_BF16><<<grid, 256, 0, sm_s(stream)>>>((const char*)y, M, N, y_ld, weights, slots, T, k, out, out_ld, vec);
+    SM_LAUNCH_CHECK();
+    return SM_OK;
+}

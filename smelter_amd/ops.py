@@ -7,10 +7,11 @@ whose pixel stride is passed as `ld`); conv weights are OHWI fp16; bias fp32.
 from __future__ import annotations
 
 import ctypes as C
+from typing import NamedTuple
 
 import torch
 
-from ._native import ConvDesc, PoolDesc, StagePhase, check, lib
+from ._native import ConvDesc, LinearDesc, PoolDesc, SmelterError, StagePhase, check, lib
 
 ACT_NONE, ACT_RELU, ACT_PRELU, ACT_CLIP = 0, 1, 2, 12
 
@@ -526,3 +527,219 @@ def mbconv_stem(x_nchw, w_stem_ohwi, b_stem, wd, bd, w2, b2, st_stride=2, st_pad
     check(lib().sm_mbconv_stem_fwd(C.byref(d), _ptr(x_nchw), c, ih, iw, st_stride, st_pad, _ptr(w_stem_ohwi), _ptr(b_stem), _ptr(wd), _ptr(bd), _ptr(w2), _ptr(b2),
                                    _ptr(y), _stream()))
     return y
+
+
+# ---- linear layers with 4-bit weights, and expert layers ---------------------------------------------------------------------------------------
+# fp16 / bf16 row-major tensors [rows, K] instead of NHWC; arguments that do not fit raise SmelterError (invalidArgument) before anything is launched.  The work goes to the
+# current stream of the tensors' own device, whichever device is current.
+
+_TYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
+_MX4 = 3
+
+
+class Mx4(NamedTuple):
+    """An MX4 tensor [..., k]: blocks of 32 e2m1 elements along the last axis with an e8m0 scale each.  codes: uint8 [..., 16 * ceil(k / 32)] (the even column in the low nibble),
+    scales: uint8 [..., ceil(k / 32)] (2^(byte - 127), 255 = NaN); both contiguous, codes 16-byte aligned."""
+    codes: torch.Tensor
+    scales: torch.Tensor
+    k: int
+
+    @property
+    def shape(self):
+        return (*self.codes.shape[:-1], self.k)
+
+
+class MoePlan(NamedTuple):
+    """What moe_route returns.  weights fp32 [T, k], experts int32 [T, k] (-1: none), offsets int32 [E + 1], rows int32 [T * k] (slot -> token, -1 behind offsets[E]), slots int32 [T, k]
+    (assignment -> slot, -1: none)"""
+    weights: torch.Tensor
+    experts: torch.Tensor
+    offsets: torch.Tensor
+    rows: torch.Tensor
+    slots: torch.Tensor
+
+
+def _require(cond, msg, *args):
+    if not cond:
+        raise SmelterError(-13, msg % args)
+
+
+def _on(dev, call, *args):
+    """run an enqueueing entry point on the current stream of `dev`"""
+    if dev.index == torch.cuda.current_device():
+        check(call(*args, torch.cuda.current_stream(dev).cuda_stream))
+    else:
+        with torch.cuda.device(dev):
+            check(call(*args, torch.cuda.current_stream(dev).cuda_stream))
+
+
+def _rows2d(t, name):
+    """(rows, columns, row stride) of a tensor [..., K] whose leading axes are evenly strided"""
+    _require(t.dim() >= 1, "%s: a tensor with at least one axis is wanted", name)
+    k = t.shape[-1]
+    n = t.numel() // k if k else 0
+    if n <= 1 or k == 0:
+        _require(k <= 1 or t.stride(-1) == 1, "%s: the last axis must be innermost", name)
+        return n, k, k
+    if t.is_contiguous():
+        return n, k, k
+    _require(t.stride(-1) == 1 or k == 1, "%s: the last axis must be innermost", name)
+    ld, step = None, None
+    for size, stride in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
+        if size == 1:
+            continue
+        if ld is None:
+            ld, step = stride, size * stride
+        else:
+            _require(stride == step, "%s: the leading axes must be evenly strided", name)
+            step *= size
+    _require(ld >= k, "%s: rows overlap (stride %d, %d columns)", name, ld, k)
+    return n, k, ld
+
+
+def _gpu(dev, name, t, dtypes):
+    _require(isinstance(t, torch.Tensor) and t.is_cuda and (dev is None or t.device == dev), "%s: a tensor on %s is wanted", name, dev or "the GPU")
+    _require(t.dtype in dtypes, "%s: type %s is not taken", name, t.dtype)
+
+
+def _check_mx4(q, dev, name):
+    _require(isinstance(q, Mx4), "%s: an Mx4 tensor is wanted", name)
+    _gpu(dev, name, q.codes, (torch.uint8,))
+    _gpu(q.codes.device, name, q.scales, (torch.uint8,))
+    nb = (q.k + 31) // 32
+    _require(q.k >= 0 and q.codes.dim() >= 1 and q.codes.shape == (*q.scales.shape[:-1], 16 * nb) and q.scales.shape[-1] == nb, "%s: codes %s and scales %s for %d columns", name,
+             tuple(q.codes.shape), tuple(q.scales.shape), q.k)
+    _require(q.codes.is_contiguous() and q.scales.is_contiguous() and q.codes.data_ptr() % 16 == 0, "%s: codes and scales must be contiguous, codes 16-byte aligned", name)
+
+
+def mx4_quantize(x):
+    """fp16 / bf16 / fp32 [..., K] -> Mx4 (sm_mx4_quantize): blocks of 32 along the last axis, scale 2^(floor(log2 amax) - 2), elements to the nearest e2m1 value, ties to even, at most 6 scales.
+    A block with a NaN or an infinity becomes NaN."""
+    _gpu(None, "mx4_quantize", x, _TYPES)
+    rows, k, ld = _rows2d(x, "mx4_quantize")
+    nb = (k + 31) // 32
+    codes = torch.empty((*x.shape[:-1], 16 * nb), dtype=torch.uint8, device=x.device)
+    scales = torch.empty((*x.shape[:-1], nb), dtype=torch.uint8, device=x.device)
+    _on(x.device, lib().sm_mx4_quantize, x.data_ptr(), _TYPES[x.dtype], rows, k, ld, codes.data_ptr(), scales.data_ptr())
+    return Mx4(codes, scales, k)
+
+
+def mx4_dequantize(q, dtype=torch.float16, out=None):
+    """the values of an Mx4 tensor, rounded once to `dtype` (sm_mx4_dequantize)"""
+    _check_mx4(q, None, "mx4_dequantize")
+    if out is None:
+        _require(dtype in _TYPES, "mx4_dequantize: type %s is not taken", dtype)
+        out = torch.empty(q.shape, dtype=dtype, device=q.codes.device)
+    _gpu(q.codes.device, "mx4_dequantize", out, _TYPES)
+    _require(tuple(out.shape) == tuple(q.shape), "mx4_dequantize: output %s for %s", tuple(out.shape), tuple(q.shape))
+    rows, k, ld = _rows2d(out, "mx4_dequantize")
+    _on(out.device, lib().sm_mx4_dequantize, q.codes.data_ptr(), q.scales.data_ptr(), rows, k, out.data_ptr(), _TYPES[out.dtype], ld)
+    return out
+
+
+def _linear(name, x, w, lead, m, offsets, rows, bias, act, slope, gated, out, dtype):
+    """the checks and the call that mx4_linear and expert_linear share; `lead` = leading axes of the weights (() or (E,)), m = slots (None: one per row of x)"""
+    x4 = isinstance(x, Mx4)
+    xt = x.codes if x4 else x
+    if x4:
+        _check_mx4(x, None, name)
+        xk, x_ld = x.k, 0
+        _require(len(x.shape) == 2, "%s: x must be [rows, K]", name)
+    else:
+        _gpu(None, name, x, (torch.float16, torch.bfloat16))
+        _require(x.dim() == 2, "%s: x must be [rows, K]", name)
+        _, xk, x_ld = _rows2d(x, name)
+    dev = xt.device
+    if isinstance(w, Mx4):
+        _check_mx4(w, dev, name)
+        w_type, wc, wsc = _MX4, w.codes, w.scales.data_ptr()
+    else:
+        _gpu(dev, name, w, (torch.float16, torch.bfloat16))
+        _require(not x4 and w.dtype == x.dtype, "%s: weights of type %s under x of type %s", name, w.dtype, "MX4" if x4 else x.dtype)
+        _require(w.is_contiguous(), "%s: weights must be contiguous", name)
+        w_type, wc, wsc = _TYPES[w.dtype], w, None
+    ws = w.shape
+    _require(len(ws) == lead + 2 and ws[-1] == xk, "%s: weights %s for x with %d columns", name, tuple(ws), xk)
+    t, n, e = xt.shape[0], ws[-2], ws[0] if lead else 1
+    if gated:
+        _require(n % 2 == 0, "%s: a gated layer has an even number of weight rows (%d)", name, n)
+        n //= 2
+    if m is None:
+        m = t
+    if out is None:
+        dtype = dtype or (torch.float16 if x4 else x.dtype)
+        _require(dtype in _TYPES, "%s: output type %s is not taken", name, dtype)
+        out = torch.empty((m, n), dtype=dtype, device=dev)
+    else:
+        _gpu(dev, name, out, _TYPES)
+        _require(dtype is None or dtype == out.dtype, "%s: out is %s, dtype %s", name, out.dtype, dtype)
+        _require(out.shape == (m, n), "%s: output %s, wanted %s", name, tuple(out.shape), (m, n))
+    y_ld = n if out.is_contiguous() else _rows2d(out, name)[2]
+    if bias is not None:
+        _gpu(dev, name, bias, (torch.float32,))
+        _require(bias.is_contiguous() and bias.shape == ws[:-1], "%s: bias %s for weights %s", name, tuple(bias.shape), tuple(ws))
+    d = LinearDesc(m, t, n, xk, e, _MX4 if x4 else _TYPES[x.dtype], w_type, _TYPES[out.dtype], act, slope, 1 if gated else 0, x_ld, y_ld)
+    _on(dev, lib().sm_linear_fwd, C.byref(d), xt.data_ptr(), x.scales.data_ptr() if x4 else None, wc.data_ptr(), wsc, bias.data_ptr() if bias is not None else None,
+        offsets.data_ptr() if offsets is not None else None, rows.data_ptr() if rows is not None else None, out.data_ptr())
+    return out
+
+
+def mx4_linear(x, w, bias=None, act=ACT_NONE, slope=0.0, gated=False, out=None, dtype=None):
+    """act(x . w^T + bias) with MX4 weights w [N, K] (sm_linear_fwd).  x [M, K]: fp16 or bf16 (the weights are read as 16-bit values, the output has x's type or fp32), or an Mx4 tensor (both
+    sides in 4 bits; dtype fp16 (default), bf16 or fp32).  gated: w has 2 N rows and the result is silu(first N columns) * last N.  bias fp32 [rows of w]."""
+    _require(isinstance(w, Mx4), "mx4_linear: the weights must be an Mx4 tensor")
+    return _linear("mx4_linear", x, w, 0, None, None, None, bias, act, slope, gated, out, dtype)
+
+
+def expert_linear(x, w, offsets, rows=None, bias=None, act=ACT_NONE, slope=0.0, gated=False, out=None, dtype=None):
+    """Products grouped by expert (sm_linear_fwd): slot s of group e (offsets[e] <= s < offsets[e + 1]) gets act(x[rows[s]] . w[e]^T + bias[e]); without `rows` slot s is row s of x.
+    x [T, K] and w [E, N, K]: both fp16, both bf16, 16-bit x on Mx4 weights, or both Mx4.  offsets int32 [E + 1], rows int32 [slots], both on the GPU (MoePlan holds them): nothing is
+    read back to the host.  Slots that no group covers are left as they were (in a new `out`: unspecified).  gated, bias [E, rows of w], dtype: as in mx4_linear."""
+    dev = x.codes.device if isinstance(x, Mx4) else x.device
+    _gpu(dev, "expert_linear", offsets, (torch.int32,))
+    e = w.codes.shape[0] if isinstance(w, Mx4) else w.shape[0]
+    _require(offsets.is_contiguous() and offsets.shape == (e + 1,) and e >= 1, "expert_linear: offsets %s for %d experts", tuple(offsets.shape), e)
+    m = None
+    if rows is not None:
+        _gpu(dev, "expert_linear", rows, (torch.int32,))
+        _require(rows.dim() == 1 and rows.is_contiguous(), "expert_linear: rows must be a contiguous vector")
+        m = rows.shape[0]
+    return _linear("expert_linear", x, w, 1, m, offsets, rows, bias, act, slope, gated, out, dtype)
+
+
+def moe_route(scores, k, renormalize=True):
+    """The k largest of each token's scores [T, E] (fp16 / bf16 / fp32; ties: the lower index), their softmax weights (over the chosen ones, or over all E) and the order of the assignments
+    by expert (sm_moe_route) -> MoePlan.  A score of -inf or NaN is never chosen."""
+    _gpu(None, "moe_route", scores, _TYPES)
+    _require(scores.dim() == 2, "moe_route: scores must be [tokens, experts]")
+    t, e = scores.shape
+    _require(1 <= e <= 1024 and 1 <= k <= min(e, 32), "moe_route: %d of %d experts (taken: up to 1024 experts, 1 .. min(32, experts) of them)", k, e)
+    ld = e if scores.is_contiguous() else _rows2d(scores, "moe_route")[2]
+    dev, n, ws = scores.device, t * k, lib().sm_moe_route_workspace_bytes(t, e, k)
+    weights = torch.empty((t, k), dtype=torch.float32, device=dev)
+    ints = torch.empty((3 * n + e + 1 + ws // 4,), dtype=torch.int32, device=dev)      # one allocation; the workspace behind the results
+    experts, slots, rows, offsets, work = ints[:n].view(t, k), ints[n:2 * n].view(t, k), ints[2 * n:3 * n], ints[3 * n:3 * n + e + 1], ints[3 * n + e + 1:]
+    _on(dev, lib().sm_moe_route, scores.data_ptr(), _TYPES[scores.dtype], t, e, k, ld, 1 if renormalize else 0, weights.data_ptr(), experts.data_ptr(), offsets.data_ptr(), rows.data_ptr(),
+        slots.data_ptr(), work.data_ptr(), ws)
+    return MoePlan(weights, experts, offsets, rows, slots)
+
+
+def moe_combine(y, slots, weights, out=None):
+    """out[t] = sum_j weights[t, j] * y[slots[t, j]] (sm_moe_combine): y fp16 / bf16 [M, N], slots int32 [T, k] (negative: nothing), weights fp32 [T, k]; fp32 sums in the order of j"""
+    _gpu(None, "moe_combine", y, (torch.float16, torch.bfloat16))
+    dev = y.device
+    _gpu(dev, "moe_combine", slots, (torch.int32,))
+    _gpu(dev, "moe_combine", weights, (torch.float32,))
+    _require(y.dim() == 2 and slots.dim() == 2 and slots.shape == weights.shape and slots.is_contiguous() and weights.is_contiguous(), "moe_combine: y %s, slots %s, weights %s",
+             tuple(y.shape), tuple(slots.shape), tuple(weights.shape))
+    m, n = y.shape
+    t, k = slots.shape
+    if out is None:
+        out = torch.empty((t, n), dtype=y.dtype, device=dev)
+    else:
+        _gpu(dev, "moe_combine", out, (y.dtype,))
+        _require(out.shape == (t, n), "moe_combine: output %s, wanted %s", tuple(out.shape), (t, n))
+    y_ld = n if y.is_contiguous() else _rows2d(y, "moe_combine")[2]
+    o_ld = n if out.is_contiguous() else _rows2d(out, "moe_combine")[2]
+    _on(dev, lib().sm_moe_combine, y.data_ptr(), _TYPES[y.dtype], m, n, y_ld, weights.data_ptr(), slots.data_ptr(), t, k, out.data_ptr(), o_ld)
+    return out

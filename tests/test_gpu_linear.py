@@ -1,0 +1,457 @@
+"""4-bit (MX4) tensors, linear layers on them, expert layers and their routing, against plain 64-bit forms (tests/mx4ref.py)."""
+import pytest
+import torch
+
+import mx4ref
+from smelter_amd import _native as N
+from smelter_amd import ops
+
+pytestmark = pytest.mark.gpu
+F16, BF16, F32 = torch.float16, torch.bfloat16, torch.float32
+INF, NAN = float("inf"), float("nan")
+
+
+def gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def randn(g, *shape, scale=1.0):
+    return torch.randn(shape, generator=g) * scale
+
+
+def mx4(w):
+    c, s = mx4ref.pack(w)
+    return ops.Mx4(c.cuda(), s.cuda(), w.shape[-1])
+
+
+def val(q):
+    return mx4ref.unpack(q.codes, q.scales, q.k)
+
+
+# ---- packing ------------------------------------------------------------------------------------------------------------------------------
+
+
+def same_pack(x):
+    q = ops.mx4_quantize(x.cuda())
+    c, s = mx4ref.pack(x)
+    assert torch.equal(q.scales.cpu(), s) and torch.equal(q.codes.cpu(), c) and q.k == x.shape[-1] and q.shape == tuple(x.shape)
+    return q
+
+
+@pytest.mark.parametrize("t", [F16, BF16, F32])
+@pytest.mark.parametrize("rows, k", [(1, 1), (1, 31), (3, 32), (2, 33), (5, 100), (1, 2048), (257, 72), (0, 64), (4, 0)])
+def test_quantize_sizes(t, rows, k):
+    same_pack(randn(gen(rows + k), rows, k).to(t))
+
+
+@pytest.mark.parametrize("t", [F16, BF16])
+def test_quantize_every_pattern(t):
+    """every 16-bit pattern once as the largest of its block (beside smaller ones), and among neighbours in value"""
+    x = torch.arange(-32768, 32768, dtype=torch.int32).to(torch.int16).view(t)
+    same_pack(x.view(-1, 32))
+    fine = x[torch.isfinite(x.float())]
+    f = fine.double()
+    block = torch.stack([(f * m).to(t) for m in (1, 0.5, -0.25, 0.3125, 0.4375, -0.625, 0.875, 0.03125)], 1)
+    same_pack(torch.where(torch.isfinite(block.float()), block, torch.zeros_like(block)))
+
+
+def test_quantize_fp32_extremes():
+    x = torch.tensor([[0.0, -0.0, 1e-45, -1e-45], [1e-38, 1.1754944e-38, -5e-39, 3e-39], [3.4028235e38, -3.4028235e38, 1e30, 2.0], [INF, 1, 2, 3], [-INF, 0, 0, 0], [NAN, INF, 1, 0], [6.0, 5.0, 3.5, 2.5]])
+    same_pack(x)
+
+
+@pytest.mark.parametrize("t", [F16, F32])
+def test_quantize_strides_and_leading_axes(t):
+    big = randn(gen(3), 6, 4, 130).to(t)
+    same_pack(big)
+    g = big.cuda()
+    for v in (g[..., :70], g[:, 1], g[..., 3:40], g[:2, :1, 5:6]):
+        q = ops.mx4_quantize(v)
+        c, s = mx4ref.pack(v.cpu())
+        assert torch.equal(q.codes.cpu(), c) and torch.equal(q.scales.cpu(), s)
+    with pytest.raises(N.SmelterError):
+        ops.mx4_quantize(g.transpose(0, 2))
+
+
+@pytest.mark.parametrize("t", [F16, BF16, F32])
+@pytest.mark.parametrize("rows, k", [(1, 1), (3, 33), (9, 70), (2, 256), (300, 40)])
+def test_dequantize(t, rows, k):
+    """exact: every value of these scales is representable in all three types"""
+    g = gen(k)
+    q = mx4(randn(g, rows, k))
+    assert torch.equal(ops.mx4_dequantize(q, t).cpu().double(), val(q))
+    wide = torch.full((rows, k + 9), 7.0, dtype=t, device="cuda")
+    ops.mx4_dequantize(q, out=wide[:, 1:k + 1])
+    assert torch.equal(wide[:, 1:k + 1].cpu().double(), val(q)) and wide[:, 0].eq(7).all() and wide[:, k + 1:].eq(7).all()
+
+
+@pytest.mark.parametrize("t", [F16, BF16, F32])
+def test_dequantize_every_scale(t):
+    codes = torch.arange(256, dtype=torch.uint8).view(1, 16, 16).repeat(256, 1, 1).reshape(256, 256)
+    scales = torch.arange(256).to(torch.uint8).view(256, 1).repeat(1, 16)
+    got = ops.mx4_dequantize(ops.Mx4(codes.cuda(), scales.cuda(), 512), t).cpu()
+    want = mx4ref.unpack(codes, scales, 512).to(t)                      # one rounding: to nearest even, to an infinity above the range
+    assert torch.equal(torch.isnan(got), torch.isnan(want)) and torch.equal(got[:255], want[:255])
+
+
+# ---- products -----------------------------------------------------------------------------------------------------------------------------
+
+KINDS = ["f16", "bf16", "f16-mx4", "bf16-mx4", "mx4-mx4"]
+
+
+def operands(kind, g, t, k, wshape, spread=False):
+    """(x as handed over, its fp64 values, w as handed over, its fp64 values, type of the output)"""
+    dt = BF16 if kind.startswith("bf16") else F16
+    x = randn(g, t, k).to(dt)
+    w = randn(g, *wshape, scale=max(k, 1) ** -0.5)
+    if kind == "mx4-mx4":
+        qx, qw = mx4(x), mx4(w)
+        return qx, val(qx), qw, val(qw), dt
+    if kind.endswith("mx4"):
+        qw = mx4(w)
+        return x.cuda(), x.double(), qw, val(qw), dt
+    w = w.to(dt)
+    return x.cuda(), x.double(), w.cuda(), w.double(), dt
+
+
+@pytest.mark.parametrize("kind", ["f16-mx4", "bf16-mx4", "mx4-mx4"])
+@pytest.mark.parametrize("m", [1, 2, 15, 16, 17, 33, 64, 65, 129, 260, 530])
+@pytest.mark.parametrize("n, k", [(1, 1), (33, 40), (100, 129), (256, 512), (72, 1000), (300, 2088)])
+def test_mx4_linear(kind, m, n, k):
+    g = gen(m * 1000 + n + k)
+    x, xv, w, wv, dt = operands(kind, g, m, k, (n, k))
+    bias = randn(g, n)
+    want, err = mx4ref.linear(xv, wv, bias)
+    mx4ref.close(ops.mx4_linear(x, w, bias.cuda(), dtype=dt), want, err)
+    mx4ref.close(ops.mx4_linear(x, w, dtype=F32), *mx4ref.linear(xv, wv))
+
+
+@pytest.mark.parametrize("kind", ["f16-mx4", "bf16-mx4", "mx4-mx4"])
+@pytest.mark.parametrize("m, n, k", [(1, 1, 32), (3, 17, 64), (70, 40, 100), (150, 128, 256), (300, 264, 328)])
+def test_mx4_linear_gated(kind, m, n, k):
+    g = gen(m + n + k)
+    x, xv, w, wv, dt = operands(kind, g, m, k, (2 * n, k))
+    bias = randn(g, 2 * n)
+    mx4ref.close(ops.mx4_linear(x, w, bias.cuda(), gated=True, dtype=dt), *mx4ref.linear(xv, wv, bias, gated=True))
+
+
+@pytest.mark.parametrize("act, slope, f", [(ops.ACT_RELU, 0.0, lambda z: z.clamp(min=0)), (ops.ACT_PRELU, 0.25, lambda z: torch.where(z < 0, 0.25 * z, z)),
+                                           (ops.ACT_CLIP, 0.5, lambda z: z.clamp(0, 0.5)), (ops.ACT_CODES["sigmoid"], 0.0, torch.sigmoid)])
+@pytest.mark.parametrize("m", [3, 200])
+def test_mx4_linear_activations(act, slope, f, m):
+    """all four have slopes of at most 1 and are computed in fp32 with a relative error below 2^-20 of values of at most 1 (sigmoid), or exactly"""
+    x, xv, w, wv, dt = operands("f16-mx4", gen(m), m, 96, (136, 96))
+    want, err = mx4ref.linear(xv, wv, act=f)
+    mx4ref.close(ops.mx4_linear(x, w, act=act, slope=slope), want, err + 2.0 ** -20)
+
+
+@pytest.mark.parametrize("kind", ["f16-mx4", "bf16-mx4"])
+@pytest.mark.parametrize("m", [4, 200])
+def test_mx4_linear_wide_scales(kind, m):
+    """block scales over 2^60 of each other, rows of tiny weights, a row of zeros, one NaN block"""
+    g = gen(5)
+    k = 640
+    w = randn(g, 70, k)
+    w = w * torch.exp2(torch.randint(-30, 30, (70, k // 32), generator=g).float()).repeat_interleave(32, 1)
+    w[1] *= 2.0 ** -60
+    w[2] = 0
+    w[3] = randn(g, k) * 2.0 ** -100
+    w[4, 33] = NAN
+    q = mx4(w)
+    x = randn(g, m, k).to(F16 if kind == "f16-mx4" else BF16)
+    got = ops.mx4_linear(x.cuda(), q, dtype=F32).cpu()
+    mx4ref.close(got, *mx4ref.linear(x, val(q)))
+    assert got[:, 4].isnan().all() and got[:, 2].eq(0).all() and got[:, 3].ne(0).all()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("m", [5, 150])
+def test_memory_beside_the_operands(kind, m):
+    """NaN behind every row of x, an output with a stride and neighbours that stay, an x that is aligned to its element only"""
+    g = gen(m)
+    n, k = 45, 88
+    x, xv, w, wv, dt = operands(kind, g, m, k, (1, n, k))
+    if kind != "mx4-mx4":
+        wide = torch.full((m, k + 13), NAN, dtype=dt, device="cuda")
+        wide[:, 3:k + 3] = x
+        x = wide[:, 3:k + 3]
+    out = torch.full((m + 2, n + 7), 7.0, dtype=dt, device="cuda")
+    off = torch.tensor([0, m], dtype=torch.int32, device="cuda")
+    ops.expert_linear(x, w, off, out=out[1:m + 1, 2:n + 2])
+    mx4ref.close(out[1:m + 1, 2:n + 2], *mx4ref.linear(xv, wv[0]))
+    out[1:m + 1, 2:n + 2] = 7
+    assert out.eq(7).all()
+
+
+def grouped(xv, wv, offsets, rows, bias=None, gated=False, m=None):
+    m = len(rows) if rows is not None else xv.shape[0]
+    n = wv.shape[1] // (2 if gated else 1)
+    want, err = torch.full((m, n), 7.0, dtype=torch.float64), torch.zeros(m, n, dtype=torch.float64)
+    for e in range(len(offsets) - 1):
+        s = torch.arange(offsets[e], offsets[e + 1])
+        at = torch.as_tensor(rows)[s].long() if rows is not None else s
+        ok = (at >= 0) & (at < xv.shape[0])
+        x = torch.where(ok[:, None], xv[at.clamp(0, max(xv.shape[0] - 1, 0))], torch.zeros(1, dtype=torch.float64))
+        want[s], err[s] = mx4ref.linear(x, wv[e], None if bias is None else bias[e], gated=gated)
+    return want, err
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("sizes, n, k, gather", [([1], 24, 32, False), ([0, 3, 0, 1, 17, 0], 40, 64, True), ([5] * 70 + [0, 16, 40], 19, 96, True), ([130, 0, 1, 300, 64], 136, 136, True),
+                                                 ([0, 0], 8, 32, False), ([257, 255, 256, 1], 264, 200, False), ([33, 31, 700], 64, 77, True)])
+def test_expert_linear(kind, gated, sizes, n, k, gather):
+    g = gen(sum(sizes) + n + k + gated)
+    m, e = sum(sizes), len(sizes)
+    t = m // 2 + 1 if gather else m
+    x, xv, w, wv, dt = operands(kind, g, t, k, (e, 2 * n if gated else n, k))
+    off = torch.tensor([0] + sizes).cumsum(0).tolist()
+    rows = torch.randint(0, t, (m,), generator=g).tolist() if gather else None
+    bias = randn(g, e, 2 * n if gated else n)
+    out = torch.full((m + 3, n), 7.0, dtype=dt, device="cuda")
+    if gather:                                                         # slots behind the last group stay as they were
+        got = ops.expert_linear(x, w, torch.tensor(off, dtype=torch.int32, device="cuda"), torch.tensor(rows + [0, -1, t], dtype=torch.int32, device="cuda"), bias.cuda(), gated=gated, out=out)
+        assert got is out and out[m:].eq(7).all()
+        got = out[:m]
+    else:
+        got = ops.expert_linear(x, w, torch.tensor(off, dtype=torch.int32, device="cuda"), bias=bias.cuda(), gated=gated)
+    want, err = grouped(xv, wv, off, rows, bias, gated)
+    mx4ref.close(got, want, err)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("scale", [1, 40])
+def test_expert_linear_odd_lists(kind, scale):
+    """the same row for many slots; indices outside x (rows of zeros); slots before the first and behind the last group; offsets outside the slots are clamped"""
+    g = gen(9)
+    x, xv, w, wv, dt = operands(kind, g, 6, 72, (3, 56, 72))
+    rows = [0, 0, 0, 5, -1, 6, 3, 3, 1 << 30, -(1 << 31), 2, 2] * scale
+    m = len(rows)
+    r = torch.tensor(rows, dtype=torch.int32, device="cuda")
+    a, b = 2 * scale, 7 * scale
+    off = [a, a, b, m - 1]
+    out = torch.full((m, 56), 7.0, dtype=dt, device="cuda")
+    ops.expert_linear(x, w, torch.tensor(off, dtype=torch.int32, device="cuda"), r, out=out)
+    mx4ref.close(out, *grouped(xv, wv, off, rows))
+    assert out[:a].eq(7).all() and out[m - 1].eq(7).all()
+    out.fill_(7)
+    ops.expert_linear(x, w, torch.tensor([-5, a, b, m + 1000], dtype=torch.int32, device="cuda"), r, out=out)
+    mx4ref.close(out, *grouped(xv, wv, [0, a, b, m], rows))
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_expert_linear_of_nothing(kind):
+    x, xv, w, wv, dt = operands(kind, gen(1), 0, 64, (2, 24, 64))
+    off = torch.zeros(3, dtype=torch.int32, device="cuda")
+    assert ops.expert_linear(x, w, off).shape == (0, 24)
+    bias = torch.ones(2, 24, device="cuda")
+    got = ops.expert_linear(x, w, torch.tensor([0, 1, 2], dtype=torch.int32, device="cuda"), torch.zeros(2, dtype=torch.int32, device="cuda"), bias)
+    assert got.eq(1).all()                                             # no row of x at all: rows of zeros
+    x, xv, w, wv, dt = operands(kind, gen(1), 2, 0, (2, 24, 0))
+    assert ops.expert_linear(x, w, torch.tensor([0, 1, 2], dtype=torch.int32, device="cuda"), None, bias).eq(1).all()
+
+
+@pytest.mark.parametrize("m", [3, 200])
+def test_linear_infinities_and_nan(m):
+    """a NaN or an infinity of x reaches its own row only"""
+    x, xv, w, wv, dt = operands("f16-mx4", gen(2), m, 96, (40, 96))
+    bad = x.clone()
+    bad[1, 5], bad[2, 95] = NAN, INF
+    got, fine = ops.mx4_linear(bad, w), ops.mx4_linear(x, w)
+    keep = [i for i in range(m) if i not in (1, 2)]
+    assert torch.equal(got[keep], fine[keep]) and got[1].isnan().all() and (~torch.isfinite(got[2])).all()
+
+
+def test_python_refusals():
+    x, xv, w, wv, dt = operands("f16-mx4", gen(2), 4, 64, (8, 64))
+    off = torch.tensor([0, 4], dtype=torch.int32, device="cuda")
+    w3 = ops.Mx4(w.codes[None], w.scales[None], 64)
+    for f in (lambda: ops.mx4_linear(x[:, :32], w), lambda: ops.mx4_linear(x.float(), w), lambda: ops.mx4_linear(x, w3), lambda: ops.mx4_linear(x, w, torch.zeros(7, device="cuda")),
+              lambda: ops.mx4_linear(x, w, torch.zeros(8, device="cuda", dtype=F16)), lambda: ops.mx4_linear(x, w, dtype=BF16), lambda: ops.mx4_linear(x, w, out=torch.empty(4, 9, device="cuda", dtype=F16)),
+              lambda: ops.mx4_linear(x, ops.Mx4(w.codes, w.scales, 40)), lambda: ops.mx4_linear(x, ops.Mx4(w.codes[:, ::2], w.scales, 64)), lambda: ops.mx4_linear(x, w, act=99),
+              lambda: ops.expert_linear(x, w3, off.long()), lambda: ops.expert_linear(x, w3, off[:1]), lambda: ops.expert_linear(x, w3, off, torch.zeros(4, device="cuda")),
+              lambda: ops.expert_linear(x, torch.zeros(1, 8, 64, device="cuda", dtype=BF16), off), lambda: ops.expert_linear(x, torch.zeros(1, 64, 8, device="cuda", dtype=F16).transpose(1, 2), off),
+              lambda: ops.expert_linear(x, ops.Mx4(w.codes[None, :7], w.scales[None, :7], 64), off, gated=True), lambda: ops.moe_route(x, 65), lambda: ops.moe_route(x, 0),
+              lambda: ops.moe_combine(x, off.view(1, 2), torch.zeros(1, 3, device="cuda")), lambda: ops.moe_combine(x.float(), off.view(1, 2), torch.zeros(1, 2, device="cuda"))):
+        with pytest.raises(N.SmelterError) as e:
+            f()
+        assert e.value.kind == "invalidArgument"
+
+
+# ---- routing ------------------------------------------------------------------------------------------------------------------------------
+
+
+def same_route(scores, k, renorm):
+    got = ops.moe_route(scores.cuda() if not scores.is_cuda else scores, k, renormalize=renorm)
+    want = mx4ref.route(scores.cpu(), k, renorm)
+    for name in ("experts", "offsets", "rows", "slots"):
+        assert torch.equal(getattr(got, name).cpu(), want[name]), name
+    # one exponential (within 2 ulp), a sum of E of them in a tree or a chain, a division
+    e = scores.shape[1]
+    assert ((got.weights.cpu().double() - want["weights"]).abs() <= (e + 8) * 2.0 ** -24 * want["weights"] + 2.0 ** -126).all()
+    return got
+
+
+@pytest.mark.parametrize("t", [F32, F16, BF16])
+@pytest.mark.parametrize("renorm", [True, False])
+@pytest.mark.parametrize("tokens, e, k", [(0, 4, 2), (1, 1, 1), (1, 8, 8), (7, 64, 6), (63, 65, 3), (64, 128, 32), (65, 60, 4), (130, 256, 8), (1000, 5, 2), (700, 1000, 8)])
+def test_route(t, renorm, tokens, e, k):
+    g = gen(tokens + e + k)
+    same_route((randn(g, tokens, e) + 2 * randn(g, e)).to(t), k, renorm)
+
+
+@pytest.mark.parametrize("tokens", [40, 300])
+@pytest.mark.parametrize("renorm", [True, False])
+def test_route_masks_and_ties(tokens, renorm):
+    g = gen(tokens)
+    z = torch.randint(-2, 3, (tokens, 70), generator=g).float()         # ties everywhere
+    z[z == 0] *= torch.where(torch.rand(int((z == 0).sum()), generator=g) < 0.5, -1.0, 1.0)   # zeros of either sign are equal
+    z[3] = -INF                                                         # nothing left
+    z[4] = NAN
+    z[5, 2:] = -INF                                                     # fewer than k left
+    z[6, 1:] = NAN
+    z[7] = torch.finfo(F32).min                                         # the lowest value is a score like any other
+    z[8, 5] = INF
+    z[9, [3, 60]] = INF
+    z[10, ::2] = -INF
+    z[11] = torch.finfo(F32).max
+    z[12, 0], z[12, 1:] = torch.finfo(F32).max, torch.finfo(F32).min
+    z[20:30] = -INF                                                     # padding
+    same_route(z, 6, renorm)
+
+
+def test_route_strided_and_many_tokens():
+    g = gen(1)
+    z = randn(g, 5000, 40).cuda()
+    same_route(z[:, 3:20], 3, True)
+    same_route(z[::7, :16], 3, False)
+    same_route(torch.zeros(3000, 64), 2, True)                          # everything to two experts
+
+
+@pytest.mark.parametrize("t", [F16, BF16])
+@pytest.mark.parametrize("tokens, k, n", [(1, 1, 1), (7, 6, 40), (50, 8, 131), (300, 2, 264), (3, 0, 8)])
+def test_combine(t, tokens, k, n):
+    g = gen(tokens + n)
+    m = max(1, tokens * k)
+    y, w = randn(g, m, n).to(t), torch.rand(tokens, k, generator=g)
+    slots = torch.randint(-1, m + 1, (tokens, k), generator=g).int()    # nothing, repeated ones, one outside
+    ok = ((slots >= 0) & (slots < m)).double() * w.double()
+    rows = y.double()[slots.clamp(0, m - 1).long()]
+    want, mag = (rows * ok[..., None]).sum(1), (rows.abs() * ok[..., None]).sum(1)
+    mx4ref.close(ops.moe_combine(y.cuda(), slots.cuda(), w.cuda()), want, (k + 1) * 2.0 ** -23 * mag)
+    wide = torch.full((tokens, n + 5), 7.0, dtype=t, device="cuda")
+    yw = torch.full((m, n + 3), NAN, dtype=t, device="cuda")
+    yw[:, 1:n + 1] = y.cuda()
+    ops.moe_combine(yw[:, 1:n + 1], slots.cuda(), w.cuda(), out=wide[:, 2:n + 2])
+    mx4ref.close(wide[:, 2:n + 2], want, (k + 1) * 2.0 ** -23 * mag)
+    assert wide[:, :2].eq(7).all() and wide[:, n + 2:].eq(7).all()
+
+
+# ---- together -----------------------------------------------------------------------------------------------------------------------------
+
+
+def layer(x, scores, hidden, answer, k):
+    r = ops.moe_route(scores, k)
+    h = ops.expert_linear(x, hidden, r.offsets, rows=r.rows, gated=True)
+    return ops.moe_combine(ops.expert_linear(h, answer, r.offsets), r.slots, r.weights)
+
+
+def layer_case(seed, tokens, kind, e=6, k=2, d=64, f=96):
+    g = gen(seed)
+    dt = BF16 if kind.startswith("bf16") else F16
+    x = randn(g, tokens, d).to(dt)
+    z = randn(g, tokens, e)
+    hidden, answer = randn(g, e, 2 * f, d, scale=d ** -0.5), randn(g, e, d, f, scale=f ** -0.5)
+    if kind.endswith("mx4"):
+        hidden, answer = mx4(hidden), mx4(answer)
+        hv, av = val(hidden), val(answer)
+    else:
+        hidden, answer = hidden.to(dt).cuda(), answer.to(dt).cuda()
+        hv, av = hidden.cpu().double(), answer.cpu().double()
+    return x, z, hidden, answer, hv, av
+
+
+def layer_want(x, z, hv, av, k):
+    r = mx4ref.route(z, k, True)
+    want, err = torch.zeros(x.shape[0], av.shape[1], dtype=torch.float64), torch.zeros(x.shape[0], av.shape[1], dtype=torch.float64)
+    step = mx4ref.half_step(x.dtype)
+    for i in range(x.shape[0]):
+        for j in range(k):
+            e = int(r["experts"][i, j])
+            if e < 0:
+                continue
+            h, he = mx4ref.linear(x[i:i + 1], hv[e], gated=True)
+            he = he + step * (h.abs() + he)                             # the hidden row is rounded once
+            y, ye = mx4ref.linear(h, av[e])
+            ye = ye * 1.01 + he @ av[e].abs().t()
+            ye = ye + step * (y.abs() + ye)                             # and the answer
+            w = float(r["weights"][i, j])
+            want[i] += w * y[0]
+            err[i] += w * (ye[0] + 2.0 ** -20 * y[0].abs())
+    return want, err
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16", "f16-mx4", "bf16-mx4"])
+@pytest.mark.parametrize("tokens", [1, 9, 80, 400])
+def test_layer(kind, tokens):
+    x, z, hidden, answer, hv, av = layer_case(tokens, tokens, kind)
+    mx4ref.close(layer(x.cuda(), z.cuda(), hidden, answer, 2), *layer_want(x, z, hv, av, 2))
+
+
+@pytest.mark.parametrize("tokens", [40, 200])
+def test_layer_padded_batch(tokens):
+    """padded tokens (all scores -inf, NaN rows of x) cost no slot, give zeros and touch nobody else"""
+    x, z, hidden, answer, hv, av = layer_case(7, tokens, "bf16-mx4")
+    full = layer(x.cuda(), z.cuda(), hidden, answer, 2)
+    pad = torch.zeros(tokens, dtype=torch.bool)
+    pad[5::3] = True
+    x2, z2 = x.clone(), z.clone()
+    x2[pad], z2[pad] = NAN, -INF
+    got = layer(x2.cuda(), z2.cuda(), hidden, answer, 2)
+    assert got[pad].eq(0).all() and torch.equal(got[~pad], full[~pad])
+
+
+@pytest.mark.parametrize("tokens", [9, 300])
+def test_layer_in_a_graph_and_on_a_stream(tokens):
+    """captured once, replayed on changing inputs with eager work between; two graphs of the same shapes share nothing"""
+    x, z, hidden, answer, hv, av = layer_case(3, tokens, "bf16-mx4")
+    xs, zs = [x.cuda(), x.cuda() * 2], [z.cuda(), -z.cuda()]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        first = layer(xs[0], zs[0], hidden, answer, 2)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(first, layer(xs[0], zs[0], hidden, answer, 2))
+    graphs, outs, ins = [], [], []
+    for i in range(2):
+        xi, zi = xs[i].clone(), zs[i].clone()
+        gr = torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(gr):
+            out = layer(xi, zi, hidden, answer, 2)
+        graphs.append(gr), outs.append(out), ins.append((xi, zi))
+    for turn in range(4):
+        for i in range(2):
+            ins[i][0].copy_(xs[(turn + i) % 2] + turn)
+            ins[i][1].copy_(zs[(turn + i) % 2])
+        graphs[0].replay()
+        graphs[1].replay()
+        for i in range(2):
+            assert torch.equal(outs[i], layer(*ins[i], hidden, answer, 2)), (turn, i)
+        torch.cuda.synchronize()
+
+
+def test_same_answer_every_time():
+    x, z, hidden, answer, hv, av = layer_case(3, 700, "f16-mx4")
+    a = (x.cuda(), z.cuda(), hidden, answer, 2)
+    first = layer(*a)
+    for _ in range(5):
+        assert torch.equal(layer(*a), first)
+
+
+def test_packed_by_the_gpu_and_used_at_once():
+    """weights and activations packed on the GPU, and the product of the packed pair"""
+    g = gen(4)
+    x, w = randn(g, 130, 200).to(BF16), randn(g, 90, 200, scale=0.07).to(BF16)
+    qx, qw = ops.mx4_quantize(x.cuda()), ops.mx4_quantize(w.cuda())
+    mx4ref.close(ops.mx4_linear(qx, qw, dtype=BF16), *mx4ref.linear(mx4ref.unpack(*mx4ref.pack(x), 200), mx4ref.unpack(*mx4ref.pack(w), 200)))
