@@ -1,7 +1,8 @@
 # Top-level build: libsmelter_hip.so (product: HIP kernels + C++ host + C ABI) and oracle/liborc.so (checker).
 HIPCC    ?= /opt/rocm/bin/hipcc
 ARCH     ?= gfx950
-HIPFLAGS ?= $(EXTRA) --offload-arch=$(ARCH) -O3 -std=c++17 -fPIC -Wall -Wno-unused-function -Wno-unused-result
+# (-packed-fp32-ops: the packed fp32 VALU forms that -O3 makes of ordinary float code have given wrong results on this hardware; the host pass does not know the feature and says so)
+HIPFLAGS ?= $(EXTRA) --offload-arch=$(ARCH) -O3 -std=c++17 -fPIC -Wall -Wno-unused-function -Wno-unused-result -Xclang -target-feature -Xclang -packed-fp32-ops
 CSRC     := smelter_amd/csrc
 KERNELS  := $(wildcard $(CSRC)/kernels/*.hip)
 HOSTSRC  := $(wildcard $(CSRC)/host/*.cpp)
