@@ -7,8 +7,7 @@ template <int XK, int WK> static int lin_stream(const LinearParams& q, hipStream
     p.n_tiles = (p.N + cols - 1) / cols;
     const long long per = p.offsets ? (p.M + p.E - 1) / p.E : p.M;      // rows of an average group
     const int mt = per <= 16 ? 1 : per <= 32 ? 2 : 4;
-    const long long groups = p.offsets ? (p.M < p.E ? p.M : p.E) : 1;
-    p.m_tiles = (p.M + (16ll * mt - 1) * groups) / (16 * mt);           // sum of ceil(rows / tile) over at most `groups` non-empty groups
+    p.m_tiles = lin_row_tiles(p, 16 * mt);
     const long long blocks = p.m_tiles * p.n_tiles;
     SM_REQUIRE(blocks < (1ll << 31), "linear: %lld row tiles x %d column tiles exceed one launch", p.m_tiles, p.n_tiles);
     if (mt == 4 && waves > 8) waves = 8;
@@ -56,8 +55,13 @@ extern "C" int sm_linear_fwd(const sm_linear_desc* d, const void* x, const void*
     SM_REQUIRE((size_t)y % ye == 0 && (size_t)bias % 4 == 0 && (size_t)offsets % 4 == 0 && (size_t)rows % 4 == 0 && (!x16 || (size_t)x % 2 == 0) && (d->w_type == SM_MX4 || (size_t)w % 2 == 0),
                "linear: an operand is not aligned to its element");
     SM_REQUIRE((x16 || (size_t)x % 16 == 0) && (d->w_type != SM_MX4 || (size_t)w % 16 == 0), "linear: MX4 codes need 16-byte alignment");
-    p.y_vec = (size_t)y % (4 * ye) == 0 && p.y_ld % 4 == 0;
+    p.y_vec = (size_t)y % 16 == 0 && p.y_ld * ye % 16 == 0;
     hipStream_t s = sm_s(stream);
+    const long long per = p.offsets ? (p.M + p.E - 1) / p.E : p.M;      // rows of an average group
+    if (per > 64 && lin_tile_fits(p)) {
+        const bool dma = d->x_type == SM_MX4 || (p.K % 8 == 0 && (size_t)x % 16 == 0 && p.x_ld % 16 == 0 && (d->w_type == SM_MX4 || (size_t)w % 16 == 0));
+        return lin_tile_launch(p, d->x_type, d->w_type, dma && per > 256 ? 1 : 0, dma, s);
+    }
     const int waves = p.K <= 256 ? 1 : p.K <= 1024 ? 4 : 8;
     if (d->x_type == SM_MX4) return lin_stream<SM_MX4, SM_MX4>(p, s, waves);
     if (d->w_type == SM_MX4) return d->x_type == SM_F16 ? lin_stream<SM_F16, SM_MX4>(p, s, waves) : lin_stream<SM_BF16, SM_MX4>(p, s, waves);

@@ -23,7 +23,7 @@ struct LinearParams {
     long long w_ld, ws_ld, w_es, ws_es;             // BYTES per weight row, scale row, expert
     long long y_ld, M, T;                           // y row stride in elements; slots; x rows
     int N, K, E, act; float slope;
-    int gated, y_type, y_vec, w_rows;               // y_vec: four consecutive outputs may be stored as one 8 / 16-byte word;  w_rows = N or 2 N
+    int gated, y_type, y_vec, w_rows;               // y_vec: eight consecutive outputs may be stored as 16-byte words;  w_rows = N or 2 N
     long long m_tiles; int n_tiles;                 // launch grid: a bound on the row tiles (the real number is known on the device only) x column tiles
 };
 
@@ -41,11 +41,21 @@ __device__ __forceinline__ void lin_store1(void* y, long long i, float v, int ty
     else if (type == SM_BF16) ((bf16_t*)y)[i] = (bf16_t)v;
     else ((float*)y)[i] = v;
 }
-__device__ __forceinline__ void lin_store4(void* y, long long i, floatx4 v, int type) {
-    if (type == SM_F16) *(half4_t*)((half_t*)y + i) = __builtin_convertvector(v, half4_t);
-    else if (type == SM_BF16) { typedef __bf16 b4 __attribute__((ext_vector_type(4))); *(b4*)((bf16_t*)y + i) = __builtin_convertvector(v, b4); }
-    else *(floatx4*)((float*)y + i) = v;
+__device__ __forceinline__ void lin_store8(void* y, long long i, const float* v, int type) {
+    if (type == SM_F16) { half8_t h; for (int q = 0; q < 8; q++) h[q] = (half_t)v[q]; *(half8_t*)((half_t*)y + i) = h; }
+    else if (type == SM_BF16) { bf16x8_t h; for (int q = 0; q < 8; q++) h[q] = (bf16_t)v[q]; *(bf16x8_t*)((bf16_t*)y + i) = h; }
+    else { *(floatx4*)((float*)y + i) = floatx4{v[0], v[1], v[2], v[3]}; *(floatx4*)((float*)y + i + 4) = floatx4{v[4], v[5], v[6], v[7]}; }
 }
+
+// a bound on the row tiles of BM slots: the sum of ceil(rows / BM) over at most min(E, M) non-empty groups
+inline long long lin_row_tiles(const LinearParams& p, int BM) {
+    const long long groups = p.offsets ? (p.M < p.E ? p.M : p.E) : 1;
+    return (p.M + (BM - 1ll) * groups) / BM;
+}
+// the tile kernels hold byte offsets inside an expert's weights, and inside x (gathered rows) or the rows of a tile, in 32 bits
+inline bool lin_tile_fits(const LinearParams& p) { return p.w_es < (1ll << 32) && (p.rows ? p.T * p.x_ld : 256 * p.x_ld) < (1ll << 32); }
+// linear_tile.hip: the tile kernels; shape 0 = 128 x 128, 1 = 256 x 256;  dma = both operands have rows of whole, 16-byte aligned chunks
+int lin_tile_launch(const LinearParams& p, int x_kind, int w_kind, int shape, bool dma, hipStream_t s);
 
 struct LinTile { int e; long long row0; int rows; long long index, total; };   // group, first slot, rows of the tile (<= BM); index of the row tile and number of row tiles
 
@@ -53,6 +63,9 @@ struct LinTile { int e; long long row0; int rows; long long index, total; };   /
 // lanes) until it has passed `t`.  Offsets are clamped to 0 .. M, a group that ends before it begins is empty: nothing outside the M slots is ever addressed, whatever they hold.
 // rows = 0: there is no such tile.  Wave-uniform.
 __device__ __forceinline__ long long lin_clamp(long long v, long long hi) { return v < 0 ? 0 : (v > hi ? hi : v); }
+__device__ __forceinline__ long long lin_uniform(long long v) {                     // a wave-uniform value into scalar registers
+    return ((long long)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32) | (unsigned)__builtin_amdgcn_readfirstlane((int)v);
+}
 __device__ __forceinline__ LinTile lin_find_tile(const LinearParams& p, int BM, long long t, bool want_total) {
     LinTile r; r.e = 0; r.row0 = 0; r.rows = 0; r.index = t; r.total = 0;
     if (!p.offsets) {
@@ -69,13 +82,14 @@ __device__ __forceinline__ LinTile lin_find_tile(const LinearParams& p, int BM, 
         int sum = n;
 #pragma unroll
         for (int d = 1; d < 64; d <<= 1) { int up = __shfl_up(sum, d); if (lane >= d) sum += up; }
-        const int all = __shfl(sum, 63);
+        const int all = __builtin_amdgcn_readlane(sum, 63);
         if (r.rows == 0 && t < r.total + all) {
             const unsigned long long past = __ballot(r.total + sum > t);
             const int at = __builtin_ctzll(past);
             const long long tl = t - r.total - (__shfl(sum, at) - __shfl(n, at));
             const long long l = __shfl(lo, at), h = __shfl(hi, at);
-            r.e = base + at; r.row0 = l + tl * BM; r.rows = (int)((h - r.row0) < BM ? (h - r.row0) : BM);
+            const long long row0 = l + tl * BM, left = h - row0;
+            r.e = base + at; r.row0 = lin_uniform(row0); r.rows = __builtin_amdgcn_readfirstlane((int)(left < BM ? left : BM));
             if (!want_total) return r;
         }
         r.total += all;
@@ -117,6 +131,6 @@ template <int KIND> __device__ __forceinline__ floatx4 lin_mma16(intx4_t a, intx
 }
 // 16 x 16 x 128 product of MX4 fragments: lane l holds row l & 15 and one block of 32, with its scale byte in the low byte of sa / sb
 __device__ __forceinline__ floatx4 lin_mma4(intx4_t a, int sa, intx4_t b, int sb, floatx4 c) {
-    const intx8_t va = {a[0], a[1], a[2], a[3], 0, 0, 0, 0}, vb = {b[0], b[1], b[2], b[3], 0, 0, 0, 0};
+    const intx8_t va = __builtin_shufflevector(a, a, 0, 1, 2, 3, -1, -1, -1, -1), vb = __builtin_shufflevector(b, b, 0, 1, 2, 3, -1, -1, -1, -1);   // (a 4-bit operand is four registers)
     return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(va, vb, c, 4, 4, 0, sa, 0, sb);
 }
