@@ -2,8 +2,8 @@
 #include "linear_tile.hpp"
 
 template <int XK, int WK> static int lin_tile_shape(const LinearParams& p, int shape, bool dma, hipStream_t s) {
-    if constexpr (XK != SM_MX4) if (!dma) return lin_tile<XK, WK, 2, 2, 4, 4, false>(p, s);
-    return shape ? lin_tile<XK, WK, 2, 4, 8, 4, true>(p, s) : lin_tile<XK, WK, 2, 2, 4, 4, true>(p, s);
+    if constexpr (XK != SM_MX4) if (!dma) return lin_tile<XK, WK, 2, 2, 2, 2, false>(p, s);
+    return shape ? lin_tile<XK, WK, 2, 4, 4, 2, true>(p, s) : lin_tile<XK, WK, 2, 2, 2, 2, true>(p, s);
 }
 
 int lin_tile_launch(const LinearParams& p, int x_kind, int w_kind, int shape, bool dma, hipStream_t s) {

@@ -2,8 +2,8 @@
 //
 // Both operands lie in LDS as rows of 128 bytes (64 16-bit elements, or 8 MX4 blocks = 256 elements), filled by the LDS-DMA without passing a register; 16-byte chunk c of row r sits at place
 // c ^ (r & 7), so that the 16 rows a fragment read touches spread over all banks.  The weights are the first operand of the matrix instruction: a lane then holds four consecutive columns of one
-// slot, which it stores together.  A 16 x 16 x 32 product of 16-bit fragments and a 16 x 16 x 128 product of MX4 fragments read the same bytes and take the same cycles, so both kinds share the
-// kernel; the MX4 one adds the scale bytes (staged for two steps at a time).  MX4 weights under a 16-bit x become 16-bit values on their way into LDS.
+// slot, which it stores together.  A 32 x 32 x 16 product of 16-bit fragments and a 32 x 32 x 64 product of MX4 fragments read the same bytes and take the same cycles, so both kinds share the
+// kernel; the MX4 one adds the scale bytes.  MX4 weights under a 16-bit x become 16-bit values on their way into LDS.
 #pragma once
 #include "linear.hpp"
 
@@ -16,10 +16,10 @@ __device__ __forceinline__ unsigned lin_lds_addr(const void* p) { return (unsign
 __device__ __forceinline__ void lin_arrive() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 template <int XK, int WK, int WN, int WM, int FN, int FM, bool DMA> struct LinTileShape {
-    static constexpr int THREADS = 64 * WN * WM, BN = 16 * FN * WN, BM = 16 * FM * WM;
+    static constexpr int THREADS = 64 * WN * WM, BN = 32 * FN * WN, BM = 32 * FM * WM;
     static constexpr bool DEQ = WK == SM_MX4 && XK != SM_MX4, MX = XK == SM_MX4;
     static constexpr int STAGE = (BN + BM) * 128;
-    static constexpr int SCALES = MX ? 2 * (BN + BM) * 16 : DEQ ? BN * 4 : 0;
+    static constexpr int SCALES = MX ? 2 * (BN + BM) * 8 : DEQ ? BN * 4 : 0;
     static constexpr int LDS = 2 * STAGE + SCALES;
 };
 
@@ -30,7 +30,7 @@ __global__ __launch_bounds__(64 * WN * WM) void lin_tile_kernel(LinearParams p) 
     constexpr bool DEQ = S::DEQ, MX = S::MX;
     __shared__ __align__(16) char lds[S::LDS];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int r = lane & 15, g = lane >> 4;
+    const int r = lane & 31, g = lane >> 5;
 
     // ---- which tile: consecutive tiles stay on one XCD (blocks are dealt to the 8 XCDs in turn), in squares of up to 8 row tiles, so that an XCD's L2 holds what its CUs read together
     const LinTile all = lin_find_tile(p, BM, 0, true);
@@ -106,7 +106,32 @@ __global__ __launch_bounds__(64 * WN * WM) void lin_tile_kernel(LinearParams p) 
             }
         }
     }
-    auto load_staged = [&](int t) {
+    // scales of MX4 operands: the eight bytes of a step of each row
+    constexpr int SB = MX ? (BN + BM) / THREADS : 1;
+    unsigned long long sreg[SB]; const unsigned char* srow[SB];
+    if constexpr (MX) {
+#pragma unroll
+        for (int i = 0; i < SB; i++) {
+            const int j = i * THREADS + tid;
+            if (j < BN) srow[i] = p.ws + tile.e * p.ws_es + weight_row(j) * p.ws_ld;
+            else { const long long s = slot_row(j - BN); srow[i] = p.xs + (s < 0 ? 0 : s) * p.xs_ld; }
+        }
+    }
+    auto load_staged = [&](int t, auto loop) {                                      // in the loop without a branch: the compiler would move products across it, out of their phase
+        if constexpr (MX) {
+            const int at = 8 * t < nb - 8 ? 8 * t : nb - 8;                         // the last ones of a row as its last eight bytes
+            if (decltype(loop)::value || nb >= 8) {
+#pragma unroll
+                for (int i = 0; i < SB; i++) __builtin_memcpy(&sreg[i], srow[i] + at, 8);
+            } else {                                                                // (a row of one step)
+#pragma unroll
+                for (int i = 0; i < SB; i++) {
+                    sreg[i] = 0;
+#pragma unroll
+                    for (int b = 0; b < 7; b++) if (b < nb) sreg[i] |= (unsigned long long)srow[i][b] << (8 * b);
+                }
+            }
+        }
         if constexpr (DEQ) {
 #pragma unroll
             for (int i = 0; i < DB; i++) {
@@ -125,6 +150,11 @@ __global__ __launch_bounds__(64 * WN * WM) void lin_tile_kernel(LinearParams p) 
         }
     };
     auto store_staged = [&](int t) {
+        if constexpr (MX) {
+            const int over = nb >= 8 && 8 * t > nb - 8 ? 8 * t - (nb - 8) : 0;      // bytes of the step before, shifted out; behind the end (codes 0) scale 0
+#pragma unroll
+            for (int i = 0; i < SB; i++) *(unsigned long long*)(lds + 2 * S::STAGE + ((t & 1) * (BN + BM) + i * THREADS + tid) * 8) = sreg[i] >> (8 * over);
+        }
         if constexpr (DEQ) {
             char* st = lds + (t & 1) * S::STAGE;
 #pragma unroll
@@ -147,86 +177,47 @@ __global__ __launch_bounds__(64 * WN * WM) void lin_tile_kernel(LinearParams p) 
             for (int i = 0; i < QX; i++) *(intx4_t*)(st + BN * 128 + (wave * QX + i) * 1024) = xreg[i];
         }
     };
-    // scales of MX4 operands: 16 bytes (two steps) of each row
-    constexpr int SB = MX ? (BN + BM) / THREADS : 1;
-    intx4_t sreg[SB]; const unsigned char* srow[SB];
-    if constexpr (MX) {
-#pragma unroll
-        for (int i = 0; i < SB; i++) {
-            const int j = i * THREADS + tid;
-            if (j < BN) srow[i] = p.ws + tile.e * p.ws_es + weight_row(j) * p.ws_ld;
-            else { const long long s = slot_row(j - BN); srow[i] = p.xs + (s < 0 ? 0 : s) * p.xs_ld; }
-        }
-    }
-    auto load_scales = [&](int u) {                                                 // of steps 2 u, 2 u + 1
-        if constexpr (MX) if (16 * u + 16 <= nb) {
-#pragma unroll
-            for (int i = 0; i < SB; i++) __builtin_memcpy(&sreg[i], srow[i] + 16 * u, 16);
-        }
-    };
-    auto store_scales = [&](int u) {
-        if constexpr (MX) {
-            char* st = lds + 2 * S::STAGE + (u & 1) * (BN + BM) * 16;
-#pragma unroll
-            for (int i = 0; i < SB; i++) {
-                intx4_t v = sreg[i];
-                if (16 * u + 16 > nb) {                                             // the last ones of a row: byte by byte; behind the end (codes 0) the last one again
-                    unsigned q[4] = {0, 0, 0, 0};
-#pragma unroll
-                    for (int b = 0; b < 16; b++) q[b >> 2] |= (unsigned)srow[i][16 * u + b < nb ? 16 * u + b : nb - 1] << (8 * (b & 3));
-                    v = intx4_t{(int)q[0], (int)q[1], (int)q[2], (int)q[3]};
-                }
-                *(intx4_t*)(st + (i * THREADS + tid) * 16) = v;
-            }
-        }
-    };
-
-    // ---- the products of a step in PH phases of 4 x FM tiles; a phase's fragments are read during the phase before it (over the step boundary too)
-    constexpr int HA = FN / 4, PH = 2 * HA;
+    // ---- the products of a step in four phases, one for each 32 bytes of K; a phase's fragments are read during the phase before it (over the step boundary too)
+    constexpr int PH = 4;
     const int wn = wave / WM, wm = wave - wn * WM;                                  // this wave's part of the tile
-    floatx4 acc[FN][FM];
+    floatx16 acc[FN][FM];
 #pragma unroll
     for (int a = 0; a < FN; a++)
 #pragma unroll
-        for (int b = 0; b < FM; b++) acc[a][b] = floatx4{0, 0, 0, 0};
-    intx4_t wf[2][4], xf[2][FM]; int wsc[2][MX ? 4 : 1], xsc[2][MX ? FM : 1];
-    const int off0 = ((g ^ (lane & 7)) << 4) + r * 128, off1 = (((4 + g) ^ (lane & 7)) << 4) + r * 128;
+        for (int b = 0; b < FM; b++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) acc[a][b][i] = 0.f;
+    intx4_t wf[2][FN], xf[2][FM]; int wsc[2][MX ? FN : 1], xsc[2][MX ? FM : 1];
     auto read = [&](int t, auto phase, bool masked) {
-        constexpr int P = decltype(phase)::value, H = P / HA, A = P % HA;
-        const char* st = lds + (t & 1) * S::STAGE + (H ? off1 : off0);
+        constexpr int P = decltype(phase)::value, B = P & 1;
+        const char* st = lds + (t & 1) * S::STAGE + r * 128 + (((2 * P + g) ^ (lane & 7)) << 4);
 #pragma unroll
-        for (int a = 0; a < 4; a++) wf[P & 1][a] = *(const intx4_t*)(st + (wn * FN + A * 4 + a) * 2048);
-        if constexpr (A == 0) {
+        for (int a = 0; a < FN; a++) wf[B][a] = *(const intx4_t*)(st + (wn * FN + a) * 4096);
 #pragma unroll
-            for (int b = 0; b < FM; b++) xf[H][b] = *(const intx4_t*)(st + (BN / 16 + wm * FM + b) * 2048);
-        }
+        for (int b = 0; b < FM; b++) xf[B][b] = *(const intx4_t*)(st + (BN / 32 + wm * FM + b) * 4096);
         if constexpr (MX) {
-            const unsigned char* sc = (const unsigned char*)lds + 2 * S::STAGE + ((t >> 1) & 1) * (BN + BM) * 16 + (t & 1) * 8 + r * 16 + g;
+            const unsigned char* sc = (const unsigned char*)lds + 2 * S::STAGE + (t & 1) * (BN + BM) * 8 + r * 8 + g + 2 * P;
 #pragma unroll
-            for (int a = 0; a < 4; a++) wsc[P & 1][a] = sc[(wn * FN + A * 4 + a) * 256 + 4 * H];
-            if constexpr (A == 0) {
+            for (int a = 0; a < FN; a++) wsc[B][a] = sc[(wn * FN + a) * 256];
 #pragma unroll
-                for (int b = 0; b < FM; b++) xsc[H][b] = sc[(BN / 16 + wm * FM + b) * 256 + 4 * H];
-            }
+            for (int b = 0; b < FM; b++) xsc[B][b] = sc[(BN / 32 + wm * FM + b) * 256];
         }
         if (masked) {                                                               // chunks behind the end of the row
-            const bool dead = t * 128 + (4 * H + g) * 16 >= x_bytes;
+            const bool dead = t * 128 + (2 * P + g) * 16 >= x_bytes;
 #pragma unroll
-            for (int a = 0; a < 4; a++) wf[P & 1][a] = dead ? intx4_t{0, 0, 0, 0} : wf[P & 1][a];
-            if constexpr (A == 0) {
+            for (int a = 0; a < FN; a++) wf[B][a] = dead ? intx4_t{0, 0, 0, 0} : wf[B][a];
 #pragma unroll
-                for (int b = 0; b < FM; b++) xf[H][b] = dead ? intx4_t{0, 0, 0, 0} : xf[H][b];
-            }
+            for (int b = 0; b < FM; b++) xf[B][b] = dead ? intx4_t{0, 0, 0, 0} : xf[B][b];
         }
     };
-    auto products = [&](auto phase, auto between) {                                 // between(i): behind the i-th row of tiles
-        constexpr int P = decltype(phase)::value, H = P / HA, A = P % HA;
-        sm_static_for<0, 4>([&](auto ai) {
+    auto products = [&](auto phase, auto between) {                                 // between(a): behind the a-th row of tiles
+        constexpr int B = decltype(phase)::value & 1;
+        sm_static_for<0, FN>([&](auto ai) {
             constexpr int a = decltype(ai)::value;
 #pragma unroll
             for (int b = 0; b < FM; b++) {
-                if constexpr (MX) acc[A * 4 + a][b] = lin_mma4(wf[P & 1][a], wsc[P & 1][a], xf[H][b], xsc[H][b], acc[A * 4 + a][b]);
-                else acc[A * 4 + a][b] = lin_mma16<XK>(wf[P & 1][a], xf[H][b], acc[A * 4 + a][b]);
+                if constexpr (MX) acc[a][b] = lin_mma4(wf[B][a], wsc[B][a], xf[B][b], xsc[B][b], acc[a][b]);
+                else acc[a][b] = lin_mma16<XK>(wf[B][a], xf[B][b], acc[a][b]);
             }
             between(a);
         });
@@ -238,16 +229,15 @@ __global__ __launch_bounds__(64 * WN * WM) void lin_tile_kernel(LinearParams p) 
 #pragma unroll
             for (int i = 0; i < QT; i++) fill(0, i);
         }
-        load_staged(0); store_staged(0); load_scales(0); store_scales(0);
+        load_staged(0, std::false_type()); store_staged(0);
         if (steps > 1) {
             if constexpr (DMA) {
 #pragma unroll
                 for (int i = 0; i < QT / 2; i++) fill(1, i);
             }
-            load_staged(1); store_staged(1);
+            load_staged(1, std::false_type()); store_staged(1);
         }
-        if (steps > 2) { load_scales(1); store_scales(1); load_staged(2); }
-        if (steps > 4) load_scales(2);
+        if (steps > 2) load_staged(2, std::false_type());
         lin_arrive();
         read(0, First(), ragged && steps == 1);
     }
@@ -259,21 +249,20 @@ __global__ __launch_bounds__(64 * WN * WM) void lin_tile_kernel(LinearParams p) 
                 if (a == 0) { __builtin_amdgcn_sched_barrier(0); read(t, std::integral_constant<int, P + 1>(), !MORE && ragged); __builtin_amdgcn_sched_barrier(0); }
                 if constexpr (DMA && P == 0 && MORE) {                              // the second half of the next step's fill, one instruction at a time
 #pragma unroll
-                    for (int i = QT / 2 + a * (QT - QT / 2) / 4; i < QT / 2 + (a + 1) * (QT - QT / 2) / 4; i++) fill(t + 1, i);
+                    for (int i = QT / 2 + a * (QT - QT / 2) / FN; i < QT / 2 + (a + 1) * (QT - QT / 2) / FN; i++) fill(t + 1, i);
                 }
             });
             __builtin_amdgcn_sched_barrier(0);
         });
         if constexpr (MORE) {
             lin_arrive();                                                           // step t + 1 is in LDS for everybody; everybody has read the whole of step t
-            if constexpr (MORE2) { store_staged(t + 2); if (t + 3 < steps) load_staged(t + 3); }
-            if constexpr (MX && MORE2) if (t & 1) { const int u = (t >> 1) + 2; if (2 * u < steps) { store_scales(u); if (2 * u + 2 < steps) load_scales(u + 1); } }
+            if constexpr (MORE2) { store_staged(t + 2); load_staged(t + 3 < steps ? t + 3 : steps - 1, std::true_type()); }
         }
         products(Last(), [&](int a) {
             if constexpr (MORE) if (a == 0) { __builtin_amdgcn_sched_barrier(0); read(t + 1, First(), !MORE2 && ragged); __builtin_amdgcn_sched_barrier(0); }
             if constexpr (DMA && MORE2) {                                           // the first half of the fill behind it
 #pragma unroll
-                for (int i = a * (QT / 2) / 4; i < (a + 1) * (QT / 2) / 4; i++) fill(t + 2, i);
+                for (int i = a * (QT / 2) / FN; i < (a + 1) * (QT / 2) / FN; i++) fill(t + 2, i);
             }
         });
         __builtin_amdgcn_sched_barrier(0);
@@ -284,26 +273,31 @@ __global__ __launch_bounds__(64 * WN * WM) void lin_tile_kernel(LinearParams p) 
     if (t + 1 < steps) { step(t, std::true_type(), std::false_type()); t++; }
     if (t < steps) step(t, std::false_type(), std::false_type());
 
-    // ---- epilogue: acc[a][b][i] = tile row 16 (wn FN + a) + 4 g + i of the weights, slot 16 (wm FM + b) + r.  The fp32 tile goes through LDS (chunks of four columns, xor-ed with the slot) so that a
+    // ---- epilogue: acc[a][b][i] = tile row 32 (wn FN + a) + 8 (i / 4) + 4 g + i % 4 of the weights, slot 32 (wm FM + b) + r.  The fp32 tile goes through LDS (chunks of four columns, xor-ed with the slot) so that a
     // thread stores eight consecutive columns: whole 512-byte rows instead of 8-byte pieces.
-    constexpr int PB = 2 * S::STAGE / (BN * 4) / (16 * WM) < FM ? 2 * S::STAGE / (BN * 4) / (16 * WM) : FM;   // slot groups of a wave that fit at once
+    constexpr int PB = 2 * S::STAGE / (BN * 4) / (32 * WM) < FM ? 2 * S::STAGE / (BN * 4) / (32 * WM) : FM;   // slot groups of a wave that fit at once
     const float* bias = p.bias ? p.bias + (long long)tile.e * p.w_rows : nullptr;
 #pragma unroll
     for (int b0 = 0; b0 < FM; b0 += PB) {
         __syncthreads();
 #pragma unroll
-        for (int a = 0; a < FN; a++) {
-            const int j = (wn * FN + a) * 4 + g;
-            floatx4 m = {1, 1, 1, 1};
-            if constexpr (DEQ && XK == SM_F16) m = *(const floatx4*)(wmul + 4 * j);
+        for (int a = 0; a < FN; a++)
 #pragma unroll
-            for (int b = 0; b < PB; b++) *(floatx4*)(lds + ((wm * PB + b) * 16 + r) * BN * 4 + ((j ^ r) << 4)) = acc[a][b0 + b] * m;
-        }
+            for (int q = 0; q < 4; q++) {
+                const int j = (wn * FN + a) * 8 + 2 * q + g;                        // chunk of four columns
+                floatx4 m = {1, 1, 1, 1};
+                if constexpr (DEQ && XK == SM_F16) m = *(const floatx4*)(wmul + 4 * j);
+#pragma unroll
+                for (int b = 0; b < PB; b++) {
+                    const floatx16 v = acc[a][b0 + b];
+                    *(floatx4*)(lds + ((wm * PB + b) * 32 + r) * BN * 4 + ((j ^ (r & 15)) << 4)) = floatx4{v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]} * m;
+                }
+            }
         __syncthreads();
         const int per = cols / 8;
-        for (int o = tid; o < PB * WM * 16 * per; o += THREADS) {
+        for (int o = tid; o < PB * WM * 32 * per; o += THREADS) {
             const int l = o / per, c = o - l * per, n = n0 + c * 8;                 // LDS row, group of eight columns
-            const int slot = (l / (16 * PB) * FM + b0) * 16 + l % (16 * PB);
+            const int slot = (l / (32 * PB) * FM + b0) * 32 + l % (32 * PB);
             if (slot >= tile.rows || n >= p.N) continue;
             const char* row = lds + l * BN * 4;
             const int j = p.gated ? (c >> 1) * 8 + (c & 1) * 2 : 2 * c, x = l & 15;
