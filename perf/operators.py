@@ -270,7 +270,8 @@ def _own(s):
         return ops.moe_combine(s["data"], s["plan"]["slots"], s["part"])
     r = ops.moe_route(s["score"], s["top"])
     h = ops.expert_linear(s["data"], _own_weight(ops, s["hidden"], s["k"]), r.offsets, rows=r.rows, gated=True)
-    return ops.moe_combine(ops.expert_linear(h, _own_weight(ops, s["answer"], s["f"]), r.offsets), r.slots, r.weights)
+    y = ops.expert_linear(h, _own_weight(ops, s["answer"], s["f"]), r.offsets, dtype=torch.float32)
+    return ops.moe_combine(y, r.slots, r.weights, dtype=s["data"].dtype)
 
 
 def run(state):
