@@ -371,7 +371,9 @@ typedef struct sm_linear_desc {
     int64_t x_ld, y_ld;             /* row strides in elements, 0 = dense (an MX4 x is dense) */
 } sm_linear_desc;
 int sm_linear_fwd(const sm_linear_desc* d, const void* x, const void* x_scales, const void* w, const void* w_scales, const float* bias /* [E][N or 2 N] or NULL */, const int32_t* offsets,
-                  const int32_t* rows, void* y, sm_stream_t stream);
+                  const int32_t* rows, void* y, void* workspace, size_t workspace_bytes, sm_stream_t stream);
+/* bytes of scratch sm_linear_fwd wants for these sizes (sums of a product whose K is cut because there are few tiles), 16-byte aligned; 0 if none.  grouped, gathered: offsets, rows are given */
+size_t sm_linear_workspace_bytes(const sm_linear_desc* d, int32_t grouped, int32_t gathered);
 
 /* Routing: for each of T tokens the k <= 32 largest of its E <= 1024 scores (ties: the lower index first) and their softmax weights (over the chosen ones, or over all E when !renormalize),
  * and the assignments in the order of their expert (stable): offsets [E + 1], rows [T k] = token of each slot, slots [T][k] = slot of each assignment.  A score of -inf or NaN is never
@@ -379,8 +381,8 @@ int sm_linear_fwd(const sm_linear_desc* d, const void* x, const void* x_scales, 
 size_t sm_moe_route_workspace_bytes(int64_t T, int32_t E, int32_t k);
 int sm_moe_route(const void* scores, int32_t type, int64_t T, int32_t E, int32_t k, int64_t ld, int32_t renormalize, float* weights /* [T][k] */, int32_t* experts /* [T][k] */,
                  int32_t* offsets, int32_t* rows, int32_t* slots, void* workspace, size_t workspace_bytes, sm_stream_t stream);
-/* out[t] = sum_j weights[t][j] * y[slots[t][j]] over [M][N] rows of y (fp16 | bf16), added in the order of j in fp32; a slot outside 0 .. M - 1 adds nothing */
-int sm_moe_combine(const void* y, int32_t type, int64_t M, int32_t N, int64_t y_ld, const float* weights, const int32_t* slots, int64_t T, int32_t k, void* out, int64_t out_ld,
+/* out[t] = sum_j weights[t][j] * y[slots[t][j]] over [M][N] rows of y (fp16 | bf16 | fp32), added in the order of j in fp32, one rounding to out_type; a slot outside 0 .. M - 1 adds nothing */
+int sm_moe_combine(const void* y, int32_t type, int64_t M, int32_t N, int64_t y_ld, const float* weights, const int32_t* slots, int64_t T, int32_t k, void* out, int32_t out_type, int64_t out_ld,
                    sm_stream_t stream);
 
 /* Host-side weight preparation Smelter does on the CPU at load time */

@@ -151,10 +151,11 @@ SYMBOLS = {
     "sm_float_array_count": (_sz, [_i32] * 4),
     "sm_mx4_quantize": (_i32, [_vp, _i32, _i64, _i32, _i64, _vp, _vp, _vp]),
     "sm_mx4_dequantize": (_i32, [_vp, _vp, _i64, _i32, _vp, _i32, _i64, _vp]),
-    "sm_linear_fwd": (_i32, [C.POINTER(LinearDesc)] + [_vp] * 9),
+    "sm_linear_fwd": (_i32, [C.POINTER(LinearDesc)] + [_vp] * 9 + [_sz, _vp]),
+    "sm_linear_workspace_bytes": (_sz, [C.POINTER(LinearDesc), _i32, _i32]),
     "sm_moe_route_workspace_bytes": (_sz, [_i64, _i32, _i32]),
     "sm_moe_route": (_i32, [_vp, _i32, _i64, _i32, _i32, _i64, _i32] + [_vp] * 6 + [_sz, _vp]),
-    "sm_moe_combine": (_i32, [_vp, _i32, _i64, _i32, _i64, _vp, _vp, _i64, _i32, _vp, _i64, _vp]),
+    "sm_moe_combine": (_i32, [_vp, _i32, _i64, _i32, _i64, _vp, _vp, _i64, _i32, _vp, _i32, _i64, _vp]),
     "sm_half_to_float": (None, [_vp, _vp, _sz]),
     "sm_float_to_half": (None, [_vp, _vp, _sz]),
     "sm_reformat_conv_weight": (_i32, [_vp, _vp] + [_i32] * 6),

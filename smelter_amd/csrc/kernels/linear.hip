@@ -5,17 +5,10 @@ template <int XK, int WK> static int lin_stream(const LinearParams& q, hipStream
     LinearParams p = q;
     const int cols = p.gated ? 16 : 32;
     p.n_tiles = (p.N + cols - 1) / cols;
-    const long long per = p.offsets ? (p.M + p.E - 1) / p.E : p.M;      // rows of an average group
-    const int mt = per <= 16 ? 1 : per <= 32 ? 2 : 4;
-    p.m_tiles = lin_row_tiles(p, 16 * mt);
+    p.m_tiles = lin_row_tiles(p, 16);
     const long long blocks = p.m_tiles * p.n_tiles;
     SM_REQUIRE(blocks < (1ll << 31), "linear: %lld row tiles x %d column tiles exceed one launch", p.m_tiles, p.n_tiles);
-    if (mt == 4 && waves > 8) waves = 8;
-    const size_t lds = (size_t)waves * 2 * mt * 16 * 17 * 4;
-    const dim3 grid((unsigned)blocks), block(64 * waves);
-    if (mt == 1) lin_stream_kernel<XK, WK, 1><<<grid, block, lds, s>>>(p);
-    else if (mt == 2) lin_stream_kernel<XK, WK, 2><<<grid, block, lds, s>>>(p);
-    else lin_stream_kernel<XK, WK, 4><<<grid, block, lds, s>>>(p);
+    lin_stream_kernel<XK, WK><<<dim3((unsigned)blocks), 64 * waves, (size_t)waves * 2 * 16 * 17 * 4, s>>>(p);
     SM_LAUNCH_CHECK();
     return SM_OK;
 }
@@ -25,8 +18,45 @@ static int lin_size(int kind, long long K, long long* row, long long* scale_row)
     return 0;
 }
 
+struct LinearPlan { int shape, splits, deep; };                                      // shape -1: the streaming kernel
+static long long lin_part_ld(long long w_rows) { return (w_rows + 3) / 4 * 4; }
+
+// Which kernel, by sizes alone (the offsets are on the device): `per` = slots of an average group.
+static LinearPlan lin_plan(const sm_linear_desc* d, bool grouped, bool gathered) {
+    LinearParams p = {};
+    long long xr, xsr, wr, wsr;
+    lin_size(d->x_type, d->K, &xr, &xsr); lin_size(d->w_type, d->K, &wr, &wsr);
+    p.M = d->M; p.T = d->T; p.N = d->N; p.E = d->E; p.gated = d->gated != 0;
+    p.offsets = grouped ? (const int*)8 : nullptr; p.rows = gathered ? (const int*)8 : nullptr;     // (looked at for being there only)
+    p.x_ld = d->x_type != SM_MX4 && d->x_ld ? 2 * d->x_ld : xr; p.w_es = wr * (p.gated ? 2 : 1) * d->N;
+    const long long per = grouped ? (d->M + d->E - 1) / d->E : d->M;
+    LinearPlan plan = {-1, 1, 0};
+    if (per <= 16 || !lin_tile_fits(p)) return plan;
+    auto tiles = [&](int bn, int bm) { const int cols = p.gated ? bn / 2 : bn; return lin_row_tiles(p, bm) * ((p.N + cols - 1) / cols); };
+    const long long n0 = tiles(128, 128), n1 = tiles(256, 256), n2 = tiles(128, 64);
+    // times in units of a round of 512 tiles of 128 x 128, two on a CU
+    const double t0 = n0 <= 256 ? 0.65 : n0 <= 384 ? 0.75 : n0 / 512.0, t1 = (n1 + 255) / 256 * 1.24, t2 = n2 <= 256 ? 0.42 : n2 * 0.75 / 512.0 < 0.7 ? 0.7 : n2 * 0.75 / 512.0;
+    plan.shape = t2 <= t0 && t2 <= t1 ? 2 : t0 <= t1 ? 0 : 1;
+    const long long n = plan.shape == 2 ? n2 : n0;
+    plan.deep = d->x_type != SM_MX4 && plan.shape != 1 && n <= SM_NUM_CU;
+    if (plan.shape == 2 && n * 2 <= SM_NUM_CU && d->E <= 64) {
+        const int steps = (int)(((d->x_type == SM_MX4 ? xr : 2ll * d->K) + 127) / 128);
+        long long s = SM_NUM_CU / n;
+        if (s > steps / 8) s = steps / 8;
+        if (s > (d->M <= 32 ? 8 : 4)) s = d->M <= 32 ? 8 : 4;                       // (the sums that go through memory grow with M)
+        if (s > 2 || (s == 2 && steps >= 48)) plan.splits = (int)s;
+    }
+    return plan;
+}
+
+extern "C" size_t sm_linear_workspace_bytes(const sm_linear_desc* d, int32_t grouped, int32_t gathered) {
+    if (!d || d->M <= 0 || d->N <= 0 || d->E < 1) return 0;
+    const LinearPlan plan = lin_plan(d, grouped, gathered);
+    return plan.shape < 0 || plan.splits <= 1 ? 0 : (size_t)plan.splits * d->M * lin_part_ld((d->gated ? 2ll : 1ll) * d->N) * 4;
+}
+
 extern "C" int sm_linear_fwd(const sm_linear_desc* d, const void* x, const void* x_scales, const void* w, const void* w_scales, const float* bias, const int32_t* offsets,
-                             const int32_t* rows, void* y, sm_stream_t stream) {
+                             const int32_t* rows, void* y, void* workspace, size_t workspace_bytes, sm_stream_t stream) {
     SM_REQUIRE(d, "linear: null descriptor");
     SM_REQUIRE(d->M >= 0 && d->T >= 0 && d->N >= 0 && d->K >= 0 && d->E >= 1, "linear: sizes M %lld, T %lld, N %d, K %d, E %d", (long long)d->M, (long long)d->T, d->N, d->K, d->E);
     SM_REQUIRE(d->N <= (1 << 29) && d->K <= (1 << 29) && d->M < (1ll << 31) && d->T < (1ll << 31) && d->E <= (1 << 20), "linear: a size beyond what the kernels index");
@@ -46,7 +76,7 @@ extern "C" int sm_linear_fwd(const sm_linear_desc* d, const void* x, const void*
     SM_REQUIRE(y, "linear: null output");
     SM_REQUIRE(d->K == 0 || d->T == 0 || (x && w && (d->x_type != SM_MX4 || x_scales) && (d->w_type != SM_MX4 || w_scales)), "linear: null operand");
     p.x = (const char*)x; p.xs = (const unsigned char*)x_scales; p.w = (const char*)w; p.ws = (const unsigned char*)w_scales; p.bias = bias; p.y = y; p.offsets = offsets; p.rows = rows;
-    p.M = d->M; p.T = d->T; p.N = d->N; p.K = d->T == 0 ? 0 : d->K; p.E = d->E; p.act = d->act; p.slope = d->slope; p.gated = d->gated != 0; p.y_type = d->y_type;
+    p.M = d->M; p.T = d->T; p.N = d->N; p.K = d->T == 0 ? 0 : d->K; p.E = d->E; p.splits = 1; p.act = d->act; p.slope = d->slope; p.gated = d->gated != 0; p.y_type = d->y_type;
     p.w_rows = p.gated ? 2 * p.N : p.N;
     p.x_ld = x16 && d->x_ld ? 2 * d->x_ld : xr; p.xs_ld = xsr; p.w_ld = wr; p.ws_ld = wsr; p.w_es = wr * p.w_rows; p.ws_es = wsr * p.w_rows; p.y_ld = d->y_ld ? d->y_ld : d->N;
     SM_REQUIRE(d->T <= 1 || p.x_ld >= xr, "linear: row stride of x %lld below its %d columns", (long long)d->x_ld, d->K);
@@ -57,10 +87,21 @@ extern "C" int sm_linear_fwd(const sm_linear_desc* d, const void* x, const void*
     SM_REQUIRE((x16 || (size_t)x % 16 == 0) && (d->w_type != SM_MX4 || (size_t)w % 16 == 0), "linear: MX4 codes need 16-byte alignment");
     p.y_vec = (size_t)y % 16 == 0 && p.y_ld * ye % 16 == 0;
     hipStream_t s = sm_s(stream);
-    const long long per = p.offsets ? (p.M + p.E - 1) / p.E : p.M;      // rows of an average group
-    if (per > 64 && lin_tile_fits(p)) {
+    LinearPlan plan = lin_plan(d, offsets != nullptr, rows != nullptr);
+    if (plan.shape >= 0) {
         const bool dma = d->x_type == SM_MX4 || (p.K % 8 == 0 && (size_t)x % 16 == 0 && p.x_ld % 16 == 0 && (d->w_type == SM_MX4 || (size_t)w % 16 == 0));
-        return lin_tile_launch(p, d->x_type, d->w_type, dma && per > 256 ? 1 : 0, dma, s);
+        if (!dma && plan.shape == 1) plan.shape = 0;
+        p.splits = plan.splits;
+        if (p.splits > 1) {
+            p.part_ld = lin_part_ld(p.w_rows);
+            SM_REQUIRE(workspace && (size_t)workspace % 16 == 0 && workspace_bytes >= (size_t)p.splits * p.M * p.part_ld * 4, "linear: workspace of %zu bytes (16-byte aligned), %zu wanted", workspace_bytes,
+                       (size_t)p.splits * p.M * p.part_ld * 4);
+            p.part = (float*)workspace;
+        }
+        int rc = 1;
+        if (dma && plan.deep) rc = lin_deep_launch(p, d->x_type, d->w_type, plan.shape, s);
+        if (rc > 0) rc = lin_tile_launch(p, d->x_type, d->w_type, plan.shape, dma, s);
+        return rc != SM_OK || p.splits == 1 ? rc : lin_join_launch(p, s);
     }
     const int waves = p.K <= 256 ? 1 : p.K <= 1024 ? 4 : 8;
     if (d->x_type == SM_MX4) return lin_stream<SM_MX4, SM_MX4>(p, s, waves);

@@ -9,6 +9,7 @@
 
 typedef __bf16 bf16_t;
 typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x4_t __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef int intx4_t __attribute__((ext_vector_type(4)));
 typedef int intx8_t __attribute__((ext_vector_type(8)));
@@ -24,6 +25,7 @@ struct LinearParams {
     long long y_ld, M, T;                           // y row stride in elements; slots; x rows
     int N, K, E, act; float slope;
     int gated, y_type, y_vec, w_rows;               // y_vec: eight consecutive outputs may be stored as 16-byte words;  w_rows = N or 2 N
+    float* part; long long part_ld; int splits;     // fp32 sums [splits][M][part_ld] of a product whose K is cut into `splits` runs (1: none)
     long long m_tiles; int n_tiles;                 // launch grid: a bound on the row tiles (the real number is known on the device only) x column tiles
 };
 
@@ -41,6 +43,11 @@ __device__ __forceinline__ void lin_store1(void* y, long long i, float v, int ty
     else if (type == SM_BF16) ((bf16_t*)y)[i] = (bf16_t)v;
     else ((float*)y)[i] = v;
 }
+__device__ __forceinline__ void lin_store4(void* y, long long i, const float* v, int type) {
+    if (type == SM_F16) { half4_t h; for (int q = 0; q < 4; q++) h[q] = (half_t)v[q]; *(half4_t*)((half_t*)y + i) = h; }
+    else if (type == SM_BF16) { bf16x4_t h; for (int q = 0; q < 4; q++) h[q] = (bf16_t)v[q]; *(bf16x4_t*)((bf16_t*)y + i) = h; }
+    else *(floatx4*)((float*)y + i) = floatx4{v[0], v[1], v[2], v[3]};
+}
 __device__ __forceinline__ void lin_store8(void* y, long long i, const float* v, int type) {
     if (type == SM_F16) { half8_t h; for (int q = 0; q < 8; q++) h[q] = (half_t)v[q]; *(half8_t*)((half_t*)y + i) = h; }
     else if (type == SM_BF16) { bf16x8_t h; for (int q = 0; q < 8; q++) h[q] = (bf16_t)v[q]; *(bf16x8_t*)((bf16_t*)y + i) = h; }
@@ -54,8 +61,11 @@ inline long long lin_row_tiles(const LinearParams& p, int BM) {
 }
 // the tile kernels hold byte offsets inside an expert's weights, and inside x (gathered rows) or the rows of a tile, in 32 bits
 inline bool lin_tile_fits(const LinearParams& p) { return p.w_es < (1ll << 32) && (p.rows ? p.T * p.x_ld : 256 * p.x_ld) < (1ll << 32); }
-// linear_tile.hip: the tile kernels; shape 0 = 128 x 128, 1 = 256 x 256;  dma = both operands have rows of whole, 16-byte aligned chunks
+// linear_tile.hip: the tile kernels; shape 0 = 128 x 128, 1 = 256 x 256, 2 = 128 columns x 64 slots;  dma = both operands have rows of whole, 16-byte aligned chunks
 int lin_tile_launch(const LinearParams& p, int x_kind, int w_kind, int shape, bool dma, hipStream_t s);
+// linear_deep.hip: the kernel for few tiles, shapes 0 and 2 of whole chunks; > 0: not enough LDS for the scales of so long a row
+int lin_deep_launch(const LinearParams& p, int x_kind, int w_kind, int shape, hipStream_t s);
+int lin_join_launch(const LinearParams& p, hipStream_t s);
 
 struct LinTile { int e; long long row0; int rows; long long index, total; };   // group, first slot, rows of the tile (<= BM); index of the row tile and number of row tiles
 

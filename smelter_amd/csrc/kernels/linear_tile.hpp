@@ -15,53 +15,137 @@ __device__ __forceinline__ void lin_dma16(const char* base, unsigned off, unsign
 __device__ __forceinline__ unsigned lin_lds_addr(const void* p) { return (unsigned)(size_t)(const __attribute__((address_space(3))) void*)p; }
 __device__ __forceinline__ void lin_arrive() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
-template <int XK, int WK, int WN, int WM, int FN, int FM, bool DMA> struct LinTileShape {
-    static constexpr int THREADS = 64 * WN * WM, BN = 32 * FN * WN, BM = 32 * FM * WM;
+// Which tile (and which run of K) this block has: consecutive tiles stay on one XCD (blocks are dealt to the 8 XCDs in turn), in squares of up to 8 row tiles, so that an XCD's L2 holds what its
+// CUs read together.  The number of row tiles is known on the device only; blocks to spare get an empty tile.
+__device__ __forceinline__ LinTile lin_pick_tile(const LinearParams& p, int BM, int* split, int* nt) {
+    LinTile none; none.rows = 0;
+    *split = p.splits > 1 ? (int)(blockIdx.x % (unsigned)p.splits) : 0;
+    const LinTile all = lin_find_tile(p, BM, 0, true);
+    const long long total = all.total * p.n_tiles;
+    const long long b = p.splits > 1 ? blockIdx.x / (unsigned)p.splits : blockIdx.x, q = total >> 3;
+    const int xcd = (int)(b & 7), rem = (int)(total & 7);
+    if ((b >> 3) >= q + (xcd < rem ? 1 : 0)) return none;
+    const long long id = xcd * q + (xcd < rem ? xcd : rem) + (b >> 3);
+    const long long band = id / (8ll * p.n_tiles);
+    const int in = (int)(id - band * 8 * p.n_tiles), high = (int)(all.total - band * 8 < 8 ? all.total - band * 8 : 8);
+    *nt = in / high;
+    return lin_find_tile(p, BM, band * 8 + in - *nt * high, false);
+}
+// weight row of tile row j: gated tiles alternate 16 gate rows and their 16 up rows
+__device__ __forceinline__ long long lin_weight_row(const LinearParams& p, int n0, int j) {
+    int n = p.gated ? n0 + ((j >> 5) << 4) + (j & 15) : n0 + j;
+    if (n >= p.N) n = p.N - 1;
+    return n + (p.gated && (j & 16) ? (long long)p.N : 0);
+}
+// row of x of tile slot j (behind the tile's end: of its last slot), -1: outside x
+__device__ __forceinline__ long long lin_slot_row(const LinearParams& p, const LinTile& tile, int j) {
+    long long s = tile.row0 + (j < tile.rows ? j : tile.rows - 1);
+    if (p.rows) { s = p.rows[s]; if (s < 0 || s >= p.T) s = -1; }
+    return s;
+}
+
+// Epilogue of the tile kernels: acc[a][b][i] = tile row FR (wn FN + a) + 8 (i / 4) + 4 g + i % 4 of the weights, slot FR (wm FM + b) + r.  The fp32 tile goes through LDS (chunks of four columns, xor-ed with the slot) so that a
+// thread stores eight consecutive columns: whole 512-byte rows instead of 8-byte pieces.  BYTES of LDS, all of it free once every wave is here.  SCALED: wmul[row] = the factor of a weight row.
+template <int FR, int WN, int WM, int FN, int FM, int BYTES, bool SCALED, class AccT>
+__device__ __forceinline__ void lin_finish(const LinearParams& p, const LinTile& tile, int split, int n0, AccT (&acc)[FN][FM], char* lds, const float* wmul) {
+    constexpr int BN = FR * FN * WN, THREADS = 64 * WN * WM;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & (FR - 1), g = lane / FR, wn = wave / WM, wm = wave - wn * WM;
+    const int cols = p.gated ? BN / 2 : BN;
+    constexpr int PB = BYTES / (BN * 4) / (FR * WM) < FM ? BYTES / (BN * 4) / (FR * WM) : FM;   // slot groups of a wave that fit at once
+    const float* bias = p.bias ? p.bias + (long long)tile.e * p.w_rows : nullptr;
+#pragma unroll
+    for (int b0 = 0; b0 < FM; b0 += PB) {
+        __syncthreads();
+#pragma unroll
+        for (int a = 0; a < FN; a++)
+#pragma unroll
+            for (int q = 0; q < FR * FR / 256; q++) {
+                const int j = (wn * FN + a) * (FR / 4) + 2 * q + g;                        // chunk of four columns
+                floatx4 m = {1, 1, 1, 1};
+                if constexpr (SCALED) m = *(const floatx4*)(wmul + 4 * j);
+#pragma unroll
+                for (int b = 0; b < PB; b++) {
+                    const AccT v = acc[a][b0 + b];
+                    *(floatx4*)(lds + ((wm * PB + b) * FR + r) * BN * 4 + ((j ^ (r & 15)) << 4)) = floatx4{v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]} * m;
+                }
+            }
+        __syncthreads();
+        if (p.splits > 1) {                                                         // the sums of a run, in the order of the weight rows; lin_join_kernel adds them
+            constexpr int per = BN / 8;
+            for (int o = tid; o < PB * WM * FR * per; o += THREADS) {
+                const int l = o / per, j = (o - l * per) * 8;
+                const int slot = (l / (FR * PB) * FM + b0) * FR + l % (FR * PB);
+                const int n = p.gated ? n0 + ((j >> 5) << 4) + (j & 15) : n0 + j;
+                if (slot >= tile.rows || n >= p.N) continue;
+                const char* row = lds + l * BN * 4;
+                const int x = l & 15;
+                const bool dead = p.rows && lin_slot_row(p, tile, slot) < 0;
+                floatx4 v[2] = {*(const floatx4*)(row + ((j / 4 ^ x) << 4)), *(const floatx4*)(row + (((j / 4 + 1) ^ x) << 4))};
+                if (dead) v[0] = v[1] = floatx4{0, 0, 0, 0};
+                float* dst = p.part + ((long long)split * p.M + tile.row0 + slot) * p.part_ld + n + (p.gated && (j & 16) ? p.N : 0);
+                if (n + 8 <= p.N && (!p.gated || p.N % 4 == 0)) { *(floatx4*)dst = v[0]; *(floatx4*)(dst + 4) = v[1]; }
+                else {
+#pragma unroll
+                    for (int i = 0; i < 8; i++) if (n + i < p.N) dst[i] = v[i >> 2][i & 3];
+                }
+            }
+            continue;
+        }
+        const int per = cols / 8;
+        for (int o = tid; o < PB * WM * FR * per; o += THREADS) {
+            const int l = o / per, c = o - l * per, n = n0 + c * 8;                 // LDS row, group of eight columns
+            const int slot = (l / (FR * PB) * FM + b0) * FR + l % (FR * PB);
+            if (slot >= tile.rows || n >= p.N) continue;
+            const char* row = lds + l * BN * 4;
+            const int j = p.gated ? (c >> 1) * 8 + (c & 1) * 2 : 2 * c, x = l & 15;
+            float v[8];
+            auto get = [&](int ch, float* q, long long up) {
+                const floatx4 q0 = *(const floatx4*)(row + ((ch ^ x) << 4)), q1 = *(const floatx4*)(row + (((ch + 1) ^ x) << 4));
+#pragma unroll
+                for (int i = 0; i < 4; i++) { q[i] = q0[i]; q[4 + i] = q1[i]; }
+                if (p.rows && lin_slot_row(p, tile, slot) < 0) for (int i = 0; i < 8; i++) q[i] = 0.f;
+                if (bias) for (int i = 0; i < 8; i++) if (n + i < p.N) q[i] += bias[n + i + up];
+            };
+            get(j, v, 0);
+            if (p.gated) {
+                float u[8]; get(j + 4, u, p.N);
+                for (int i = 0; i < 8; i++) v[i] = lin_silu(v[i]) * u[i];
+            } else if (p.act != SM_ACT_NONE) for (int i = 0; i < 8; i++) v[i] = lin_act(v[i], p.act, p.slope);
+            const long long out = (tile.row0 + slot) * p.y_ld + n;
+            if (p.y_vec && n + 8 <= p.N) lin_store8(p.y, out, v, p.y_type);
+            else for (int i = 0; i < 8; i++) if (n + i < p.N) lin_store1(p.y, out + i, v[i], p.y_type);
+        }
+    }
+}
+
+template <int XK, int WK, int FR, int WN, int WM, int FN, int FM, bool DMA> struct LinTileShape {
+    static constexpr int THREADS = 64 * WN * WM, BN = FR * FN * WN, BM = FR * FM * WM;
     static constexpr bool DEQ = WK == SM_MX4 && XK != SM_MX4, MX = XK == SM_MX4;
     static constexpr int STAGE = (BN + BM) * 128;
     static constexpr int SCALES = MX ? 2 * (BN + BM) * 8 : DEQ ? BN * 4 : 0;
     static constexpr int LDS = 2 * STAGE + SCALES;
 };
 
-template <int XK, int WK, int WN, int WM, int FN, int FM, bool DMA>
+template <int XK, int WK, int FR, int WN, int WM, int FN, int FM, bool DMA>
 __global__ __launch_bounds__(64 * WN * WM) void lin_tile_kernel(LinearParams p) {
-    typedef LinTileShape<XK, WK, WN, WM, FN, FM, DMA> S;
+    typedef LinTileShape<XK, WK, FR, WN, WM, FN, FM, DMA> S;
     constexpr int THREADS = S::THREADS, BN = S::BN, BM = S::BM, WAVES = WN * WM;
     constexpr bool DEQ = S::DEQ, MX = S::MX;
     __shared__ __align__(16) char lds[S::LDS];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int r = lane & 31, g = lane >> 5;
+    const int r = lane & (FR - 1), g = lane / FR;
 
-    // ---- which tile: consecutive tiles stay on one XCD (blocks are dealt to the 8 XCDs in turn), in squares of up to 8 row tiles, so that an XCD's L2 holds what its CUs read together
-    const LinTile all = lin_find_tile(p, BM, 0, true);
-    const long long total = all.total * p.n_tiles;
-    long long id;
-    {
-        const long long b = blockIdx.x; const int xcd = (int)(b & 7); const long long q = total >> 3; const int rem = (int)(total & 7);
-        if ((b >> 3) >= q + (xcd < rem ? 1 : 0)) return;
-        id = xcd * q + (xcd < rem ? xcd : rem) + (b >> 3);
-    }
-    const long long band = id / (8ll * p.n_tiles);
-    const int in = (int)(id - band * 8 * p.n_tiles), high = (int)(all.total - band * 8 < 8 ? all.total - band * 8 : 8);
-    const int nt = in / high;
-    const LinTile tile = lin_find_tile(p, BM, band * 8 + in - nt * high, false);
+    int split, nt;
+    const LinTile tile = lin_pick_tile(p, BM, &split, &nt);
     if (tile.rows == 0) return;
     const int row_bytes = MX || DEQ ? 16 * ((p.K + 31) >> 5) : 2 * p.K;             // of a weight row
     const int x_bytes = MX ? row_bytes : 2 * p.K;
-    const int steps = (x_bytes + 127) >> 7, nb = (p.K + 31) >> 5;
+    const int every = (x_bytes + 127) >> 7, nb = (p.K + 31) >> 5;
+    const int first = (int)((long long)every * split / p.splits), steps = (int)((long long)every * (split + 1) / p.splits);   // the steps first .. steps - 1 of all
     const int cols = p.gated ? BN / 2 : BN, n0 = nt * cols;
 
-    // weight row of tile row j: gated tiles alternate 16 gate rows and their 16 up rows
-    auto weight_row = [&](int j) -> long long {
-        int n = p.gated ? n0 + ((j >> 5) << 4) + (j & 15) : n0 + j;
-        if (n >= p.N) n = p.N - 1;
-        return n + (p.gated && (j & 16) ? (long long)p.N : 0);
-    };
-    auto slot_row = [&](int j) -> long long {                                       // row of x of tile slot j, -1: outside x
-        long long s = tile.row0 + (j < tile.rows ? j : tile.rows - 1);
-        if (p.rows) { s = p.rows[s]; if (s < 0 || s >= p.T) s = -1; }
-        return s;
-    };
+    auto weight_row = [&](int j) { return lin_weight_row(p, n0, j); };
+    auto slot_row = [&](int j) { return lin_slot_row(p, tile, j); };
     const char* wexp = p.w + tile.e * p.w_es;
 
     // ---- LDS-DMA: instruction q of a wave fills rows 8 q .. 8 q + 7 of a stage
@@ -99,7 +183,15 @@ __global__ __launch_bounds__(64 * WN * WM) void lin_tile_kernel(LinearParams p) 
             stop[i] = 127;
             if constexpr (XK == SM_F16) {                                           // values relative to the row's largest scale: inside fp16's range whatever the scales are
                 int top = 1;
-                for (int b = tid & 1; b < nb; b += 2) { const int s = ssrc[i][b]; top = top > s ? top : s; }
+                auto up = [&](unsigned v) {
+#pragma unroll
+                    for (int k = 0; k < 32; k += 8) { const int s = v >> k & 255; top = top > s ? top : s; }
+                };
+                for (int b = 16 * (tid & 1); b < nb && nb >= 16; b += 32) {
+                    intx4_t v; __builtin_memcpy(&v, ssrc[i] + (b < nb - 16 ? b : nb - 16), 16);
+                    up(v[0]); up(v[1]); up(v[2]); up(v[3]);
+                }
+                for (int b = 0; b < nb && nb < 16; b++) up(ssrc[i][b]);
                 const int o = __shfl_xor(top, 1); top = top > o ? top : o;
                 stop[i] = top;
                 if (!(tid & 1)) wmul[j] = mx4_scale(top);
@@ -107,12 +199,12 @@ __global__ __launch_bounds__(64 * WN * WM) void lin_tile_kernel(LinearParams p) 
         }
     }
     // scales of MX4 operands: the eight bytes of a step of each row
-    constexpr int SB = MX ? (BN + BM) / THREADS : 1;
+    constexpr int SB = MX ? (BN + BM + THREADS - 1) / THREADS : 1;
     unsigned long long sreg[SB]; const unsigned char* srow[SB];
     if constexpr (MX) {
 #pragma unroll
         for (int i = 0; i < SB; i++) {
-            const int j = i * THREADS + tid;
+            const int j = i * THREADS + tid < BN + BM ? i * THREADS + tid : BN + BM - 1;   // (threads to spare repeat the last row)
             if (j < BN) srow[i] = p.ws + tile.e * p.ws_es + weight_row(j) * p.ws_ld;
             else { const long long s = slot_row(j - BN); srow[i] = p.xs + (s < 0 ? 0 : s) * p.xs_ld; }
         }
@@ -153,7 +245,7 @@ __global__ __launch_bounds__(64 * WN * WM) void lin_tile_kernel(LinearParams p) 
         if constexpr (MX) {
             const int over = nb >= 8 && 8 * t > nb - 8 ? 8 * t - (nb - 8) : 0;      // bytes of the step before, shifted out; behind the end (codes 0) scale 0
 #pragma unroll
-            for (int i = 0; i < SB; i++) *(unsigned long long*)(lds + 2 * S::STAGE + ((t & 1) * (BN + BM) + i * THREADS + tid) * 8) = sreg[i] >> (8 * over);
+            for (int i = 0; i < SB; i++) *(unsigned long long*)(lds + 2 * S::STAGE + ((t & 1) * (BN + BM) + (i * THREADS + tid < BN + BM ? i * THREADS + tid : BN + BM - 1)) * 8) = sreg[i] >> (8 * over);
         }
         if constexpr (DEQ) {
             char* st = lds + (t & 1) * S::STAGE;
@@ -177,69 +269,79 @@ __global__ __launch_bounds__(64 * WN * WM) void lin_tile_kernel(LinearParams p) 
             for (int i = 0; i < QX; i++) *(intx4_t*)(st + BN * 128 + (wave * QX + i) * 1024) = xreg[i];
         }
     };
-    // ---- the products of a step in four phases, one for each 32 bytes of K; a phase's fragments are read during the phase before it (over the step boundary too)
-    constexpr int PH = 4;
+    // ---- the products of a step in four phases (fragments of 32 rows: one for each 32 bytes of K; of 16 rows: one for each 64 bytes of K and each half of the wave's weight rows; 128-row tiles of
+    // them: two phases); a phase's fragments are read during the phase before it (over the step boundary too)
+    typedef float AccT __attribute__((ext_vector_type(FR * FR / 64)));
+    constexpr int GA = FR == 32 ? FN : 4, HA = FN / GA, PH = (FR == 32 ? 4 : 2) * HA;
     const int wn = wave / WM, wm = wave - wn * WM;                                  // this wave's part of the tile
-    floatx16 acc[FN][FM];
+    AccT acc[FN][FM];
 #pragma unroll
     for (int a = 0; a < FN; a++)
 #pragma unroll
         for (int b = 0; b < FM; b++)
 #pragma unroll
-            for (int i = 0; i < 16; i++) acc[a][b][i] = 0.f;
-    intx4_t wf[2][FN], xf[2][FM]; int wsc[2][MX ? FN : 1], xsc[2][MX ? FM : 1];
+            for (int i = 0; i < FR * FR / 64; i++) acc[a][b][i] = 0.f;
+    intx4_t wf[2][GA], xf[2][FM]; int wsc[2][MX ? GA : 1], xsc[2][MX ? FM : 1];
     auto read = [&](int t, auto phase, bool masked) {
-        constexpr int P = decltype(phase)::value, B = P & 1;
-        const char* st = lds + (t & 1) * S::STAGE + r * 128 + (((2 * P + g) ^ (lane & 7)) << 4);
+        constexpr int P = decltype(phase)::value, H = P / HA, A = P % HA, WB = P & 1, XB = H & 1;
+        const int ch = H * (64 / FR) + g;                                           // this lane's chunk of the row
+        const char* st = lds + (t & 1) * S::STAGE + r * 128 + ((ch ^ (lane & 7)) << 4);
 #pragma unroll
-        for (int a = 0; a < FN; a++) wf[B][a] = *(const intx4_t*)(st + (wn * FN + a) * 4096);
+        for (int a = 0; a < GA; a++) wf[WB][a] = *(const intx4_t*)(st + (wn * FN + A * GA + a) * (FR * 128));
+        if constexpr (A == 0) {
 #pragma unroll
-        for (int b = 0; b < FM; b++) xf[B][b] = *(const intx4_t*)(st + (BN / 32 + wm * FM + b) * 4096);
+            for (int b = 0; b < FM; b++) xf[XB][b] = *(const intx4_t*)(st + (BN / FR + wm * FM + b) * (FR * 128));
+        }
         if constexpr (MX) {
-            const unsigned char* sc = (const unsigned char*)lds + 2 * S::STAGE + (t & 1) * (BN + BM) * 8 + r * 8 + g + 2 * P;
+            const unsigned char* sc = (const unsigned char*)lds + 2 * S::STAGE + (t & 1) * (BN + BM) * 8 + r * 8 + ch;
 #pragma unroll
-            for (int a = 0; a < FN; a++) wsc[B][a] = sc[(wn * FN + a) * 256];
+            for (int a = 0; a < GA; a++) wsc[WB][a] = sc[(wn * FN + A * GA + a) * (FR * 8)];
+            if constexpr (A == 0) {
 #pragma unroll
-            for (int b = 0; b < FM; b++) xsc[B][b] = sc[(BN / 32 + wm * FM + b) * 256];
+                for (int b = 0; b < FM; b++) xsc[XB][b] = sc[(BN / FR + wm * FM + b) * (FR * 8)];
+            }
         }
         if (masked) {                                                               // chunks behind the end of the row
-            const bool dead = t * 128 + (2 * P + g) * 16 >= x_bytes;
+            const bool dead = t * 128 + ch * 16 >= x_bytes;
 #pragma unroll
-            for (int a = 0; a < FN; a++) wf[B][a] = dead ? intx4_t{0, 0, 0, 0} : wf[B][a];
+            for (int a = 0; a < GA; a++) wf[WB][a] = dead ? intx4_t{0, 0, 0, 0} : wf[WB][a];
+            if constexpr (A == 0) {
 #pragma unroll
-            for (int b = 0; b < FM; b++) xf[B][b] = dead ? intx4_t{0, 0, 0, 0} : xf[B][b];
+                for (int b = 0; b < FM; b++) xf[XB][b] = dead ? intx4_t{0, 0, 0, 0} : xf[XB][b];
+            }
         }
     };
     auto products = [&](auto phase, auto between) {                                 // between(a): behind the a-th row of tiles
-        constexpr int B = decltype(phase)::value & 1;
-        sm_static_for<0, FN>([&](auto ai) {
+        constexpr int P = decltype(phase)::value, A = P % HA, WB = P & 1, XB = (P / HA) & 1;
+        sm_static_for<0, GA>([&](auto ai) {
             constexpr int a = decltype(ai)::value;
 #pragma unroll
             for (int b = 0; b < FM; b++) {
-                if constexpr (MX) acc[a][b] = lin_mma4(wf[B][a], wsc[B][a], xf[B][b], xsc[B][b], acc[a][b]);
-                else acc[a][b] = lin_mma16<XK>(wf[B][a], xf[B][b], acc[a][b]);
+                AccT& c = acc[A * GA + a][b];
+                if constexpr (MX) c = lin_mma4(wf[WB][a], wsc[WB][a], xf[XB][b], xsc[XB][b], c);
+                else c = lin_mma16<XK>(wf[WB][a], xf[XB][b], c);
             }
             between(a);
         });
     };
     typedef std::integral_constant<int, 0> First; typedef std::integral_constant<int, PH - 1> Last;
-    const bool ragged = DMA && (x_bytes & 127);
-    if (steps > 0) {
+    const bool ragged = DMA && (x_bytes & 127) && steps == every;
+    if (steps > first) {
         if constexpr (DMA) {
 #pragma unroll
-            for (int i = 0; i < QT; i++) fill(0, i);
+            for (int i = 0; i < QT; i++) fill(first, i);
         }
-        load_staged(0, std::false_type()); store_staged(0);
-        if (steps > 1) {
+        load_staged(first, std::false_type()); store_staged(first);
+        if (steps > first + 1) {
             if constexpr (DMA) {
 #pragma unroll
-                for (int i = 0; i < QT / 2; i++) fill(1, i);
+                for (int i = 0; i < QT / 2; i++) fill(first + 1, i);
             }
-            load_staged(1, std::false_type()); store_staged(1);
+            load_staged(first + 1, std::false_type()); store_staged(first + 1);
         }
-        if (steps > 2) load_staged(2, std::false_type());
+        if (steps > first + 2) load_staged(first + 2, std::false_type());
         lin_arrive();
-        read(0, First(), ragged && steps == 1);
+        read(first, First(), ragged && steps == first + 1);
     }
     auto step = [&](int t, auto has1, auto has2) {                                  // has1, has2: steps t + 1, t + 2 exist
         constexpr bool MORE = decltype(has1)::value, MORE2 = decltype(has2)::value;
@@ -249,7 +351,7 @@ __global__ __launch_bounds__(64 * WN * WM) void lin_tile_kernel(LinearParams p) 
                 if (a == 0) { __builtin_amdgcn_sched_barrier(0); read(t, std::integral_constant<int, P + 1>(), !MORE && ragged); __builtin_amdgcn_sched_barrier(0); }
                 if constexpr (DMA && P == 0 && MORE) {                              // the second half of the next step's fill, one instruction at a time
 #pragma unroll
-                    for (int i = QT / 2 + a * (QT - QT / 2) / FN; i < QT / 2 + (a + 1) * (QT - QT / 2) / FN; i++) fill(t + 1, i);
+                    for (int i = QT / 2 + a * (QT - QT / 2) / GA; i < QT / 2 + (a + 1) * (QT - QT / 2) / GA; i++) fill(t + 1, i);
                 }
             });
             __builtin_amdgcn_sched_barrier(0);
@@ -262,74 +364,29 @@ __global__ __launch_bounds__(64 * WN * WM) void lin_tile_kernel(LinearParams p) 
             if constexpr (MORE) if (a == 0) { __builtin_amdgcn_sched_barrier(0); read(t + 1, First(), !MORE2 && ragged); __builtin_amdgcn_sched_barrier(0); }
             if constexpr (DMA && MORE2) {                                           // the first half of the fill behind it
 #pragma unroll
-                for (int i = a * (QT / 2) / FN; i < (a + 1) * (QT / 2) / FN; i++) fill(t + 2, i);
+                for (int i = a * (QT / 2) / GA; i < (a + 1) * (QT / 2) / GA; i++) fill(t + 2, i);
             }
         });
         __builtin_amdgcn_sched_barrier(0);
     };
-    int t = 0;
+    int t = first;
 #pragma unroll 1
     for (; t + 2 < steps; t++) step(t, std::true_type(), std::true_type());
     if (t + 1 < steps) { step(t, std::true_type(), std::false_type()); t++; }
     if (t < steps) step(t, std::false_type(), std::false_type());
 
-    // ---- epilogue: acc[a][b][i] = tile row 32 (wn FN + a) + 8 (i / 4) + 4 g + i % 4 of the weights, slot 32 (wm FM + b) + r.  The fp32 tile goes through LDS (chunks of four columns, xor-ed with the slot) so that a
-    // thread stores eight consecutive columns: whole 512-byte rows instead of 8-byte pieces.
-    constexpr int PB = 2 * S::STAGE / (BN * 4) / (32 * WM) < FM ? 2 * S::STAGE / (BN * 4) / (32 * WM) : FM;   // slot groups of a wave that fit at once
-    const float* bias = p.bias ? p.bias + (long long)tile.e * p.w_rows : nullptr;
-#pragma unroll
-    for (int b0 = 0; b0 < FM; b0 += PB) {
-        __syncthreads();
-#pragma unroll
-        for (int a = 0; a < FN; a++)
-#pragma unroll
-            for (int q = 0; q < 4; q++) {
-                const int j = (wn * FN + a) * 8 + 2 * q + g;                        // chunk of four columns
-                floatx4 m = {1, 1, 1, 1};
-                if constexpr (DEQ && XK == SM_F16) m = *(const floatx4*)(wmul + 4 * j);
-#pragma unroll
-                for (int b = 0; b < PB; b++) {
-                    const floatx16 v = acc[a][b0 + b];
-                    *(floatx4*)(lds + ((wm * PB + b) * 32 + r) * BN * 4 + ((j ^ (r & 15)) << 4)) = floatx4{v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]} * m;
-                }
-            }
-        __syncthreads();
-        const int per = cols / 8;
-        for (int o = tid; o < PB * WM * 32 * per; o += THREADS) {
-            const int l = o / per, c = o - l * per, n = n0 + c * 8;                 // LDS row, group of eight columns
-            const int slot = (l / (32 * PB) * FM + b0) * 32 + l % (32 * PB);
-            if (slot >= tile.rows || n >= p.N) continue;
-            const char* row = lds + l * BN * 4;
-            const int j = p.gated ? (c >> 1) * 8 + (c & 1) * 2 : 2 * c, x = l & 15;
-            float v[8];
-            auto get = [&](int ch, float* q, long long up) {
-                const floatx4 q0 = *(const floatx4*)(row + ((ch ^ x) << 4)), q1 = *(const floatx4*)(row + (((ch + 1) ^ x) << 4));
-#pragma unroll
-                for (int i = 0; i < 4; i++) { q[i] = q0[i]; q[4 + i] = q1[i]; }
-                if (p.rows && slot_row(slot) < 0) for (int i = 0; i < 8; i++) q[i] = 0.f;
-                if (bias) for (int i = 0; i < 8; i++) if (n + i < p.N) q[i] += bias[n + i + up];
-            };
-            get(j, v, 0);
-            if (p.gated) {
-                float u[8]; get(j + 4, u, p.N);
-                for (int i = 0; i < 8; i++) v[i] = lin_silu(v[i]) * u[i];
-            } else if (p.act != SM_ACT_NONE) for (int i = 0; i < 8; i++) v[i] = lin_act(v[i], p.act, p.slope);
-            const long long out = (tile.row0 + slot) * p.y_ld + n;
-            if (p.y_vec && n + 8 <= p.N) lin_store8(p.y, out, v, p.y_type);
-            else for (int i = 0; i < 8; i++) if (n + i < p.N) lin_store1(p.y, out + i, v[i], p.y_type);
-        }
-    }
+    lin_finish<FR, WN, WM, FN, FM, 2 * S::STAGE, DEQ && XK == SM_F16>(p, tile, split, n0, acc, lds, wmul);
 }
 
-template <int XK, int WK, int WN, int WM, int FN, int FM, bool DMA> static int lin_tile(const LinearParams& q, hipStream_t s) {
-    typedef LinTileShape<XK, WK, WN, WM, FN, FM, DMA> S;
+template <int XK, int WK, int FR, int WN, int WM, int FN, int FM, bool DMA> static int lin_tile(const LinearParams& q, hipStream_t s) {
+    typedef LinTileShape<XK, WK, FR, WN, WM, FN, FM, DMA> S;
     LinearParams p = q;
     const int cols = p.gated ? S::BN / 2 : S::BN;
     p.n_tiles = (p.N + cols - 1) / cols;
     p.m_tiles = lin_row_tiles(p, S::BM);
-    const long long blocks = (p.m_tiles * p.n_tiles + 7) / 8 * 8;
+    const long long blocks = (p.m_tiles * p.n_tiles + 7) / 8 * 8 * p.splits;
     SM_REQUIRE(blocks < (1ll << 31), "linear: %lld row tiles x %d column tiles exceed one launch", p.m_tiles, p.n_tiles);
-    lin_tile_kernel<XK, WK, WN, WM, FN, FM, DMA><<<dim3((unsigned)blocks), S::THREADS, 0, s>>>(p);
+    lin_tile_kernel<XK, WK, FR, WN, WM, FN, FM, DMA><<<dim3((unsigned)blocks), S::THREADS, 0, s>>>(p);
     SM_LAUNCH_CHECK();
     return SM_OK;
 }

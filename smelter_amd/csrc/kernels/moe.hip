@@ -214,7 +214,19 @@ extern "C" int sm_moe_route(const void* scores, int32_t type, int64_t T, int32_t
 
 // out[t, n] = sum_j weights[t, j] * y[slots[t, j], n]: one thread per eight columns of a token, terms added in the order of j in fp32, one rounding; a slot outside 0 .. M - 1 adds nothing.
 // Bound by the reading of the k rows.
-template <int KIND> __global__ void combine_kernel(const char* y, long long M, int N, long long y_ld, const float* weights, const int* slots, long long T, int k, void* out, long long out_ld, int vec) {
+template <int KIND> __device__ __forceinline__ void combine_load8(const char* row, int c, int N, float* v) {
+    if constexpr (KIND == SM_F32) {
+        const float* q = (const float*)row + c;
+        if (c + 8 <= N) __builtin_memcpy(v, q, 32);
+        else for (int i = 0; i < 8; i++) v[i] = c + i < N ? q[i] : 0.f;
+    } else {
+        const intx4_t b = lin_load8(row, c, N);
+        if constexpr (KIND == SM_F16) { const half8_t h = __builtin_bit_cast(half8_t, b); for (int i = 0; i < 8; i++) v[i] = (float)h[i]; }
+        else { const bf16x8_t h = __builtin_bit_cast(bf16x8_t, b); for (int i = 0; i < 8; i++) v[i] = (float)h[i]; }
+    }
+}
+template <int KIND> __global__ void combine_kernel(const char* y, long long M, int N, long long y_ld, const float* weights, const int* slots, long long T, int k, void* out, int out_type, long long out_ld,
+                                                   int vec) {
     const int chunks = (N + 7) / 8;
     const long long units = T * chunks;
     for (long long u = (long long)blockIdx.x * blockDim.x + threadIdx.x; u < units; u += (long long)gridDim.x * blockDim.x) {
@@ -225,31 +237,30 @@ template <int KIND> __global__ void combine_kernel(const char* y, long long M, i
             const int at = slots[t * k + j];
             if (at < 0 || at >= M) continue;
             const float w = weights[t * k + j];
-            const intx4_t v = lin_load8(y + 2ll * at * y_ld, c, N);
-            if constexpr (KIND == SM_F16) { const half8_t h = __builtin_bit_cast(half8_t, v); for (int i = 0; i < 8; i++) s[i] += w * (float)h[i]; }
-            else { const bf16x8_t h = __builtin_bit_cast(bf16x8_t, v); for (int i = 0; i < 8; i++) s[i] += w * (float)h[i]; }
+            float v[8]; combine_load8<KIND>(y + (KIND == SM_F32 ? 4ll : 2ll) * at * y_ld, c, N, v);
+            for (int i = 0; i < 8; i++) s[i] += w * v[i];
         }
         const long long o = t * out_ld + c;
-        if (vec && c + 8 <= N) {
-            if constexpr (KIND == SM_F16) { half8_t h; for (int i = 0; i < 8; i++) h[i] = (half_t)s[i]; *(half8_t*)((half_t*)out + o) = h; }
-            else { bf16x8_t h; for (int i = 0; i < 8; i++) h[i] = (bf16_t)s[i]; *(bf16x8_t*)((bf16_t*)out + o) = h; }
-        } else for (int i = 0; i < 8; i++) if (c + i < N) lin_store1(out, o + i, s[i], KIND);
+        if (vec && c + 8 <= N) lin_store8(out, o, s, out_type);
+        else for (int i = 0; i < 8; i++) if (c + i < N) lin_store1(out, o + i, s[i], out_type);
     }
 }
 
-extern "C" int sm_moe_combine(const void* y, int32_t type, int64_t M, int32_t N, int64_t y_ld, const float* weights, const int32_t* slots, int64_t T, int32_t k, void* out, int64_t out_ld,
-                              sm_stream_t stream) {
-    SM_REQUIRE(type == SM_F16 || type == SM_BF16, "moe_combine: type %d is not fp16 or bf16", type);
+extern "C" int sm_moe_combine(const void* y, int32_t type, int64_t M, int32_t N, int64_t y_ld, const float* weights, const int32_t* slots, int64_t T, int32_t k, void* out, int32_t out_type,
+                              int64_t out_ld, sm_stream_t stream) {
+    SM_REQUIRE((type == SM_F16 || type == SM_BF16 || type == SM_F32) && (out_type == SM_F16 || out_type == SM_BF16 || out_type == SM_F32), "moe_combine: types %d -> %d (taken: fp16, bf16, fp32)", type, out_type);
     SM_REQUIRE(M >= 0 && N >= 0 && T >= 0 && k >= 0 && M < (1ll << 31) && T < (1ll << 31) && N <= (1 << 29), "moe_combine: sizes M %lld, N %d, T %lld, k %d", (long long)M, N, (long long)T, k);
     if (T == 0 || N == 0) return SM_OK;
     SM_REQUIRE(out && (k == 0 || (weights && slots)) && (k == 0 || M == 0 || y), "moe_combine: null operand");
     SM_REQUIRE((M <= 1 || y_ld >= N) && (T == 1 || out_ld >= N), "moe_combine: row strides %lld, %lld below the %d columns", (long long)y_ld, (long long)out_ld, N);
-    SM_REQUIRE((size_t)y % 2 == 0 && (size_t)out % 2 == 0, "moe_combine: an operand is not aligned to its element");
-    const int vec = (size_t)out % 16 == 0 && (T == 1 || out_ld % 8 == 0);
+    const int oe = out_type == SM_F32 ? 4 : 2;
+    SM_REQUIRE((size_t)y % (type == SM_F32 ? 4 : 2) == 0 && (size_t)out % oe == 0, "moe_combine: an operand is not aligned to its element");
+    const int vec = (size_t)out % 16 == 0 && (T == 1 || out_ld * oe % 16 == 0);
     const long long units = T * ((N + 7) / 8), want = (units + 255) / 256, cap = (long long)SM_NUM_CU * 32;
     const dim3 grid((unsigned)(want < cap ? want : cap));
-    if (type == SM_F16) combine_kernel<SM_F16><<<grid, 256, 0, sm_s(stream)>>>((const char*)y, M, N, y_ld, weights, slots, T, k, out, out_ld, vec);
-    else combine_kernel<SM_BF16><<<grid, 256, 0, sm_s(stream)>>>((const char*)y, M, N, y_ld, weights, slots, T, k, out, out_ld, vec);
+    if (type == SM_F16) combine_kernel<SM_F16><<<grid, 256, 0, sm_s(stream)>>>((const char*)y, M, N, y_ld, weights, slots, T, k, out, out_type, out_ld, vec);
+    else if (type == SM_BF16) combine_kernel<SM_BF16><<<grid, 256, 0, sm_s(stream)>>>((const char*)y, M, N, y_ld, weights, slots, T, k, out, out_type, out_ld, vec);
+    else combine_kernel<SM_F32><<<grid, 256, 0, sm_s(stream)>>>((const char*)y, M, N, y_ld, weights, slots, T, k, out, out_type, out_ld, vec);
     SM_LAUNCH_CHECK();
     return SM_OK;
 }

@@ -559,31 +559,33 @@ class MoePlan(NamedTuple):
     slots: torch.Tensor
 
 
-def _require(cond, msg, *args):
-    if not cond:
-        raise SmelterError(-13, msg % args)
+def _refuse(msg, *args):
+    raise SmelterError(-13, msg % args)
 
 
-def _on(dev, call, *args):
-    """run an enqueueing entry point on the current stream of `dev`"""
-    if dev.index == torch.cuda.current_device():
-        check(call(*args, torch.cuda.current_stream(dev).cuda_stream))
+def _on(index, call, *args):
+    """run an enqueueing entry point on the current stream of device `index`"""
+    if index == torch.cuda.current_device():
+        rc = call(*args, torch._C._cuda_getCurrentRawStream(index))        # (torch.cuda.current_stream(index).cuda_stream without the Stream object: 2 us of a 4 us call)
     else:
-        with torch.cuda.device(dev):
-            check(call(*args, torch.cuda.current_stream(dev).cuda_stream))
+        with torch.cuda.device(index):
+            rc = call(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc:
+        check(rc)
 
 
 def _rows2d(t, name):
     """(rows, columns, row stride) of a tensor [..., K] whose leading axes are evenly strided"""
-    _require(t.dim() >= 1, "%s: a tensor with at least one axis is wanted", name)
+    if t.dim() < 1:
+        _refuse("%s: a tensor with at least one axis is wanted", name)
     k = t.shape[-1]
     n = t.numel() // k if k else 0
-    if n <= 1 or k == 0:
-        _require(k <= 1 or t.stride(-1) == 1, "%s: the last axis must be innermost", name)
-        return n, k, k
     if t.is_contiguous():
         return n, k, k
-    _require(t.stride(-1) == 1 or k == 1, "%s: the last axis must be innermost", name)
+    if t.stride(-1) != 1 and k > 1:
+        _refuse("%s: the last axis must be innermost", name)
+    if n <= 1:
+        return n, k, k
     ld, step = None, None
     for size, stride in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
         if size == 1:
@@ -591,155 +593,192 @@ def _rows2d(t, name):
         if ld is None:
             ld, step = stride, size * stride
         else:
-            _require(stride == step, "%s: the leading axes must be evenly strided", name)
+            if stride != step:
+                _refuse("%s: the leading axes must be evenly strided", name)
             step *= size
-    _require(ld >= k, "%s: rows overlap (stride %d, %d columns)", name, ld, k)
+    if ld < k:
+        _refuse("%s: rows overlap (stride %d, %d columns)", name, ld, k)
     return n, k, ld
 
 
-def _gpu(dev, name, t, dtypes):
-    _require(isinstance(t, torch.Tensor) and t.is_cuda and (dev is None or t.device == dev), "%s: a tensor on %s is wanted", name, dev or "the GPU")
-    _require(t.dtype in dtypes, "%s: type %s is not taken", name, t.dtype)
+def _gpu(index, name, t, dtypes):
+    """the device index of a tensor of one of `dtypes` (on device `index`, if given)"""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        _refuse("%s: a tensor on the GPU is wanted", name)
+    if t.dtype not in dtypes:
+        _refuse("%s: type %s is not taken", name, t.dtype)
+    at = t.get_device()
+    if index is not None and at != index:
+        _refuse("%s: tensors on devices %d and %d", name, index, at)
+    return at
 
 
-def _check_mx4(q, dev, name):
-    _require(isinstance(q, Mx4), "%s: an Mx4 tensor is wanted", name)
-    _gpu(dev, name, q.codes, (torch.uint8,))
-    _gpu(q.codes.device, name, q.scales, (torch.uint8,))
-    nb = (q.k + 31) // 32
-    _require(q.k >= 0 and q.codes.dim() >= 1 and q.codes.shape == (*q.scales.shape[:-1], 16 * nb) and q.scales.shape[-1] == nb, "%s: codes %s and scales %s for %d columns", name,
-             tuple(q.codes.shape), tuple(q.scales.shape), q.k)
-    _require(q.codes.is_contiguous() and q.scales.is_contiguous() and q.codes.data_ptr() % 16 == 0, "%s: codes and scales must be contiguous, codes 16-byte aligned", name)
+_BYTES, _INTS, _HALVES, _FLOATS = (torch.uint8,), (torch.int32,), (torch.float16, torch.bfloat16), (torch.float32,)
+
+
+def _check_mx4(q, index, name):
+    if not isinstance(q, Mx4):
+        _refuse("%s: an Mx4 tensor is wanted", name)
+    c, s, k = q
+    index = _gpu(index, name, c, _BYTES)
+    _gpu(index, name, s, _BYTES)
+    nb, cs, ss = (k + 31) // 32, c.shape, s.shape
+    if k < 0 or not cs or len(cs) != len(ss) or cs[-1] != 16 * nb or ss[-1] != nb or cs[:-1] != ss[:-1]:
+        _refuse("%s: codes %s and scales %s for %d columns", name, tuple(cs), tuple(ss), k)
+    if not c.is_contiguous() or not s.is_contiguous() or c.data_ptr() & 15:
+        _refuse("%s: codes and scales must be contiguous, codes 16-byte aligned", name)
+    return index
 
 
 def mx4_quantize(x):
     """fp16 / bf16 / fp32 [..., K] -> Mx4 (sm_mx4_quantize): blocks of 32 along the last axis, scale 2^(floor(log2 amax) - 2), elements to the nearest e2m1 value, ties to even, at most 6 scales.
     A block with a NaN or an infinity becomes NaN."""
-    _gpu(None, "mx4_quantize", x, _TYPES)
+    index = _gpu(None, "mx4_quantize", x, _TYPES)
     rows, k, ld = _rows2d(x, "mx4_quantize")
-    nb = (k + 31) // 32
-    codes = torch.empty((*x.shape[:-1], 16 * nb), dtype=torch.uint8, device=x.device)
-    scales = torch.empty((*x.shape[:-1], nb), dtype=torch.uint8, device=x.device)
-    _on(x.device, lib().sm_mx4_quantize, x.data_ptr(), _TYPES[x.dtype], rows, k, ld, codes.data_ptr(), scales.data_ptr())
+    nb, lead = (k + 31) // 32, x.shape[:-1]
+    codes, scales = x.new_empty((*lead, 16 * nb), dtype=torch.uint8), x.new_empty((*lead, nb), dtype=torch.uint8)
+    _on(index, lib().sm_mx4_quantize, x.data_ptr(), _TYPES[x.dtype], rows, k, ld, codes.data_ptr(), scales.data_ptr())
     return Mx4(codes, scales, k)
 
 
 def mx4_dequantize(q, dtype=torch.float16, out=None):
     """the values of an Mx4 tensor, rounded once to `dtype` (sm_mx4_dequantize)"""
-    _check_mx4(q, None, "mx4_dequantize")
+    index = _check_mx4(q, None, "mx4_dequantize")
     if out is None:
-        _require(dtype in _TYPES, "mx4_dequantize: type %s is not taken", dtype)
-        out = torch.empty(q.shape, dtype=dtype, device=q.codes.device)
-    _gpu(q.codes.device, "mx4_dequantize", out, _TYPES)
-    _require(tuple(out.shape) == tuple(q.shape), "mx4_dequantize: output %s for %s", tuple(out.shape), tuple(q.shape))
+        if dtype not in _TYPES:
+            _refuse("mx4_dequantize: type %s is not taken", dtype)
+        out = q.codes.new_empty(q.shape, dtype=dtype)
+    else:
+        _gpu(index, "mx4_dequantize", out, _TYPES)
+        if tuple(out.shape) != q.shape:
+            _refuse("mx4_dequantize: output %s for %s", tuple(out.shape), q.shape)
     rows, k, ld = _rows2d(out, "mx4_dequantize")
-    _on(out.device, lib().sm_mx4_dequantize, q.codes.data_ptr(), q.scales.data_ptr(), rows, k, out.data_ptr(), _TYPES[out.dtype], ld)
+    _on(index, lib().sm_mx4_dequantize, q.codes.data_ptr(), q.scales.data_ptr(), rows, k, out.data_ptr(), _TYPES[out.dtype], ld)
     return out
 
 
-def _linear(name, x, w, lead, m, offsets, rows, bias, act, slope, gated, out, dtype):
-    """the checks and the call that mx4_linear and expert_linear share; `lead` = leading axes of the weights (() or (E,)), m = slots (None: one per row of x)"""
-    x4 = isinstance(x, Mx4)
-    xt = x.codes if x4 else x
-    if x4:
-        _check_mx4(x, None, name)
-        xk, x_ld = x.k, 0
-        _require(len(x.shape) == 2, "%s: x must be [rows, K]", name)
+def _linear(name, x, w, lead, offsets, rows, bias, act, slope, gated, out, dtype):
+    """the checks and the call that mx4_linear and expert_linear share; `lead` = leading axes of the weights (0 or 1)"""
+    if isinstance(x, Mx4):
+        index = _check_mx4(x, None, name)
+        xt, xs, x_type, xk, x_ld = x.codes, x.scales.data_ptr(), _MX4, x.k, 0
+        if xt.dim() != 2:
+            _refuse("%s: x must be [rows, K]", name)
     else:
-        _gpu(None, name, x, (torch.float16, torch.bfloat16))
-        _require(x.dim() == 2, "%s: x must be [rows, K]", name)
+        index = _gpu(None, name, x, _HALVES)
+        if x.dim() != 2:
+            _refuse("%s: x must be [rows, K]", name)
+        xt, xs, x_type = x, None, _TYPES[x.dtype]
         _, xk, x_ld = _rows2d(x, name)
-    dev = xt.device
     if isinstance(w, Mx4):
-        _check_mx4(w, dev, name)
-        w_type, wc, wsc = _MX4, w.codes, w.scales.data_ptr()
+        _check_mx4(w, index, name)
+        wc, wsc, w_type, wk = w.codes, w.scales.data_ptr(), _MX4, w.k
     else:
-        _gpu(dev, name, w, (torch.float16, torch.bfloat16))
-        _require(not x4 and w.dtype == x.dtype, "%s: weights of type %s under x of type %s", name, w.dtype, "MX4" if x4 else x.dtype)
-        _require(w.is_contiguous(), "%s: weights must be contiguous", name)
-        w_type, wc, wsc = _TYPES[w.dtype], w, None
-    ws = w.shape
-    _require(len(ws) == lead + 2 and ws[-1] == xk, "%s: weights %s for x with %d columns", name, tuple(ws), xk)
-    t, n, e = xt.shape[0], ws[-2], ws[0] if lead else 1
-    if gated:
-        _require(n % 2 == 0, "%s: a gated layer has an even number of weight rows (%d)", name, n)
-        n //= 2
-    if m is None:
-        m = t
-    if out is None:
-        dtype = dtype or (torch.float16 if x4 else x.dtype)
-        _require(dtype in _TYPES, "%s: output type %s is not taken", name, dtype)
-        out = torch.empty((m, n), dtype=dtype, device=dev)
-    else:
-        _gpu(dev, name, out, _TYPES)
-        _require(dtype is None or dtype == out.dtype, "%s: out is %s, dtype %s", name, out.dtype, dtype)
-        _require(out.shape == (m, n), "%s: output %s, wanted %s", name, tuple(out.shape), (m, n))
-    y_ld = n if out.is_contiguous() else _rows2d(out, name)[2]
+        _gpu(index, name, w, _HALVES)
+        wc, wsc, w_type = w, None, _TYPES[w.dtype]
+        if w_type != x_type:
+            _refuse("%s: weights of type %s under x of type %s", name, w.dtype, "MX4" if x_type == _MX4 else x.dtype)
+        if not w.is_contiguous():
+            _refuse("%s: weights must be contiguous", name)
+        wk = w.shape[-1]
+    wsh = wc.shape
+    if len(wsh) != lead + 2 or wk != xk:
+        _refuse("%s: weights %s for x with %d columns", name, tuple(w.shape), xk)
+    t, n, e = xt.shape[0], wsh[-2], wsh[0] if lead else 1
+    m = t if rows is None else rows.shape[0]
     if bias is not None:
-        _gpu(dev, name, bias, (torch.float32,))
-        _require(bias.is_contiguous() and bias.shape == ws[:-1], "%s: bias %s for weights %s", name, tuple(bias.shape), tuple(ws))
-    d = LinearDesc(m, t, n, xk, e, _MX4 if x4 else _TYPES[x.dtype], w_type, _TYPES[out.dtype], act, slope, 1 if gated else 0, x_ld, y_ld)
-    _on(dev, lib().sm_linear_fwd, C.byref(d), xt.data_ptr(), x.scales.data_ptr() if x4 else None, wc.data_ptr(), wsc, bias.data_ptr() if bias is not None else None,
-        offsets.data_ptr() if offsets is not None else None, rows.data_ptr() if rows is not None else None, out.data_ptr())
+        _gpu(index, name, bias, _FLOATS)
+        if not bias.is_contiguous() or bias.shape != wsh[:-1]:
+            _refuse("%s: bias %s for weights %s", name, tuple(bias.shape), tuple(w.shape))
+    if gated:
+        if n % 2:
+            _refuse("%s: a gated layer has an even number of weight rows (%d)", name, n)
+        n //= 2
+    if out is None:
+        if dtype is None:
+            dtype = torch.float16 if x_type == _MX4 else x.dtype
+        elif dtype not in _TYPES:
+            _refuse("%s: output type %s is not taken", name, dtype)
+        out, y_ld = xt.new_empty((m, n), dtype=dtype), n
+    else:
+        _gpu(index, name, out, _TYPES)
+        if dtype is not None and dtype != out.dtype:
+            _refuse("%s: out is %s, dtype %s", name, out.dtype, dtype)
+        if out.shape != (m, n):
+            _refuse("%s: output %s, wanted %s", name, tuple(out.shape), (m, n))
+        y_ld = _rows2d(out, name)[2]
+    L = lib()
+    d = C.byref(LinearDesc(m, t, n, xk, e, x_type, w_type, _TYPES[out.dtype], act, slope, 1 if gated else 0, x_ld, y_ld))
+    wsb = L.sm_linear_workspace_bytes(d, offsets is not None, rows is not None)
+    work = xt.new_empty((wsb,), dtype=torch.uint8) if wsb else None
+    _on(index, L.sm_linear_fwd, d, xt.data_ptr(), xs, wc.data_ptr(), wsc, bias.data_ptr() if bias is not None else None, offsets.data_ptr() if offsets is not None else None,
+        rows.data_ptr() if rows is not None else None, out.data_ptr(), work.data_ptr() if wsb else None, wsb)
     return out
 
 
 def mx4_linear(x, w, bias=None, act=ACT_NONE, slope=0.0, gated=False, out=None, dtype=None):
     """act(x . w^T + bias) with MX4 weights w [N, K] (sm_linear_fwd).  x [M, K]: fp16 or bf16 (the weights are read as 16-bit values, the output has x's type or fp32), or an Mx4 tensor (both
     sides in 4 bits; dtype fp16 (default), bf16 or fp32).  gated: w has 2 N rows and the result is silu(first N columns) * last N.  bias fp32 [rows of w]."""
-    _require(isinstance(w, Mx4), "mx4_linear: the weights must be an Mx4 tensor")
-    return _linear("mx4_linear", x, w, 0, None, None, None, bias, act, slope, gated, out, dtype)
+    if not isinstance(w, Mx4):
+        _refuse("mx4_linear: the weights must be an Mx4 tensor")
+    return _linear("mx4_linear", x, w, 0, None, None, bias, act, slope, gated, out, dtype)
 
 
 def expert_linear(x, w, offsets, rows=None, bias=None, act=ACT_NONE, slope=0.0, gated=False, out=None, dtype=None):
     """Products grouped by expert (sm_linear_fwd): slot s of group e (offsets[e] <= s < offsets[e + 1]) gets act(x[rows[s]] . w[e]^T + bias[e]); without `rows` slot s is row s of x.
     x [T, K] and w [E, N, K]: both fp16, both bf16, 16-bit x on Mx4 weights, or both Mx4.  offsets int32 [E + 1], rows int32 [slots], both on the GPU (MoePlan holds them): nothing is
     read back to the host.  Slots that no group covers are left as they were (in a new `out`: unspecified).  gated, bias [E, rows of w], dtype: as in mx4_linear."""
-    dev = x.codes.device if isinstance(x, Mx4) else x.device
-    _gpu(dev, "expert_linear", offsets, (torch.int32,))
-    e = w.codes.shape[0] if isinstance(w, Mx4) else w.shape[0]
-    _require(offsets.is_contiguous() and offsets.shape == (e + 1,) and e >= 1, "expert_linear: offsets %s for %d experts", tuple(offsets.shape), e)
-    m = None
+    index = _gpu(None, "expert_linear", offsets, _INTS)
+    wc = w.codes if isinstance(w, Mx4) else w
+    _gpu(index, "expert_linear", x.codes if isinstance(x, Mx4) else x, (torch.float16, torch.bfloat16, torch.uint8))
+    e = wc.shape[0] if isinstance(wc, torch.Tensor) and wc.dim() else 0
+    if e < 1 or not offsets.is_contiguous() or offsets.shape != (e + 1,):
+        _refuse("expert_linear: offsets %s for %d experts", tuple(offsets.shape), e)
     if rows is not None:
-        _gpu(dev, "expert_linear", rows, (torch.int32,))
-        _require(rows.dim() == 1 and rows.is_contiguous(), "expert_linear: rows must be a contiguous vector")
-        m = rows.shape[0]
-    return _linear("expert_linear", x, w, 1, m, offsets, rows, bias, act, slope, gated, out, dtype)
+        _gpu(index, "expert_linear", rows, _INTS)
+        if rows.dim() != 1 or not rows.is_contiguous():
+            _refuse("expert_linear: rows must be a contiguous vector")
+    return _linear("expert_linear", x, w, 1, offsets, rows, bias, act, slope, gated, out, dtype)
 
 
 def moe_route(scores, k, renormalize=True):
     """The k largest of each token's scores [T, E] (fp16 / bf16 / fp32; ties: the lower index), their softmax weights (over the chosen ones, or over all E) and the order of the assignments
     by expert (sm_moe_route) -> MoePlan.  A score of -inf or NaN is never chosen."""
-    _gpu(None, "moe_route", scores, _TYPES)
-    _require(scores.dim() == 2, "moe_route: scores must be [tokens, experts]")
+    index = _gpu(None, "moe_route", scores, _TYPES)
+    if scores.dim() != 2:
+        _refuse("moe_route: scores must be [tokens, experts]")
     t, e = scores.shape
-    _require(1 <= e <= 1024 and 1 <= k <= min(e, 32), "moe_route: %d of %d experts (taken: up to 1024 experts, 1 .. min(32, experts) of them)", k, e)
+    if not 1 <= e <= 1024 or not 1 <= k <= min(e, 32):
+        _refuse("moe_route: %d of %d experts (taken: up to 1024 experts, 1 .. min(32, experts) of them)", k, e)
     ld = e if scores.is_contiguous() else _rows2d(scores, "moe_route")[2]
-    dev, n, ws = scores.device, t * k, lib().sm_moe_route_workspace_bytes(t, e, k)
-    weights = torch.empty((t, k), dtype=torch.float32, device=dev)
-    ints = torch.empty((3 * n + e + 1 + ws // 4,), dtype=torch.int32, device=dev)      # one allocation; the workspace behind the results
-    experts, slots, rows, offsets, work = ints[:n].view(t, k), ints[n:2 * n].view(t, k), ints[2 * n:3 * n], ints[3 * n:3 * n + e + 1], ints[3 * n + e + 1:]
-    _on(dev, lib().sm_moe_route, scores.data_ptr(), _TYPES[scores.dtype], t, e, k, ld, 1 if renormalize else 0, weights.data_ptr(), experts.data_ptr(), offsets.data_ptr(), rows.data_ptr(),
+    L, n = lib(), t * k
+    ws = L.sm_moe_route_workspace_bytes(t, e, k)
+    weights = scores.new_empty((t, k), dtype=torch.float32)
+    # the integers in one allocation, the workspace behind the results
+    experts, slots, rows, offsets, work = scores.new_empty((3 * n + e + 1 + ws // 4,), dtype=torch.int32).split_with_sizes((n, n, n, e + 1, ws // 4))
+    _on(index, L.sm_moe_route, scores.data_ptr(), _TYPES[scores.dtype], t, e, k, ld, 1 if renormalize else 0, weights.data_ptr(), experts.data_ptr(), offsets.data_ptr(), rows.data_ptr(),
         slots.data_ptr(), work.data_ptr(), ws)
-    return MoePlan(weights, experts, offsets, rows, slots)
+    return MoePlan(weights, experts.view(t, k), offsets, rows, slots.view(t, k))
 
 
-def moe_combine(y, slots, weights, out=None):
-    """out[t] = sum_j weights[t, j] * y[slots[t, j]] (sm_moe_combine): y fp16 / bf16 [M, N], slots int32 [T, k] (negative: nothing), weights fp32 [T, k]; fp32 sums in the order of j"""
-    _gpu(None, "moe_combine", y, (torch.float16, torch.bfloat16))
-    dev = y.device
-    _gpu(dev, "moe_combine", slots, (torch.int32,))
-    _gpu(dev, "moe_combine", weights, (torch.float32,))
-    _require(y.dim() == 2 and slots.dim() == 2 and slots.shape == weights.shape and slots.is_contiguous() and weights.is_contiguous(), "moe_combine: y %s, slots %s, weights %s",
-             tuple(y.shape), tuple(slots.shape), tuple(weights.shape))
+def moe_combine(y, slots, weights, out=None, dtype=None):
+    """out[t] = sum_j weights[t, j] * y[slots[t, j]] (sm_moe_combine): y fp16 / bf16 / fp32 [M, N], slots int32 [T, k] (negative: nothing), weights fp32 [T, k]; fp32 sums in the order of j,
+    one rounding to `dtype` (default: y's own)"""
+    index = _gpu(None, "moe_combine", y, _TYPES)
+    _gpu(index, "moe_combine", slots, _INTS)
+    _gpu(index, "moe_combine", weights, _FLOATS)
+    if y.dim() != 2 or slots.dim() != 2 or slots.shape != weights.shape or not slots.is_contiguous() or not weights.is_contiguous():
+        _refuse("moe_combine: y %s, slots %s, weights %s", tuple(y.shape), tuple(slots.shape), tuple(weights.shape))
     m, n = y.shape
     t, k = slots.shape
     if out is None:
-        out = torch.empty((t, n), dtype=y.dtype, device=dev)
+        if dtype is not None and dtype not in _TYPES:
+            _refuse("moe_combine: type %s is not taken", dtype)
+        out, o_ld = y.new_empty((t, n), dtype=dtype or y.dtype), n
     else:
-        _gpu(dev, "moe_combine", out, (y.dtype,))
-        _require(out.shape == (t, n), "moe_combine: output %s, wanted %s", tuple(out.shape), (t, n))
-    y_ld = n if y.is_contiguous() else _rows2d(y, "moe_combine")[2]
-    o_ld = n if out.is_contiguous() else _rows2d(out, "moe_combine")[2]
-    _on(dev, lib().sm_moe_combine, y.data_ptr(), _TYPES[y.dtype], m, n, y_ld, weights.data_ptr(), slots.data_ptr(), t, k, out.data_ptr(), o_ld)
+        _gpu(index, "moe_combine", out, _TYPES)
+        if out.shape != (t, n) or (dtype is not None and dtype != out.dtype):
+            _refuse("moe_combine: output %s of type %s, wanted %s", tuple(out.shape), out.dtype, (t, n))
+        o_ld = _rows2d(out, "moe_combine")[2]
+    _on(index, lib().sm_moe_combine, y.data_ptr(), _TYPES[y.dtype], m, n, _rows2d(y, "moe_combine")[2], weights.data_ptr(), slots.data_ptr(), t, k, out.data_ptr(), _TYPES[out.dtype], o_ld)
     return out

@@ -272,7 +272,8 @@ def test_python_refusals():
               lambda: ops.expert_linear(x, w3, off.long()), lambda: ops.expert_linear(x, w3, off[:1]), lambda: ops.expert_linear(x, w3, off, torch.zeros(4, device="cuda")),
               lambda: ops.expert_linear(x, torch.zeros(1, 8, 64, device="cuda", dtype=BF16), off), lambda: ops.expert_linear(x, torch.zeros(1, 64, 8, device="cuda", dtype=F16).transpose(1, 2), off),
               lambda: ops.expert_linear(x, ops.Mx4(w.codes[None, :7], w.scales[None, :7], 64), off, gated=True), lambda: ops.moe_route(x, 65), lambda: ops.moe_route(x, 0),
-              lambda: ops.moe_combine(x, off.view(1, 2), torch.zeros(1, 3, device="cuda")), lambda: ops.moe_combine(x.float(), off.view(1, 2), torch.zeros(1, 2, device="cuda"))):
+              lambda: ops.moe_combine(x, off.view(1, 2), torch.zeros(1, 3, device="cuda")), lambda: ops.moe_combine(x.double(), off.view(1, 2), torch.zeros(1, 2, device="cuda")),
+              lambda: ops.moe_combine(x, off.view(1, 2), torch.zeros(1, 2, device="cuda"), dtype=torch.int32)):
         with pytest.raises(N.SmelterError) as e:
             f()
         assert e.value.kind == "invalidArgument"
@@ -328,7 +329,7 @@ def test_route_strided_and_many_tokens():
     same_route(torch.zeros(3000, 64), 2, True)                          # everything to two experts
 
 
-@pytest.mark.parametrize("t", [F16, BF16])
+@pytest.mark.parametrize("t", [F16, BF16, F32])
 @pytest.mark.parametrize("tokens, k, n", [(1, 1, 1), (7, 6, 40), (50, 8, 131), (300, 2, 264), (3, 0, 8)])
 def test_combine(t, tokens, k, n):
     g = gen(tokens + n)
@@ -339,6 +340,8 @@ def test_combine(t, tokens, k, n):
     rows = y.double()[slots.clamp(0, m - 1).long()]
     want, mag = (rows * ok[..., None]).sum(1), (rows.abs() * ok[..., None]).sum(1)
     mx4ref.close(ops.moe_combine(y.cuda(), slots.cuda(), w.cuda()), want, (k + 1) * 2.0 ** -23 * mag)
+    for d in (F16, BF16, F32):
+        mx4ref.close(ops.moe_combine(y.cuda(), slots.cuda(), w.cuda(), dtype=d), want, (k + 1) * 2.0 ** -23 * mag)
     wide = torch.full((tokens, n + 5), 7.0, dtype=t, device="cuda")
     yw = torch.full((m, n + 3), NAN, dtype=t, device="cuda")
     yw[:, 1:n + 1] = y.cuda()

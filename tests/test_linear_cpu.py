@@ -19,7 +19,7 @@ def desc(**k):
 
 
 def linear(d, x=P, xs=P, w=P, ws=P, bias=None, offsets=None, rows=None, y=P):
-    return N.lib().sm_linear_fwd(C.byref(d), x, xs, w, ws, bias, offsets, rows, y, None)
+    return N.lib().sm_linear_fwd(C.byref(d), x, xs, w, ws, bias, offsets, rows, y, None, 0, None)
 
 
 def refused(rc, word):
@@ -44,7 +44,7 @@ def test_linear_refuses_operands():
     refused(linear(desc(), x=C.c_void_p(4097)), "aligned")
     refused(linear(desc(w_type=MX4), w=C.c_void_p(4104)), "16-byte")
     refused(linear(desc(), bias=C.c_void_p(4098)), "aligned")
-    refused(N.lib().sm_linear_fwd(None, P, P, P, P, None, None, None, P, None), "null")
+    refused(N.lib().sm_linear_fwd(None, P, P, P, P, None, None, None, P, None, 0, None), "null")
 
 
 def test_linear_of_nothing_is_done_at_once():
@@ -84,12 +84,13 @@ def test_route_and_combine_refuse():
     refused(call(z=None), "null")
     refused(call(off=None), "null")
     refused(call(T=1000), "workspace")
-    refused(c(P, F32, 4, 8, 8, P, P, 2, 2, P, 8, None), "type")
-    refused(c(P, F16, 4, 8, 7, P, P, 2, 2, P, 8, None), "strides")
-    refused(c(P, F16, 4, 8, 8, P, P, 2, 2, P, 7, None), "strides")
-    refused(c(None, F16, 4, 8, 8, P, P, 2, 2, P, 8, None), "null")
-    refused(c(P, F16, -1, 8, 8, P, P, 2, 2, P, 8, None), "sizes")
-    assert c(None, F16, 4, 8, 8, None, None, 0, 2, None, 8, None) == 0
+    refused(c(P, MX4, 4, 8, 8, P, P, 2, 2, P, F16, 8, None), "type")
+    refused(c(P, F16, 4, 8, 8, P, P, 2, 2, P, MX4, 8, None), "type")
+    refused(c(P, F16, 4, 8, 7, P, P, 2, 2, P, F16, 8, None), "strides")
+    refused(c(P, F16, 4, 8, 8, P, P, 2, 2, P, F16, 7, None), "strides")
+    refused(c(None, F16, 4, 8, 8, P, P, 2, 2, P, F16, 8, None), "null")
+    refused(c(P, F16, -1, 8, 8, P, P, 2, 2, P, F16, 8, None), "sizes")
+    assert c(None, F16, 4, 8, 8, None, None, 0, 2, None, F16, 8, None) == 0
 
 
 def test_python_entry_points_refuse_cpu_tensors():
