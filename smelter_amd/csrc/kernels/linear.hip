@@ -1,16 +1,23 @@
 // smelter_amd/csrc/kernels/linear.hip — linear layers with 16-bit or MX4 weights, dense or grouped by expert: argument checks and the choice of kernel.
 #include "linear_stream.hpp"
 
-template <int XK, int WK> static int lin_stream(const LinearParams& q, hipStream_t s, int waves) {
-    LinearParams p = q;
-    const int cols = p.gated ? 16 : 32;
+template <int XK, int WK, int NB> static int lin_stream_nb(LinearParams p, hipStream_t s) {
+    const int cols = p.gated ? 8 * NB : 16 * NB;
     p.n_tiles = (p.N + cols - 1) / cols;
     p.m_tiles = lin_row_tiles(p, 16);
     const long long blocks = p.m_tiles * p.n_tiles;
     SM_REQUIRE(blocks < (1ll << 31), "linear: %lld row tiles x %d column tiles exceed one launch", p.m_tiles, p.n_tiles);
-    lin_stream_kernel<XK, WK><<<dim3((unsigned)blocks), 64 * waves, (size_t)waves * 2 * 16 * 17 * 4, s>>>(p);
+    const int chunks = ((p.K + 31) / 32 + (WK == SM_MX4 ? 15 : 3)) / (WK == SM_MX4 ? 16 : 4);
+    int waves = blocks >= 4 * SM_NUM_CU ? 4 : 8;                                    // many blocks: fewer sums to join (16 experts bf16 2048 x 2048: 13.2 us with 4 waves, 15.4 with 8; one 4096 x 4096: 15.0, 13.6)
+    while (waves > 1 && waves > chunks) waves /= 2;
+    lin_stream_kernel<XK, WK, NB><<<dim3((unsigned)blocks), 64 * waves, (size_t)waves * NB * 16 * 17 * 4, s>>>(p);
     SM_LAUNCH_CHECK();
     return SM_OK;
+}
+// four groups of weight rows for a wave where that leaves a block for every CU (64 experts 8192 x 2048 MX4: 77 us against 89), two otherwise (4096 x 4096: 7.7 against 10.6)
+template <int XK, int WK> static int lin_stream(const LinearParams& p, hipStream_t s) {
+    const long long tiles = lin_row_tiles(p, 16) * ((p.w_rows + 63) / 64);
+    return tiles >= SM_NUM_CU ? lin_stream_nb<XK, WK, 4>(p, s) : lin_stream_nb<XK, WK, 2>(p, s);
 }
 
 static int lin_size(int kind, long long K, long long* row, long long* scale_row) {
@@ -31,7 +38,7 @@ static LinearPlan lin_plan(const sm_linear_desc* d, bool grouped, bool gathered)
     p.x_ld = d->x_type != SM_MX4 && d->x_ld ? 2 * d->x_ld : xr; p.w_es = wr * (p.gated ? 2 : 1) * d->N;
     const long long per = grouped ? (d->M + d->E - 1) / d->E : d->M;
     LinearPlan plan = {-1, 1, 0};
-    if (per <= 16 || !lin_tile_fits(p)) return plan;
+    if (per <= 16 || d->K < 8 || !lin_tile_fits(p)) return plan;
     auto tiles = [&](int bn, int bm) { const int cols = p.gated ? bn / 2 : bn; return lin_row_tiles(p, bm) * ((p.N + cols - 1) / cols); };
     const long long n0 = tiles(128, 128), n1 = tiles(256, 256), n2 = tiles(128, 64);
     // times in units of a round of 512 tiles of 128 x 128, two on a CU
@@ -90,7 +97,6 @@ extern "C" int sm_linear_fwd(const sm_linear_desc* d, const void* x, const void*
     LinearPlan plan = lin_plan(d, offsets != nullptr, rows != nullptr);
     if (plan.shape >= 0) {
         const bool dma = d->x_type == SM_MX4 || (p.K % 8 == 0 && (size_t)x % 16 == 0 && p.x_ld % 16 == 0 && (d->w_type == SM_MX4 || (size_t)w % 16 == 0));
-        if (!dma && plan.shape == 1) plan.shape = 0;
         p.splits = plan.splits;
         if (p.splits > 1) {
             p.part_ld = lin_part_ld(p.w_rows);
@@ -103,8 +109,7 @@ extern "C" int sm_linear_fwd(const sm_linear_desc* d, const void* x, const void*
         if (rc > 0) rc = lin_tile_launch(p, d->x_type, d->w_type, plan.shape, dma, s);
         return rc != SM_OK || p.splits == 1 ? rc : lin_join_launch(p, s);
     }
-    const int waves = p.K <= 256 ? 1 : p.K <= 1024 ? 4 : 8;
-    if (d->x_type == SM_MX4) return lin_stream<SM_MX4, SM_MX4>(p, s, waves);
-    if (d->w_type == SM_MX4) return d->x_type == SM_F16 ? lin_stream<SM_F16, SM_MX4>(p, s, waves) : lin_stream<SM_BF16, SM_MX4>(p, s, waves);
-    return d->x_type == SM_F16 ? lin_stream<SM_F16, SM_F16>(p, s, waves) : lin_stream<SM_BF16, SM_BF16>(p, s, waves);
+    if (d->x_type == SM_MX4) return lin_stream<SM_MX4, SM_MX4>(p, s);
+    if (d->w_type == SM_MX4) return d->x_type == SM_F16 ? lin_stream<SM_F16, SM_MX4>(p, s) : lin_stream<SM_BF16, SM_MX4>(p, s);
+    return d->x_type == SM_F16 ? lin_stream<SM_F16, SM_F16>(p, s) : lin_stream<SM_BF16, SM_BF16>(p, s);
 }

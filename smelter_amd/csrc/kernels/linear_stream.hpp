@@ -1,11 +1,12 @@
 // smelter_amd/csrc/kernels/linear_stream.hpp — linear layers on FEW rows (decoding, small groups): the weights stream through the registers once, nothing is staged.
 //
-// A block owns 16 slots of one group and two groups of 16 weight rows (32 output columns, or 16 gated ones: gate rows and up rows); its waves split K and join their sums in LDS, in a fixed
-// order.  Bound by the weights' bytes: a lane holds 32 consecutive k of one weight row (64 bytes of fp16, or one or two 16-byte MX4 blocks), so that a wave reads whole 128 / 256-byte pieces
-// of 16 rows; which k a matrix instruction multiplies does not matter as long as both operands agree, so x is read in the same order (k = 32 (4 it + g) + 8 i for lane group g, step i) and no
-// operand is re-arranged.  MX4 weights under 16-bit x become 16-bit values in the registers.  bf16: value times scale, exact.  fp16: the range of 2^-24 .. 65504 does not hold every scale, so
-// the values are taken relative to the largest scale of their 256 (row, k) neighbours and the partial sum is multiplied by it in fp32 (a block 2^23 below that neighbour rounds, by less
-// than the fp32 sum does).
+// A block owns 16 slots of one group and NB groups of 16 weight rows (16 NB output columns, or half as many gated ones: gate rows and up rows); its waves split K and join their sums in LDS, in a
+// fixed order.  Bound by the weights' bytes: a lane holds 32 consecutive k of one weight row (64 bytes of fp16, or two 16-byte MX4 blocks), so that a wave reads whole 128 / 256-byte pieces of 16
+// rows; which k a matrix instruction multiplies does not matter as long as both operands agree, so x is read in the same order and no operand is re-arranged.  What else goes through a CU's L1 is
+// kept small beside the weights: the scales come as one dword per lane for 16 blocks and are handed to their lanes by a shuffle (byte loads cost 8 of 28 us of a 5-row layer of 16384 x 8192),
+// lanes without a slot load no x, and where there are blocks enough a wave takes four groups of weight rows with the same x.
+// MX4 weights under 16-bit x become 16-bit values in the registers.  bf16: value times scale, exact.  fp16: the range of 2^-24 .. 65504 does not hold every scale, so the values are taken
+// relative to the largest scale of their row in these 512 k and the partial sum is multiplied by it in fp32 (a block 2^23 below that neighbour rounds, by less than the fp32 sum does).
 #pragma once
 #include "linear.hpp"
 
@@ -26,97 +27,121 @@ template <int KIND> __device__ __forceinline__ void lin_load_block(LinBlk<KIND>&
     }
 }
 
-template <int XK, int WK> __global__ void lin_stream_kernel(LinearParams p) {
-    constexpr int NB = 2, BL = WK == SM_MX4 ? 2 : 1;                    // weight row groups; blocks of 32 k per lane and step
+// four scale bytes of the blocks b .. b + 3 of a row, zero behind its end
+__device__ __forceinline__ unsigned lin_load_scales4(const unsigned char* row, int b, int nb) {
+    unsigned v = 0;
+    if (b + 4 <= nb) __builtin_memcpy(&v, row + b, 4);
+    else {
+#pragma unroll
+        for (int i = 0; i < 3; i++) if (b + i < nb) v |= (unsigned)row[b + i] << (8 * i);
+    }
+    return v;
+}
+
+template <int XK, int WK, int NB> __global__ __launch_bounds__(512) void lin_stream_kernel(LinearParams p) {
+    constexpr bool MXW = WK == SM_MX4;
+    constexpr int BL = MXW ? 2 : 1, U = MXW ? 2 : 1, CB = 4 * BL * U;  // blocks of 32 k per lane and step; steps of a chunk; blocks of a chunk
     extern __shared__ float part[];                                     // [waves][NB][16 slots][17]
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
     const int r = lane & 15, g = lane >> 4;
-    const long long mt = blockIdx.x / p.n_tiles; const int nt = (int)(blockIdx.x - mt * p.n_tiles);
+    const long long mt = blockIdx.x / (unsigned)p.n_tiles; const int nt = (int)(blockIdx.x - mt * p.n_tiles);
     const LinTile tile = lin_find_tile(p, 16, mt, false);
     if (tile.rows == 0) return;
     const int nb = (p.K + 31) >> 5;
-    const int cols = p.gated ? 16 : 32, n0 = nt * cols;
-    // operand rows of this lane; rows behind the end repeat the last one and are not stored
-    long long xrow = tile.row0 + (r < tile.rows ? r : tile.rows - 1);
+    constexpr int G = NB / 2;                                           // groups of gate rows of a gated layer
+    const int cols = p.gated ? 16 * G : 16 * NB, n0 = nt * cols;
+    long long xrow = tile.row0 + (r < tile.rows ? r : 0);
     if (p.rows) xrow = p.rows[xrow];
-    const bool live = xrow >= 0 && xrow < p.T;                          // a row index outside x reads as a row of zeros
+    const bool live = r < tile.rows && xrow >= 0 && xrow < p.T;         // lanes without a slot, and row indices outside x: zeros
     if (!live) xrow = 0;
     const char* xr = p.x + xrow * p.x_ld; const unsigned char* xsr = p.xs + xrow * p.xs_ld;
+    const int xk = live ? p.K : 0, xnb = live ? nb : 0;
     const char* wr[NB]; const unsigned char* wsr[NB];
 #pragma unroll
     for (int b = 0; b < NB; b++) {
-        int n = n0 + r + (p.gated ? 0 : 16 * b); if (n >= p.N) n = p.N - 1;
-        const long long row = n + (p.gated ? (long long)b * p.N : 0);
+        int n = n0 + r + 16 * (p.gated ? b % G : b); if (n >= p.N) n = p.N - 1;
+        const long long row = n + (p.gated && b >= G ? (long long)p.N : 0);
         wr[b] = p.w + tile.e * p.w_es + row * p.w_ld;
-        if constexpr (WK == SM_MX4) wsr[b] = p.ws + tile.e * p.ws_es + row * p.ws_ld;
+        wsr[b] = p.ws + tile.e * p.ws_es + row * p.ws_ld;
     }
     floatx4 acc[NB];
 #pragma unroll
     for (int b = 0; b < NB; b++) acc[b] = floatx4{0, 0, 0, 0};
 
-    const int steps = (nb + 4 * BL - 1) / (4 * BL);
-    for (int it = wave; it < steps; it += waves) {
-        const int b0 = it * 4 * BL + g * BL;                            // this lane's first block
-        LinBlk<WK> w[NB][BL]; int sc[NB][BL];
+    for (int c = wave * CB; c < nb; c += waves * CB) {
+        // the weights of a chunk are asked for at once: a wave's share of K is short, what counts is how much of it is under way
+        LinBlk<WK> w[U][NB][BL]; unsigned wsc[NB], xsc = 0;
 #pragma unroll
-        for (int b = 0; b < NB; b++)
+        for (int b = 0; b < NB; b++) { wsc[b] = 0; if constexpr (MXW) wsc[b] = lin_load_scales4(wsr[b], c + 4 * g, nb); }
+        if constexpr (XK == SM_MX4) xsc = lin_load_scales4(xsr, c + 4 * g, xnb);
 #pragma unroll
-            for (int j = 0; j < BL; j++) {
-                lin_load_block<WK>(w[b][j], wr[b], b0 + j, nb, p.K);
-                sc[b][j] = 0;
-                if constexpr (WK == SM_MX4) if (b0 + j < nb) sc[b][j] = wsr[b][b0 + j];
-            }
+        for (int u = 0; u < U; u++)
+#pragma unroll
+            for (int b = 0; b < NB; b++)
+#pragma unroll
+                for (int j = 0; j < BL; j++) lin_load_block<WK>(w[u][b][j], wr[b], c + u * 4 * BL + g * BL + j, nb, p.K);
+        // the scales of this lane's blocks c + 8 u + 2 g + {0, 1} lie in lane group 2 u + g / 2, bytes 2 (g & 1) + {0, 1}
+        auto pair = [&](unsigned dw, int u) { return (unsigned)__shfl((int)dw, r + 16 * (2 * u + (g >> 1))) >> (16 * (g & 1)); };
         if constexpr (XK == SM_MX4) {
 #pragma unroll
-            for (int j = 0; j < BL; j++) {
-                LinBlk<SM_MX4> x; int sx = 0;
-                lin_load_block<SM_MX4>(x, xr, live ? b0 + j : nb, nb, p.K);
-                if (live && b0 + j < nb) sx = xsr[b0 + j];
+            for (int u = 0; u < U; u++) {
+                const unsigned sx = pair(xsc, u);
+                unsigned sw[NB];
 #pragma unroll
-                for (int b = 0; b < NB; b++) acc[b] = lin_mma4(x.v[0], sx, w[b][j].v[0], sc[b][j], acc[b]);
+                for (int b = 0; b < NB; b++) sw[b] = pair(wsc[b], u);
+#pragma unroll
+                for (int j = 0; j < BL; j++) {
+                    LinBlk<SM_MX4> x;
+                    lin_load_block<SM_MX4>(x, xr, c + u * 4 * BL + g * BL + j, xnb, p.K);
+#pragma unroll
+                    for (int b = 0; b < NB; b++) acc[b] = lin_mma4(x.v[0], (int)(sx >> (8 * j)), w[u][b][j].v[0], (int)(sw[b] >> (8 * j)), acc[b]);
+                }
             }
         } else {
-            float mul[NB], rel[NB][BL];
-            floatx4 sum[NB];
-            if constexpr (WK == SM_MX4) {
+            constexpr bool OWN = MXW && XK == SM_F16;                   // sums of their own, multiplied by `mul`
+            float mul[NB]; int top[NB]; floatx4 sum[NB];
 #pragma unroll
-                for (int b = 0; b < NB; b++) {
-                    mul[b] = 1.f;
-                    if constexpr (XK == SM_F16) {
-                        int top = sc[b][0];
+            for (int b = 0; b < NB; b++) {
+                sum[b] = OWN ? floatx4{0, 0, 0, 0} : acc[b];
+                if constexpr (OWN) {
+                    int t = 1;
 #pragma unroll
-                        for (int j = 1; j < BL; j++) top = top > sc[b][j] ? top : sc[b][j];
-                        int o = __shfl_xor(top, 16); top = top > o ? top : o;
-                        o = __shfl_xor(top, 32); top = top > o ? top : o;
-                        if (top < 1) top = 1;
-                        mul[b] = mx4_scale(top);                        // >= 2^-126
-#pragma unroll
-                        for (int j = 0; j < BL; j++) { int d = sc[b][j] - top + 127; rel[b][j] = mx4_scale(sc[b][j] == 255 ? 255 : (d > 0 ? d : 0)); }
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < BL; j++) rel[b][j] = mx4_scale(sc[b][j]);
-                    }
+                    for (int i = 0; i < 4; i++) { const int v = wsc[b] >> (8 * i) & 255; t = t > v ? t : v; }
+                    int o = __shfl_xor(t, 16); t = t > o ? t : o;
+                    o = __shfl_xor(t, 32); top[b] = t > o ? t : o;
+                    mul[b] = mx4_scale(top[b]);                         // >= 2^-126
                 }
             }
-            constexpr bool OWN = WK == SM_MX4 && XK == SM_F16;          // partial sums of their own
 #pragma unroll
-            for (int b = 0; b < NB; b++) sum[b] = OWN ? floatx4{0, 0, 0, 0} : acc[b];
+            for (int u = 0; u < U; u++) {
+                unsigned sw[NB];
+                if constexpr (MXW) {
 #pragma unroll
-            for (int j = 0; j < BL; j++) {
-                LinBlk<XK> x;
-                lin_load_block<XK>(x, xr, b0 + j, nb, live ? p.K : 0);
+                    for (int b = 0; b < NB; b++) sw[b] = pair(wsc[b], u);
+                }
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
+                for (int j = 0; j < BL; j++) {
+                    LinBlk<XK> x;
+                    lin_load_block<XK>(x, xr, c + u * 4 * BL + g * BL + j, nb, xk);
 #pragma unroll
                     for (int b = 0; b < NB; b++) {
-                        intx4_t v;
-                        if constexpr (WK == SM_MX4) v = mx4_to16<XK>(w[b][j].v[0][i], rel[b][j]); else v = w[b][j].v[i];
-                        sum[b] = lin_mma16<XK>(x.v[i], v, sum[b]);
+                        float rel = 0.f;
+                        if constexpr (MXW) {
+                            int byte = sw[b] >> (8 * j) & 255;
+                            if constexpr (OWN) { const int d = byte - top[b] + 127; byte = byte == 255 ? 255 : d > 0 ? d : 0; }
+                            rel = mx4_scale(byte);
+                        }
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            intx4_t v;
+                            if constexpr (MXW) v = mx4_to16<XK>(w[u][b][j].v[0][i], rel); else v = w[u][b][j].v[i];
+                            sum[b] = lin_mma16<XK>(x.v[i], v, sum[b]);
+                        }
                     }
                 }
             }
 #pragma unroll
-            for (int b = 0; b < NB; b++) acc[b] = OWN ? acc[b] + sum[b] * mul[b] : sum[b];
+            for (int b = 0; b < NB; b++) { if constexpr (OWN) acc[b] += sum[b] * mul[b]; else acc[b] = sum[b]; }
         }
     }
     // acc[b][i] = slot 4 g + i, weight row r of group b
@@ -132,7 +157,7 @@ template <int XK, int WK> __global__ void lin_stream_kernel(LinearParams p) {
         if (n >= p.N) continue;
         float v[2] = {0.f, 0.f};
         for (int h = 0; h < (p.gated ? 2 : 1); h++) {
-            const int b = p.gated ? h : c >> 4;
+            const int b = (c >> 4) + h * G;
             for (int q = 0; q < waves; q++) v[h] += part[((q * NB + b) * 16 + i) * 17 + (c & 15)];
             if (bias) v[h] += bias[n + (h ? p.N : 0)];
         }

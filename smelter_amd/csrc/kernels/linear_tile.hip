@@ -2,7 +2,8 @@
 #include "linear_tile.hpp"
 
 template <int XK, int WK> static int lin_tile_shape(const LinearParams& p, int shape, bool dma, hipStream_t s) {
-    if constexpr (XK != SM_MX4) if (!dma) return shape == 2 ? lin_tile<XK, WK, 32, 2, 2, 2, 1, false>(p, s) : lin_tile<XK, WK, 32, 2, 2, 2, 2, false>(p, s);
+    if constexpr (XK != SM_MX4) if (!dma)
+        return shape == 1 ? lin_tile<XK, WK, 16, 2, 4, 8, 4, false>(p, s) : shape == 2 ? lin_tile<XK, WK, 32, 2, 2, 2, 1, false>(p, s) : lin_tile<XK, WK, 32, 2, 2, 2, 2, false>(p, s);
     return shape == 1 ? lin_tile<XK, WK, 16, 2, 4, 8, 4, true>(p, s) : shape == 2 ? lin_tile<XK, WK, 32, 2, 2, 2, 1, true>(p, s) : lin_tile<XK, WK, 32, 2, 2, 2, 2, true>(p, s);
 }
 

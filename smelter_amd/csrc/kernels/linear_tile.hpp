@@ -104,18 +104,40 @@ __device__ __forceinline__ void lin_finish(const LinearParams& p, const LinTile&
 #pragma unroll
                 for (int i = 0; i < 4; i++) { q[i] = q0[i]; q[4 + i] = q1[i]; }
                 if (p.rows && lin_slot_row(p, tile, slot) < 0) for (int i = 0; i < 8; i++) q[i] = 0.f;
-                if (bias) for (int i = 0; i < 8; i++) if (n + i < p.N) q[i] += bias[n + i + up];
+                if (bias) {
+                    if (n + 8 <= p.N) {
+                        float t[8]; __builtin_memcpy(t, bias + n + up, 32);
+#pragma unroll
+                        for (int i = 0; i < 8; i++) q[i] += t[i];
+                    } else for (int i = 0; i < 8; i++) if (n + i < p.N) q[i] += bias[n + i + up];
+                }
             };
             get(j, v, 0);
             if (p.gated) {
                 float u[8]; get(j + 4, u, p.N);
                 for (int i = 0; i < 8; i++) v[i] = lin_silu(v[i]) * u[i];
-            } else if (p.act != SM_ACT_NONE) for (int i = 0; i < 8; i++) v[i] = lin_act(v[i], p.act, p.slope);
+            } else if (p.act > SM_ACT_PRELU) {
+                for (int i = 0; i < 8; i++) v[i] = sm_act_other(v[i], p.act, p.slope);
+            } else if (p.act != SM_ACT_NONE) {
+                const float slope = p.act == SM_ACT_RELU ? 0.f : p.slope;
+#pragma unroll
+                for (int i = 0; i < 8; i++) v[i] = v[i] < 0.f ? (p.act == SM_ACT_RELU ? 0.f : v[i] * slope) : v[i];
+            }
             const long long out = (tile.row0 + slot) * p.y_ld + n;
             if (p.y_vec && n + 8 <= p.N) lin_store8(p.y, out, v, p.y_type);
             else for (int i = 0; i < 8; i++) if (n + i < p.N) lin_store1(p.y, out + i, v[i], p.y_type);
         }
     }
+}
+
+// the eight 16-bit elements of v without the first n, zeros behind them
+__device__ __forceinline__ intx4_t lin_drop(intx4_t v, int n) {
+    typedef unsigned long long ull;
+    const ull lo = (unsigned)v[0] | (ull)(unsigned)v[1] << 32, hi = (unsigned)v[2] | (ull)(unsigned)v[3] << 32;
+    const int s = 16 * n, t = s & 63;
+    const ull a = t ? (lo >> t) | (hi << (64 - t)) : lo, b = hi >> t;
+    const ull l = s < 64 ? a : s < 128 ? b : 0, h = s < 64 ? b : 0;
+    return intx4_t{(int)l, (int)(l >> 32), (int)h, (int)(h >> 32)};
 }
 
 template <int XK, int WK, int FR, int WN, int WM, int FN, int FM, bool DMA> struct LinTileShape {
@@ -232,16 +254,16 @@ __global__ __launch_bounds__(64 * WN * WM) void lin_tile_kernel(LinearParams p) 
             }
         }
         if constexpr (!DMA) {
-            const int k = t * 64 + chunk * 8;
+            const int k = t * 64 + chunk * 8, at = k < p.K - 8 ? k : p.K - 8;       // the last ones of a row as its last eight elements
             if constexpr (!DEQ) {
 #pragma unroll
-                for (int i = 0; i < QW; i++) wreg[i] = lin_load8(wexp + woff[i], k, p.K);
+                for (int i = 0; i < QW; i++) __builtin_memcpy(&wreg[i], wexp + woff[i] + 2ll * at, 16);
             }
 #pragma unroll
-            for (int i = 0; i < QX; i++) xreg[i] = lin_load8(xbase + xoff[i], k, p.K);
+            for (int i = 0; i < QX; i++) __builtin_memcpy(&xreg[i], xbase + xoff[i] + 2ll * at, 16);
         }
     };
-    auto store_staged = [&](int t) {
+    auto store_staged = [&](int t, auto end) {                                      // end: t may be the last step of a row
         if constexpr (MX) {
             const int over = nb >= 8 && 8 * t > nb - 8 ? 8 * t - (nb - 8) : 0;      // bytes of the step before, shifted out; behind the end (codes 0) scale 0
 #pragma unroll
@@ -261,12 +283,13 @@ __global__ __launch_bounds__(64 * WN * WM) void lin_tile_kernel(LinearParams p) 
         }
         if constexpr (!DMA) {
             char* st = lds + (t & 1) * S::STAGE + lane * 16;
+            const int k = t * 64 + chunk * 8, over = k > p.K - 8 ? k - (p.K - 8) : 0;   // elements before k in the eight; behind the row's end zeros
             if constexpr (!DEQ) {
 #pragma unroll
-                for (int i = 0; i < QW; i++) *(intx4_t*)(st + (wave * QW + i) * 1024) = wreg[i];
+                for (int i = 0; i < QW; i++) { if constexpr (decltype(end)::value) wreg[i] = lin_drop(wreg[i], over); *(intx4_t*)(st + (wave * QW + i) * 1024) = wreg[i]; }
             }
 #pragma unroll
-            for (int i = 0; i < QX; i++) *(intx4_t*)(st + BN * 128 + (wave * QX + i) * 1024) = xreg[i];
+            for (int i = 0; i < QX; i++) { if constexpr (decltype(end)::value) xreg[i] = lin_drop(xreg[i], over); *(intx4_t*)(st + BN * 128 + (wave * QX + i) * 1024) = xreg[i]; }
         }
     };
     // ---- the products of a step in four phases (fragments of 32 rows: one for each 32 bytes of K; of 16 rows: one for each 64 bytes of K and each half of the wave's weight rows; 128-row tiles of
@@ -331,19 +354,19 @@ __global__ __launch_bounds__(64 * WN * WM) void lin_tile_kernel(LinearParams p) 
 #pragma unroll
             for (int i = 0; i < QT; i++) fill(first, i);
         }
-        load_staged(first, std::false_type()); store_staged(first);
+        load_staged(first, std::false_type()); store_staged(first, std::true_type());
         if (steps > first + 1) {
             if constexpr (DMA) {
 #pragma unroll
                 for (int i = 0; i < QT / 2; i++) fill(first + 1, i);
             }
-            load_staged(first + 1, std::false_type()); store_staged(first + 1);
+            load_staged(first + 1, std::false_type()); store_staged(first + 1, std::true_type());
         }
         if (steps > first + 2) load_staged(first + 2, std::false_type());
         lin_arrive();
         read(first, First(), ragged && steps == first + 1);
     }
-    auto step = [&](int t, auto has1, auto has2) {                                  // has1, has2: steps t + 1, t + 2 exist
+    auto step = [&](int t, auto has1, auto has2, auto end2) {                       // has1, has2: steps t + 1, t + 2 exist; end2: t + 2 may be the last
         constexpr bool MORE = decltype(has1)::value, MORE2 = decltype(has2)::value;
         sm_static_for<0, PH - 1>([&](auto phase) {
             constexpr int P = decltype(phase)::value;
@@ -358,7 +381,7 @@ __global__ __launch_bounds__(64 * WN * WM) void lin_tile_kernel(LinearParams p) 
         });
         if constexpr (MORE) {
             lin_arrive();                                                           // step t + 1 is in LDS for everybody; everybody has read the whole of step t
-            if constexpr (MORE2) { store_staged(t + 2); load_staged(t + 3 < steps ? t + 3 : steps - 1, std::true_type()); }
+            if constexpr (MORE2) { store_staged(t + 2, end2); load_staged(t + 3 < steps ? t + 3 : steps - 1, std::true_type()); }
         }
         products(Last(), [&](int a) {
             if constexpr (MORE) if (a == 0) { __builtin_amdgcn_sched_barrier(0); read(t + 1, First(), !MORE2 && ragged); __builtin_amdgcn_sched_barrier(0); }
@@ -371,9 +394,10 @@ __global__ __launch_bounds__(64 * WN * WM) void lin_tile_kernel(LinearParams p) 
     };
     int t = first;
 #pragma unroll 1
-    for (; t + 2 < steps; t++) step(t, std::true_type(), std::true_type());
-    if (t + 1 < steps) { step(t, std::true_type(), std::false_type()); t++; }
-    if (t < steps) step(t, std::false_type(), std::false_type());
+    for (; t + (DMA ? 2 : 3) < steps; t++) step(t, std::true_type(), std::true_type(), std::false_type());
+    if constexpr (!DMA) if (t + 2 < steps) { step(t, std::true_type(), std::true_type(), std::true_type()); t++; }
+    if (t + 1 < steps) { step(t, std::true_type(), std::false_type(), std::false_type()); t++; }
+    if (t < steps) step(t, std::false_type(), std::false_type(), std::false_type());
 
     lin_finish<FR, WN, WM, FN, FM, 2 * S::STAGE, DEQ && XK == SM_F16>(p, tile, split, n0, acc, lds, wmul);
 }
