@@ -31,46 +31,58 @@ __device__ __forceinline__ float route_load(const RouteParams& p, long long t, i
     return p.type == SM_F32 ? ((const float*)p.z)[i] : p.type == SM_F16 ? (float)((const half_t*)p.z)[i] : (float)((const bf16_t*)p.z)[i];
 }
 
-// one token by one wave: lane l holds the scores of experts l, 64 + l, ...
-template <int EPL> __device__ __forceinline__ void route_token(const RouteParams& p, long long t, int* hist) {
-    const int lane = threadIdx.x & 63;
+// maximum / minimum / sum over the 16 lanes of a row, in every one of them (rotations inside the row: no LDS)
+template <class F> __device__ __forceinline__ unsigned route_row(unsigned v, F f) {
+    v = f(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x128, 0xf, 0xf, true)); v = f(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x124, 0xf, 0xf, true));
+    v = f(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x122, 0xf, 0xf, true)); return f(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x121, 0xf, 0xf, true));
+}
+__device__ __forceinline__ unsigned route_max(unsigned v) { return route_row(v, [](unsigned a, unsigned b) { return a > b ? a : b; }); }
+__device__ __forceinline__ unsigned route_min(unsigned v) { return route_row(v, [](unsigned a, unsigned b) { return a < b ? a : b; }); }
+__device__ __forceinline__ float route_sum(float v) {
+    return __builtin_bit_cast(float, route_row(__builtin_bit_cast(unsigned, v), [](unsigned a, unsigned b) { return __builtin_bit_cast(unsigned, __builtin_bit_cast(float, a) + __builtin_bit_cast(float, b)); }));
+}
+
+// Four tokens by one wave, each by a row of 16 lanes: lane l of a row holds the scores of experts l, 16 + l, ...  (one token by a whole wave with shuffles: 64 us for 16384 tokens of 128 scores.)
+// t >= t1: no token (its lanes run along).
+template <int EPL> __device__ __forceinline__ void route_tokens(const RouteParams& p, long long t, long long t1, int* hist) {
+    const int l = threadIdx.x & 15;
+    const bool in = t < t1;
     unsigned key[EPL];
 #pragma unroll
-    for (int j = 0; j < EPL; j++) { const int e = j * 64 + lane; float z = e < p.E ? route_load(p, t, e) : -__builtin_inff(); if (z == 0.f) z = 0.f; key[j] = route_key(z); }
-    unsigned all[EPL];
+    for (int j = 0; j < EPL; j++) { const int e = j * 16 + l; float z = in && e < p.E ? route_load(p, t, e) : -__builtin_inff(); if (z == 0.f) z = 0.f; key[j] = route_key(z); }
+    unsigned first = 0; float total = 0.f;
+    if (!p.renorm) {                                                               // the maximum first: the sum goes over all scores
 #pragma unroll
-    for (int j = 0; j < EPL; j++) all[j] = key[j];
-    unsigned first = 0; float chosen = 0.f, mine = 0.f; int expert = -1;      // lane i < k keeps the i-th choice
+        for (int j = 0; j < EPL; j++) first = first > key[j] ? first : key[j];
+        first = route_max(first);
+#pragma unroll
+        for (int j = 0; j < EPL; j++) total += key[j] == 0 ? 0.f : key[j] == first ? 1.f : expf(route_value(key[j]) - route_value(first));
+        total = route_sum(total);
+    }
+    float mine[2] = {0.f, 0.f}; int expert[2] = {-1, -1};                           // lane l keeps the choices l and 16 + l
     for (int i = 0; i < p.k; i++) {
         unsigned m = 0;
 #pragma unroll
         for (int j = 0; j < EPL; j++) m = m > key[j] ? m : key[j];
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) { const unsigned o = __shfl_xor(m, d); m = m > o ? m : o; }
-        if (m == 0) break;
+        m = route_max(m);
         if (i == 0) first = m;
-        const float e1 = m == first ? 1.f : expf(route_value(m) - route_value(first));
-        chosen += e1;
-        int at = -1;
+        unsigned at = ~0u;                                                          // the lowest expert with that score
 #pragma unroll
-        for (int j = 0; j < EPL; j++) {
-            const unsigned long long hit = __ballot(at < 0 && key[j] == m);
-            if (hit) { const int l = __builtin_ctzll(hit); at = j * 64 + l; if (lane == l) key[j] = 0; }
-        }
-        if (lane == i) { mine = e1; expert = at; }
+        for (int j = EPL - 1; j >= 0; j--) at = key[j] == m ? (unsigned)(j * 16 + l) : at;
+        at = route_min(at);
+#pragma unroll
+        for (int j = 0; j < EPL; j++) key[j] = (unsigned)(j * 16 + l) == at ? 0 : key[j];
+        const float e1 = m == 0 ? 0.f : m == first ? 1.f : expf(route_value(m) - route_value(first));
+        if (p.renorm) total += e1;
+        if ((i & 15) == l) { if (i < 16) { mine[0] = e1; expert[0] = m == 0 ? -1 : (int)at; } else { mine[1] = e1; expert[1] = m == 0 ? -1 : (int)at; } }
     }
-    if (!p.renorm) {
-        float s = 0.f;
 #pragma unroll
-        for (int j = 0; j < EPL; j++) s += all[j] == 0 ? 0.f : all[j] == first ? 1.f : expf(route_value(all[j]) - route_value(first));
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) s += __shfl_xor(s, d);
-        chosen = s;
-    }
-    if (lane < p.k) {
-        p.experts[t * p.k + lane] = expert;
-        p.weights[t * p.k + lane] = expert < 0 ? 0.f : mine / chosen;
-        if (expert >= 0) atomicAdd(&hist[expert], 1);                          // a count: the same in any order
+    for (int h = 0; h < 2; h++) {
+        const int i = 16 * h + l;
+        if (!in || i >= p.k) continue;
+        p.experts[t * p.k + i] = expert[h];
+        p.weights[t * p.k + i] = expert[h] < 0 ? 0.f : mine[h] / total;
+        if (expert[h] >= 0) atomicAdd(&hist[expert[h]], 1);                         // a count: the same in any order
     }
 }
 
@@ -118,14 +130,14 @@ __device__ __forceinline__ void route_scan(const int* total, int* offs, int E) {
 }
 
 // ONE = true: the whole of a small routing in one block
-template <int EPL, bool ONE> __global__ void route_select_kernel(RouteParams p) {
+template <int EPL, bool ONE> __global__ __launch_bounds__(EPL <= 16 ? 1024 : 512) void route_select_kernel(RouteParams p) {
     extern __shared__ int lds[];
     int* hist = lds;                                                             // [E]
     const int wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
     for (int e = threadIdx.x; e < p.E; e += blockDim.x) hist[e] = 0;
     __syncthreads();
     const long long t0 = (long long)blockIdx.x * p.per_block, t1 = t0 + p.per_block < p.T ? t0 + p.per_block : p.T;
-    for (long long t = t0 + wave; t < t1; t += waves) route_token<EPL>(p, t, hist);
+    for (long long t = t0 + wave * 4; t < t1; t += waves * 4) route_tokens<EPL>(p, t + ((threadIdx.x & 63) >> 4), t1, hist);
     __syncthreads();
     if constexpr (!ONE) { for (int e = threadIdx.x; e < p.E; e += blockDim.x) p.counts[(long long)blockIdx.x * p.E + e] = hist[e]; }
     else {
@@ -145,10 +157,20 @@ __global__ void route_place_kernel(RouteParams p, int blocks) {
     int* total = lds; int* before = total + p.E; int* offs = before + p.E; int* wcount = offs + p.E + 1;
     for (int e = threadIdx.x; e < 2 * p.E; e += blockDim.x) lds[e] = 0;
     __syncthreads();
-    // counts of all blocks and of the blocks before this one; integer sums, the same in any order
-    for (long long i = threadIdx.x; i < (long long)blocks * p.E; i += blockDim.x) {
-        const int b = (int)(i / p.E), e = (int)(i - (long long)b * p.E), c = p.counts[i];
-        if (c) { atomicAdd(&total[e], c); if (b < (int)blockIdx.x) atomicAdd(&before[e], c); }
+    // counts of all blocks and of the blocks before this one (integer sums, the same in any order): a thread adds one expert's over every parts-th block, eight loads at a time
+    const int parts = (int)blockDim.x / p.E > 0 ? (int)blockDim.x / p.E : 1;
+    for (int i = threadIdx.x; i < parts * p.E; i += blockDim.x) {
+        const int e = i % p.E, part = i / p.E;
+        int all = 0, low = 0;
+        for (int b0 = part; b0 < blocks; b0 += 8 * parts) {
+            int c[8];
+#pragma unroll
+            for (int q = 0; q < 8; q++) { const int b = b0 + q * parts; c[q] = b < blocks ? p.counts[(long long)b * p.E + e] : 0; }
+#pragma unroll
+            for (int q = 0; q < 8; q++) { all += c[q]; low += b0 + q * parts < (int)blockIdx.x ? c[q] : 0; }
+        }
+        if (all) atomicAdd(&total[e], all);
+        if (low) atomicAdd(&before[e], low);
     }
     __syncthreads();
     route_scan(total, offs, p.E);
@@ -177,13 +199,14 @@ extern "C" size_t sm_moe_route_workspace_bytes(int64_t T, int32_t E, int32_t k) 
 }
 
 template <int EPL> static int route_launch(RouteParams p, hipStream_t s) {
+    constexpr int WAVES = EPL <= 16 ? 16 : 8;                                     // of the selecting kernel: 64 tokens at once, 32 where a lane holds more scores
     const size_t place = (size_t)(MOE_WAVES * p.E + p.E + 1) * sizeof(int);
     if (p.T <= ROUTE_SMALL) {
         p.per_block = (int)p.T;
-        route_select_kernel<EPL, true><<<1, 64 * MOE_WAVES, p.E * sizeof(int) + place, s>>>(p);
+        route_select_kernel<EPL, true><<<1, 64 * WAVES, p.E * sizeof(int) + (size_t)(WAVES * p.E + p.E + 1) * sizeof(int), s>>>(p);
     } else {
         const long long blocks = route_blocks(p.T, &p.per_block);
-        route_select_kernel<EPL, false><<<dim3((unsigned)blocks), 64 * MOE_WAVES, p.E * sizeof(int), s>>>(p);
+        route_select_kernel<EPL, false><<<dim3((unsigned)blocks), 64 * WAVES, p.E * sizeof(int), s>>>(p);
         SM_LAUNCH_CHECK();
         route_place_kernel<<<dim3((unsigned)blocks), 64 * MOE_WAVES, 2 * p.E * sizeof(int) + place, s>>>(p, (int)blocks);
     }
@@ -206,10 +229,11 @@ extern "C" int sm_moe_route(const void* scores, int32_t type, int64_t T, int32_t
     p.z = (const char*)scores; p.type = type; p.T = T; p.E = E; p.k = k; p.ld = ld; p.renorm = renormalize;
     p.weights = weights; p.experts = experts; p.offsets = offsets; p.rows = rows; p.slots = slots; p.counts = (int*)workspace;
     hipStream_t s = sm_s(stream);
-    if (E <= 64) return route_launch<1>(p, s);
-    if (E <= 128) return route_launch<2>(p, s);
-    if (E <= 256) return route_launch<4>(p, s);
-    return route_launch<16>(p, s);
+    if (E <= 64) return route_launch<4>(p, s);
+    if (E <= 128) return route_launch<8>(p, s);
+    if (E <= 256) return route_launch<16>(p, s);
+    if (E <= 512) return route_launch<32>(p, s);
+    return route_launch<64>(p, s);
 }
 
 // out[t, n] = sum_j weights[t, j] * y[slots[t, j], n]: one thread per eight columns of a token, terms added in the order of j in fp32, one rounding; a slot outside 0 .. M - 1 adds nothing.
