@@ -93,7 +93,7 @@ template <int XK, int WK, int FM, int ST> __global__ __launch_bounds__(256) void
         }
     }
 
-    const int wn = wave >> 1, wm = wave & 1;
+    const int wn = wave & 1, wm = wave >> 1;
     floatx16 acc[FN][FM];
 #pragma unroll
     for (int a = 0; a < FN; a++)

@@ -49,7 +49,7 @@ __device__ __forceinline__ long long lin_slot_row(const LinearParams& p, const L
 template <int FR, int WN, int WM, int FN, int FM, int BYTES, bool SCALED, class AccT>
 __device__ __forceinline__ void lin_finish(const LinearParams& p, const LinTile& tile, int split, int n0, AccT (&acc)[FN][FM], char* lds, const float* wmul) {
     constexpr int BN = FR * FN * WN, THREADS = 64 * WN * WM;
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & (FR - 1), g = lane / FR, wn = wave / WM, wm = wave - wn * WM;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & (FR - 1), g = lane / FR, wn = wave % WN, wm = wave / WN;
     const int cols = p.gated ? BN / 2 : BN;
     constexpr int PB = BYTES / (BN * 4) / (FR * WM) < FM ? BYTES / (BN * 4) / (FR * WM) : FM;   // slot groups of a wave that fit at once
     const float* bias = p.bias ? p.bias + (long long)tile.e * p.w_rows : nullptr;
@@ -296,7 +296,7 @@ __global__ __launch_bounds__(64 * WN * WM) void lin_tile_kernel(LinearParams p) 
     // them: two phases); a phase's fragments are read during the phase before it (over the step boundary too)
     typedef float AccT __attribute__((ext_vector_type(FR * FR / 64)));
     constexpr int GA = FR == 32 ? FN : 4, HA = FN / GA, PH = (FR == 32 ? 4 : 2) * HA;
-    const int wn = wave / WM, wm = wave - wn * WM;                                  // this wave's part of the tile
+    const int wn = wave % WN, wm = wave / WN;                                       // this wave's part of the tile
     AccT acc[FN][FM];
 #pragma unroll
     for (int a = 0; a < FN; a++)
@@ -393,6 +393,21 @@ __global__ __launch_bounds__(64 * WN * WM) void lin_tile_kernel(LinearParams p) 
         __builtin_amdgcn_sched_barrier(0);
     };
     int t = first;
+    if constexpr (DMA && !DEQ && !MX) {
+        // a wave whose slots lie behind the tile's last one (the end of a group) only fills; the four SIMDs hold waves of all parts, so that the others run faster
+        if (wm * FM * FR >= tile.rows) {
+            for (; t + 1 < steps; t++) {
+#pragma unroll
+                for (int i = QT / 2; i < QT; i++) fill(t + 1, i);
+                lin_arrive();
+                if (t + 2 < steps) {
+#pragma unroll
+                    for (int i = 0; i < QT / 2; i++) fill(t + 2, i);
+                }
+            }
+            t = steps;
+        }
+    }
 #pragma unroll 1
     for (; t + (DMA ? 2 : 3) < steps; t++) step(t, std::true_type(), std::true_type(), std::false_type());
     if constexpr (!DMA) if (t + 2 < steps) { step(t, std::true_type(), std::true_type(), std::true_type()); t++; }
