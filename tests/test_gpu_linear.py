@@ -458,3 +458,162 @@ def test_packed_by_the_gpu_and_used_at_once():
     x, w = randn(g, 130, 200).to(BF16), randn(g, 90, 200, scale=0.07).to(BF16)
     qx, qw = ops.mx4_quantize(x.cuda()), ops.mx4_quantize(w.cuda())
     mx4ref.close(ops.mx4_linear(qx, qw, dtype=BF16), *mx4ref.linear(mx4ref.unpack(*mx4ref.pack(x), 200), mx4ref.unpack(*mx4ref.pack(w), 200)))
+
+
+# ---- sizes behind 32 bits -----------------------------------------------------------------------------------------------------------------
+
+
+def test_gather_from_more_than_4_gb():
+    """rows of x behind 2^32 bytes, for few and for many slots"""
+    g = gen(1)
+    t, k, n = 270000, 8192, 40
+    x = torch.empty((t, k), dtype=F16, device="cuda")                   # 4.4 GB; only the rows that are read are written
+    w = randn(g, 2, n, k, scale=k ** -0.5).to(F16)
+    for m in (7, 90):
+        at = torch.randint(t - 9000, t, (m,), generator=g)
+        at[0], at[-1] = t - 1, 0
+        v = randn(g, m, k).to(F16)
+        x[at.cuda()] = v.cuda()
+        v = x[at.cuda()].cpu()                                          # (a row drawn twice)
+        off = [0, m // 3, m]
+        got = ops.expert_linear(x, w.cuda(), torch.tensor(off, dtype=torch.int32, device="cuda"), at.int().cuda())
+        mx4ref.close(got, *grouped(v.double(), w.double(), off, list(range(m))))
+
+
+@pytest.mark.parametrize("m", [3, 20, 300])
+def test_weights_of_more_than_2_gb(m):
+    """one matrix of 2.6 GB: the last rows' offsets need all 32 bits"""
+    g = gen(2)
+    n, k = 40000, 32768
+    w = torch.zeros((1, n, k), dtype=BF16, device="cuda")
+    rows = [0, 1, 20000, n - 2, n - 1]
+    v = randn(g, len(rows), k, scale=k ** -0.5).to(BF16)
+    w[0, rows] = v.cuda()
+    x = randn(g, m, k).to(BF16)
+    got = ops.expert_linear(x.cuda(), w, torch.tensor([0, m], dtype=torch.int32, device="cuda")).cpu()
+    mx4ref.close(got[:, rows], *mx4ref.linear(x, v))
+    rest = torch.ones(n, dtype=torch.bool)
+    rest[rows] = False
+    assert got[:, rest].eq(0).all()
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16-mx4"])
+def test_experts_behind_4_gb(kind):
+    """the last of many experts lies behind 2^32 bytes (fp16) of the first"""
+    g = gen(3)
+    e, n, k = 80, 4096, 8192
+    last = randn(g, n, k, scale=k ** -0.5)
+    if kind == "f16":
+        w = torch.empty((e, n, k), dtype=F16, device="cuda")
+        w[-1] = last.to(F16).cuda()
+        wv, dt = last.to(F16).double(), F16
+    else:
+        c, s = mx4ref.pack(last)
+        w = ops.Mx4(torch.empty((e, n, k // 2), dtype=torch.uint8, device="cuda"), torch.empty((e, n, k // 32), dtype=torch.uint8, device="cuda"), k)
+        w.codes[-1], w.scales[-1] = c.cuda(), s.cuda()
+        wv, dt = mx4ref.unpack(c, s, k), BF16
+    for m in (5, 40):
+        x = randn(g, m, k).to(dt)
+        off = torch.zeros(e + 1, dtype=torch.int32)
+        off[-1] = m
+        mx4ref.close(ops.expert_linear(x.cuda(), w, off.cuda()), *mx4ref.linear(x, wv))
+
+
+def test_outputs_of_more_than_2_31_elements():
+    g = gen(4)
+    m, n, k = 300000, 8192, 32
+    w = randn(g, n, k, scale=0.2)
+    q = mx4(w)
+    x = randn(g, m, k).to(BF16)
+    got = ops.mx4_linear(x.cuda(), q)
+    some = torch.cat((torch.arange(40), torch.arange(262100, 262200), torch.arange(m - 40, m)))
+    mx4ref.close(got[some.cuda()], *mx4ref.linear(x[some], val(q)))
+    # ... as the operand of the weighted sum, of the packing and of the reading back
+    slots = torch.stack((some, some.flip(0)), 1).int()
+    wt = torch.rand(slots.shape, generator=g)
+    y = got[slots.flatten().long().cuda()].cpu().double().view(*slots.shape, n)
+    mx4ref.close(ops.moe_combine(got, slots.cuda(), wt.cuda()), (y * wt.double()[..., None]).sum(1), 2.0 ** -21 * (y.abs() * wt.double()[..., None]).sum(1))
+    p = ops.mx4_quantize(got)
+    c, s = mx4ref.pack(got[some.cuda()].cpu())
+    assert torch.equal(p.codes[some.cuda()].cpu(), c) and torch.equal(p.scales[some.cuda()].cpu(), s)
+    back = ops.mx4_dequantize(p, BF16)
+    assert torch.equal(back[some.cuda()].cpu().double(), mx4ref.unpack(c, s, n))
+
+
+@pytest.mark.parametrize("tokens, e, k", [(70, 300, 5), (33, 600, 17), (200, 1024, 32), (100000, 16, 2)])
+def test_route_wide_and_long(tokens, e, k):
+    z = randn(gen(e), tokens, e)
+    if tokens < 1000:
+        same_route(z, k, True)
+        same_route(z.to(BF16), k, False)                                # many ties
+        return
+    got = ops.moe_route(z.cuda(), k)
+    ex = torch.sort(z, dim=-1, descending=True, stable=True).indices[:, :k]
+    order = torch.sort(ex.flatten(), stable=True).indices
+    assert torch.equal(got.experts.cpu().long(), ex) and torch.equal(got.rows.cpu().long(), order // k)
+    assert torch.equal(got.slots.cpu().flatten()[order].long(), torch.arange(tokens * k)) and got.offsets.cpu().tolist() == [0] + torch.bincount(ex.flatten(), minlength=e).cumsum(0).tolist()
+
+
+# ---- every kernel behind the products ------------------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("kind, aligned", [(k, True) for k in KINDS] + [(k, False) for k in KINDS if k != "mx4-mx4"])
+@pytest.mark.parametrize("m, n, k", [(17, 256, 4096), (40, 130, 8192), (129, 1000, 2048), (1000, 1100, 264), (700, 4096, 72), (2500, 3300, 136), (2048, 4096, 1000), (3100, 4100, 200), (4096, 4096, 1032)])
+def test_products_of_all_shapes(kind, m, n, k, aligned):
+    """split and whole K, the three tile shapes, whole and ragged rows; every output against fp64 on the GPU"""
+    g = torch.Generator("cuda").manual_seed(m + n + k)
+    k -= 0 if aligned else 3
+    dt = BF16 if kind.startswith("bf16") else F16
+    x = torch.randn((m, k), generator=g, device="cuda").to(dt)
+    w = torch.randn((n, k), generator=g, device="cuda") * k ** -0.5
+    xv = x.double()
+    if kind == "mx4-mx4":
+        x = ops.mx4_quantize(x)
+        xv = ops.mx4_dequantize(x, F32).double()                        # (exact: tested above)
+    if kind.endswith("mx4"):
+        w = ops.mx4_quantize(w)
+        wv = ops.mx4_dequantize(w, F32).double()
+        got = ops.mx4_linear(x, w, dtype=F32)
+    else:
+        w = w.to(dt)[None]
+        wv = w[0].double()
+        got = ops.expert_linear(x, w, torch.tensor([0, m], dtype=torch.int32, device="cuda"), dtype=F32)
+    want, mag = xv @ wv.t(), xv.abs() @ wv.abs().t()
+    lim = (k / 8 + 64) * 2.0 ** -23 * mag + 2.0 ** -23 * xv.abs().sum(1, keepdim=True) * wv.abs().amax(1)
+    assert ((got.double() - want).abs() <= lim).all()
+
+
+@pytest.mark.parametrize("kind, k", [(k, 264) for k in KINDS] + [(k, 261) for k in KINDS if k != "mx4-mx4"])
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("sizes, n", [([0, 700, 1, 2500, 256, 130, 900], 2100), ([40, 90, 33, 64, 0, 17], 520), ([20] * 20, 100)])
+def test_groups_of_all_shapes(kind, k, gated, sizes, n):
+    """ragged groups with gathered rows and a bias on the tile kernels; every output against fp64 on the GPU"""
+    g = torch.Generator("cuda").manual_seed(n + k + gated)
+    dt = BF16 if kind.startswith("bf16") else F16
+    m, e, wn = sum(sizes), len(sizes), 2 * n if gated else n
+    x = torch.randn((m, k), generator=g, device="cuda").to(dt)
+    w = torch.randn((e, wn, k), generator=g, device="cuda") * k ** -0.5
+    rows = torch.randint(-1, m, (m,), generator=g, device="cuda").int()      # -1: a row of zeros
+    bias = torch.randn((e, wn), generator=g, device="cuda")
+    xv = x.double()
+    if kind == "mx4-mx4":
+        x = ops.mx4_quantize(x)
+        xv = ops.mx4_dequantize(x, F32).double()
+    if kind.endswith("mx4"):
+        w = ops.mx4_quantize(w)
+        wv = ops.mx4_dequantize(w, F32).double()
+    else:
+        w = w.to(dt)
+        wv = w.double()
+    off = [0] + torch.tensor(sizes).cumsum(0).tolist()
+    got = ops.expert_linear(x, w, torch.tensor(off, dtype=torch.int32, device="cuda"), rows, bias, gated=gated, dtype=F32).double()
+    for i in range(e):
+        r = rows[off[i]:off[i + 1]].long()
+        v = torch.where(r[:, None] >= 0, xv[r.clamp(min=0)], torch.zeros((), dtype=torch.float64, device="cuda"))
+        z, mag = v @ wv[i].t() + bias[i].double(), v.abs() @ wv[i].abs().t()
+        lim = (k / 8 + 64) * 2.0 ** -23 * mag + 2.0 ** -23 * v.abs().sum(1, keepdim=True) * wv[i].abs().amax(1) + 2.0 ** -23 * z.abs()
+        if gated:                                                       # |silu'| < 1.1; the exponential, the division and the products below 2^-19 of the result
+            a, b, la, lb = z[:, :n], z[:, n:], lim[:, :n], lim[:, n:]
+            s = a * torch.sigmoid(a)
+            z, lim = s * b, 1.1 * la * b.abs() + s.abs() * lb + 1.1 * la * lb + 2.0 ** -19 * (s * b).abs()
+        assert ((got[off[i]:off[i + 1]] - z).abs() <= lim).all(), i
