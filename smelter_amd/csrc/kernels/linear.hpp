@@ -144,12 +144,12 @@ template <int KIND> __device__ __forceinline__ floatx16 lin_mma16(intx4_t a, int
     if constexpr (KIND == SM_F16) return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8_t, a), __builtin_bit_cast(half8_t, b), c, 0, 0, 0);
     else return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
 }
-// 16 x 16 x 128 product of MX4 fragments: lane l holds row l & 15 and one block of 32, with its scale byte in the low byte of sa / sb
-__device__ __forceinline__ floatx4 lin_mma4(intx4_t a, int sa, intx4_t b, int sb, floatx4 c) {
+// 16 x 16 x 128 (32 x 32 x 64) product of MX4 fragments: lane l holds row l % 16 (32) and one block of 32, with its scale in byte SEL of sa, in the low byte of sb
+template <int SEL> __device__ __forceinline__ floatx4 lin_mma4(intx4_t a, int sa, intx4_t b, int sb, floatx4 c) {
     const intx8_t va = __builtin_shufflevector(a, a, 0, 1, 2, 3, -1, -1, -1, -1), vb = __builtin_shufflevector(b, b, 0, 1, 2, 3, -1, -1, -1, -1);   // (a 4-bit operand is four registers)
-    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(va, vb, c, 4, 4, 0, sa, 0, sb);
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(va, vb, c, 4, 4, SEL, sa, 0, sb);
 }
-__device__ __forceinline__ floatx16 lin_mma4(intx4_t a, int sa, intx4_t b, int sb, floatx16 c) {   // 32 x 32 x 64
+template <int SEL> __device__ __forceinline__ floatx16 lin_mma4(intx4_t a, int sa, intx4_t b, int sb, floatx16 c) {
     const intx8_t va = __builtin_shufflevector(a, a, 0, 1, 2, 3, -1, -1, -1, -1), vb = __builtin_shufflevector(b, b, 0, 1, 2, 3, -1, -1, -1, -1);
-    return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(va, vb, c, 4, 4, 0, sa, 0, sb);
+    return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(va, vb, c, 4, 4, SEL, sa, 0, sb);
 }

@@ -94,7 +94,7 @@ template <int XK, int WK, int NB> __global__ __launch_bounds__(512) void lin_str
                     LinBlk<SM_MX4> x;
                     lin_load_block<SM_MX4>(x, xr, c + u * 4 * BL + g * BL + j, xnb, p.K);
 #pragma unroll
-                    for (int b = 0; b < NB; b++) acc[b] = lin_mma4(x.v[0], (int)(sx >> (8 * j)), w[u][b][j].v[0], (int)(sw[b] >> (8 * j)), acc[b]);
+                    for (int b = 0; b < NB; b++) acc[b] = lin_mma4<0>(x.v[0], (int)(sx >> (8 * j)), w[u][b][j].v[0], (int)(sw[b] >> (8 * j)), acc[b]);
                 }
             }
         } else {

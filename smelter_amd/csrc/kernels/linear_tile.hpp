@@ -304,10 +304,12 @@ __global__ __launch_bounds__(64 * WN * WM) void lin_tile_kernel(LinearParams p) 
         for (int b = 0; b < FM; b++)
 #pragma unroll
             for (int i = 0; i < FR * FR / 64; i++) acc[a][b][i] = 0.f;
-    intx4_t wf[2][GA], xf[2][FM]; int wsc[2][MX ? GA : 1], xsc[2][MX ? FM : 1];
+    intx4_t wf[2][GA], xf[2][FM];
+    int wall[MX ? FN : 1], xall[MX ? FM : 1], wsc[2][MX && HA == 1 ? GA : 1], xsc[2][MX ? FM : 1];   // scale bytes: of a lane's blocks of the step, and of the phase
     auto read = [&](int t, auto phase, bool masked) {
         constexpr int P = decltype(phase)::value, H = P / HA, A = P % HA, WB = P & 1, XB = H & 1;
-        const int ch = H * (64 / FR) + g;                                           // this lane's chunk of the row
+        // this lane's chunk of the row; of MX4 rows a lane takes neighbouring ones, whose scales are one 16- or 32-bit read a step (a byte read for each: 2.25 us a step of 256 x 256, against 1.9)
+        const int ch = MX ? g * (FR / 8) + H : H * (64 / FR) + g;
         const char* st = lds + (t & 1) * S::STAGE + r * 128 + ((ch ^ (lane & 7)) << 4);
 #pragma unroll
         for (int a = 0; a < GA; a++) wf[WB][a] = *(const intx4_t*)(st + (wn * FN + A * GA + a) * (FR * 128));
@@ -316,12 +318,23 @@ __global__ __launch_bounds__(64 * WN * WM) void lin_tile_kernel(LinearParams p) 
             for (int b = 0; b < FM; b++) xf[XB][b] = *(const intx4_t*)(st + (BN / FR + wm * FM + b) * (FR * 128));
         }
         if constexpr (MX) {
-            const unsigned char* sc = (const unsigned char*)lds + 2 * S::STAGE + (t & 1) * (BN + BM) * 8 + r * 8 + ch;
+            typedef std::conditional_t<FR == 16, unsigned short, int> Word;
+            const char* sc = lds + 2 * S::STAGE + (t & 1) * (BN + BM) * 8 + r * 8 + g * (FR / 8);
+            if constexpr (H == 0) {
 #pragma unroll
-            for (int a = 0; a < GA; a++) wsc[WB][a] = sc[(wn * FN + A * GA + a) * (FR * 8)];
+                for (int a = 0; a < GA; a++) wall[A * GA + a] = *(const Word*)(sc + (wn * FN + A * GA + a) * (FR * 8));
+                if constexpr (A == 0) {
+#pragma unroll
+                    for (int b = 0; b < FM; b++) xall[b] = *(const Word*)(sc + (BN / FR + wm * FM + b) * (FR * 8));
+                }
+            }
+            if constexpr (HA == 1) {                                                // (copies: the next step's are read while the last phase runs)
+#pragma unroll
+                for (int a = 0; a < GA; a++) wsc[WB][a] = wall[a] >> (8 * H);
+            }
             if constexpr (A == 0) {
 #pragma unroll
-                for (int b = 0; b < FM; b++) xsc[XB][b] = sc[(BN / FR + wm * FM + b) * (FR * 8)];
+                for (int b = 0; b < FM; b++) xsc[XB][b] = xall[b] >> (8 * H);
             }
         }
         if (masked) {                                                               // chunks behind the end of the row
@@ -341,7 +354,8 @@ __global__ __launch_bounds__(64 * WN * WM) void lin_tile_kernel(LinearParams p) 
 #pragma unroll
             for (int b = 0; b < FM; b++) {
                 AccT& c = acc[A * GA + a][b];
-                if constexpr (MX) c = lin_mma4(wf[WB][a], wsc[WB][a], xf[XB][b], xsc[XB][b], c);
+                if constexpr (MX && HA == 1) c = lin_mma4<0>(wf[WB][a], wsc[WB][a], xf[XB][b], xsc[XB][b], c);
+                else if constexpr (MX) c = lin_mma4<P / HA>(wf[WB][a], wall[A * GA + a], xf[XB][b], xsc[XB][b], c);
                 else c = lin_mma16<XK>(wf[WB][a], xf[XB][b], c);
             }
             between(a);
