@@ -351,6 +351,7 @@ __global__ __launch_bounds__(64 * WN * WM) void lin_tile_kernel(LinearParams p) 
         constexpr int P = decltype(phase)::value, A = P % HA, WB = P & 1, XB = (P / HA) & 1;
         sm_static_for<0, GA>([&](auto ai) {
             constexpr int a = decltype(ai)::value;
+            if constexpr (a == 1) __builtin_amdgcn_s_setprio(1);                    // the wave that has its fragments goes first, the other one of the SIMD reads: 1 - 2 %
 #pragma unroll
             for (int b = 0; b < FM; b++) {
                 AccT& c = acc[A * GA + a][b];
@@ -359,6 +360,7 @@ __global__ __launch_bounds__(64 * WN * WM) void lin_tile_kernel(LinearParams p) 
                 else c = lin_mma16<XK>(wf[WB][a], xf[XB][b], c);
             }
             between(a);
+            if constexpr (a == GA - 1) __builtin_amdgcn_s_setprio(0);
         });
     };
     typedef std::integral_constant<int, 0> First; typedef std::integral_constant<int, PH - 1> Last;
