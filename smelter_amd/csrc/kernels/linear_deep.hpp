@@ -37,10 +37,11 @@ template <int XK, int WK, int FM, int ST> __global__ __launch_bounds__(256) void
     const char* wexp = p.w + tile.e * p.w_es;
     const char* xbase = p.rows ? p.x : p.x + tile.row0 * p.x_ld;
 
-    // ---- LDS-DMA: 64 lanes fill 1 KB: 8 rows of 128 bytes (chunk c of row r at place c ^ (r & 7)), or 32 rows of 32 bytes of packed weights
+    // ---- LDS-DMA: 64 lanes fill 1 KB: 8 rows of 128 bytes (chunk c of row r at place c ^ (r & 7) ^ (r >> 4 & 1)), or 32 rows of 32 bytes of packed weights
     constexpr int QW = BN * S::WB / 4096, QX = BM / 32, QT = QW + QX;
     unsigned woff[QW], xoff[QX];
     const int wrow = DEQ ? lane >> 1 : lane >> 3, chunk = (lane & 7) ^ (lane >> 3);
+    auto swz = [](int row) { return row >> 4 & 1; };
 #pragma unroll
     for (int i = 0; i < QW; i++) woff[i] = (unsigned)(lin_weight_row(p, n0, (wave * QW + i) * (DEQ ? 32 : 8) + wrow) * p.w_ld);
 #pragma unroll
@@ -49,10 +50,10 @@ template <int XK, int WK, int FM, int ST> __global__ __launch_bounds__(256) void
     auto fill = [&](int t, int slot, int i) {                                       // instruction i of QT of step t; behind the end of a row: its last chunk again
         const unsigned st = lds0 + slot * S::STAGE;
         if (i < QW) {
-            int k = DEQ ? t * 32 + (lane & 1) * 16 : t * 128 + chunk * 16; if (k > w_bytes - 16) k = w_bytes - 16;
+            int k = DEQ ? t * 32 + (lane & 1) * 16 : t * 128 + (chunk ^ swz((wave * QW + i) * 8)) * 16; if (k > w_bytes - 16) k = w_bytes - 16;
             lin_dma16(wexp, woff[i < QW ? i : 0] + k, st + (wave * QW + i) * 1024);
         } else {
-            int k = t * 128 + chunk * 16; if (k > x_bytes - 16) k = x_bytes - 16;
+            int k = t * 128 + (chunk ^ swz((wave * QX + i - QW) * 8)) * 16; if (k > x_bytes - 16) k = x_bytes - 16;
             lin_dma16(xbase, xoff[i < QW ? 0 : i - QW] + k, st + BN * S::WB + (wave * QX + i - QW) * 1024);
         }
     };
@@ -118,7 +119,7 @@ template <int XK, int WK, int FM, int ST> __global__ __launch_bounds__(256) void
         }
 #pragma unroll
         for (int P = 0; P < 4; P++) {
-            const int ch = DEQ ? 4 * g + P : 2 * P + g, at = (ch ^ (lane & 7)) << 4;
+            const int ch = DEQ ? 4 * g + P : 2 * P + g, at = (ch ^ (lane & 7) ^ swz(r)) << 4;
             if constexpr (!DEQ) {
 #pragma unroll
                 for (int a = 0; a < FN; a++) wf[B][a][P] = *(const intx4_t*)(st + (wn * FN + a) * 32 * S::WB + at);

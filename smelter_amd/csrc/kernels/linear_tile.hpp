@@ -1,9 +1,11 @@
 // smelter_amd/csrc/kernels/linear_tile.hpp — linear layers on MANY rows: tiles of BN weight rows x BM slots through LDS, 128 bytes of K at a time.
 //
-// Both operands lie in LDS as rows of 128 bytes (64 16-bit elements, or 8 MX4 blocks = 256 elements), filled by the LDS-DMA without passing a register; 16-byte chunk c of row r sits at place
-// c ^ (r & 7), so that the 16 rows a fragment read touches spread over all banks.  The weights are the first operand of the matrix instruction: a lane then holds four consecutive columns of one
-// slot, which it stores together.  A 32 x 32 x 16 product of 16-bit fragments and a 32 x 32 x 64 product of MX4 fragments read the same bytes and take the same cycles, so both kinds share the
-// kernel; the MX4 one adds the scale bytes.  MX4 weights under a 16-bit x become 16-bit values on their way into LDS.
+// Both operands lie in LDS as rows of 128 bytes (64 16-bit elements, or 8 MX4 blocks = 256 elements), filled by the LDS-DMA without passing a register.  16-byte chunk c of row r sits at place
+// c ^ (r & 7), for fragments of 32 rows at c ^ (r & 7) ^ (r >> 4 & 1): the sixteen lanes that a 16-byte LDS read serves together (0 - 3, 12 - 15, 20 - 23, 24 - 27 and their like) then touch all
+// banks.  Without the second term 1000 x 4096 x 4096 in bfloat16 takes 50 us instead of 47; fragments of 16 rows with neighbouring chunks to a lane instead (their scales then lie together by
+// themselves) make 42 % of the LDS cycles conflicts, 3 % of the time of 8192^3 in MX4.
+// The weights are the first operand of the matrix instruction: a lane then holds four consecutive columns of one slot, which it stores together.  A product of 16-bit fragments and one of MX4
+// fragments read the same bytes in the same order, so both kinds share the kernel; the MX4 one adds the scale bytes.  MX4 weights under a 16-bit x become 16-bit values on their way into LDS.
 #pragma once
 #include "linear.hpp"
 
@@ -175,6 +177,7 @@ __global__ __launch_bounds__(64 * WN * WM) void lin_tile_kernel(LinearParams p) 
     unsigned woff[QW > 0 ? QW : 1], xoff[QX];                                        // bytes from the expert's weights / the tile's rows: lin_tile_fits() holds them below 2^32
     const char* xbase = p.rows ? p.x : p.x + tile.row0 * p.x_ld;
     const int chunk = (lane & 7) ^ (lane >> 3);
+    auto swz = [](int row) { return FR == 32 ? row >> 4 & 1 : 0; };
     if constexpr (!DEQ) {
 #pragma unroll
         for (int i = 0; i < QW; i++) woff[i] = (unsigned)(weight_row((wave * QW + i) * 8 + (lane >> 3)) * p.w_ld);
@@ -184,7 +187,8 @@ __global__ __launch_bounds__(64 * WN * WM) void lin_tile_kernel(LinearParams p) 
     const unsigned lds0 = lin_lds_addr(lds);
     constexpr int QT = QW + QX;
     auto fill = [&](int t, int i) {                                                 // instruction i of QT
-        int k = t * 128 + chunk * 16; if (k > x_bytes - 16) k = x_bytes - 16;       // behind the end: the row's last chunk again (masked when it is read)
+        const int q = i < QW ? wave * QW + i : wave * QX + i - QW;
+        int k = t * 128 + (chunk ^ swz(q * 8)) * 16; if (k > x_bytes - 16) k = x_bytes - 16;   // behind the end: the row's last chunk again (masked when it is read)
         const unsigned st = lds0 + (t & 1) * S::STAGE;
         if (i < QW) lin_dma16(wexp, woff[i < QW ? i : 0] + k, st + (wave * QW + i) * 1024);
         else lin_dma16(xbase, xoff[i - QW] + k, st + BN * 128 + (wave * QX + i - QW) * 1024);
@@ -254,20 +258,27 @@ __global__ __launch_bounds__(64 * WN * WM) void lin_tile_kernel(LinearParams p) 
             }
         }
         if constexpr (!DMA) {
-            const int k = t * 64 + chunk * 8, at = k < p.K - 8 ? k : p.K - 8;       // the last ones of a row as its last eight elements
+            auto at = [&](int q) { const int k = t * 64 + (chunk ^ swz(q * 8)) * 8; return 2ll * (k < p.K - 8 ? k : p.K - 8); };   // the last ones of a row as its last eight elements
             if constexpr (!DEQ) {
 #pragma unroll
-                for (int i = 0; i < QW; i++) __builtin_memcpy(&wreg[i], wexp + woff[i] + 2ll * at, 16);
+                for (int i = 0; i < QW; i++) __builtin_memcpy(&wreg[i], wexp + woff[i] + at(wave * QW + i), 16);
             }
 #pragma unroll
-            for (int i = 0; i < QX; i++) __builtin_memcpy(&xreg[i], xbase + xoff[i] + 2ll * at, 16);
+            for (int i = 0; i < QX; i++) __builtin_memcpy(&xreg[i], xbase + xoff[i] + at(wave * QX + i), 16);
         }
     };
     auto store_staged = [&](int t, auto end) {                                      // end: t may be the last step of a row
         if constexpr (MX) {
             const int over = nb >= 8 && 8 * t > nb - 8 ? 8 * t - (nb - 8) : 0;      // bytes of the step before, shifted out; behind the end (codes 0) scale 0
 #pragma unroll
-            for (int i = 0; i < SB; i++) *(unsigned long long*)(lds + 2 * S::STAGE + ((t & 1) * (BN + BM) + (i * THREADS + tid < BN + BM ? i * THREADS + tid : BN + BM - 1)) * 8) = sreg[i] >> (8 * over);
+            for (int i = 0; i < SB; i++) {
+                const unsigned long long v = sreg[i] >> (8 * over);
+                const unsigned lo = (unsigned)v, hi = (unsigned)(v >> 32);
+                // the bytes of a lane group side by side (one LDS read a step): blocks g, 4 + g of fragments of 16 rows, g, 2 + g, 4 + g, 6 + g of 32
+                const unsigned a = FR == 16 ? __builtin_amdgcn_perm(hi, lo, 0x05010400) : __builtin_amdgcn_perm(hi, lo, 0x06040200);
+                const unsigned b = FR == 16 ? __builtin_amdgcn_perm(hi, lo, 0x07030602) : __builtin_amdgcn_perm(hi, lo, 0x07050301);
+                *(unsigned long long*)(lds + 2 * S::STAGE + ((t & 1) * (BN + BM) + (i * THREADS + tid < BN + BM ? i * THREADS + tid : BN + BM - 1)) * 8) = a | (unsigned long long)b << 32;
+            }
         }
         if constexpr (DEQ) {
             char* st = lds + (t & 1) * S::STAGE;
@@ -278,18 +289,18 @@ __global__ __launch_bounds__(64 * WN * WM) void lin_tile_kernel(LinearParams p) 
                 if constexpr (XK == SM_F16) { const int d = byte - stop[i] + 127; byte = byte == 255 ? 255 : d > 0 ? d : 0; }
                 const float s = mx4_scale(byte);
 #pragma unroll
-                for (int q = 0; q < 4; q++) *(intx4_t*)(st + j * 128 + ((((tid & 1) * 4 + q) ^ (j & 7)) << 4)) = mx4_to16<XK>(code[i][q], s);
+                for (int q = 0; q < 4; q++) *(intx4_t*)(st + j * 128 + ((((tid & 1) * 4 + q) ^ (j & 7) ^ swz(j)) << 4)) = mx4_to16<XK>(code[i][q], s);
             }
         }
         if constexpr (!DMA) {
             char* st = lds + (t & 1) * S::STAGE + lane * 16;
-            const int k = t * 64 + chunk * 8, over = k > p.K - 8 ? k - (p.K - 8) : 0;   // elements before k in the eight; behind the row's end zeros
+            auto over = [&](int q) { const int k = t * 64 + (chunk ^ swz(q * 8)) * 8; return k > p.K - 8 ? k - (p.K - 8) : 0; };   // elements before k in the eight; behind the row's end zeros
             if constexpr (!DEQ) {
 #pragma unroll
-                for (int i = 0; i < QW; i++) { if constexpr (decltype(end)::value) wreg[i] = lin_drop(wreg[i], over); *(intx4_t*)(st + (wave * QW + i) * 1024) = wreg[i]; }
+                for (int i = 0; i < QW; i++) { if constexpr (decltype(end)::value) wreg[i] = lin_drop(wreg[i], over(wave * QW + i)); *(intx4_t*)(st + (wave * QW + i) * 1024) = wreg[i]; }
             }
 #pragma unroll
-            for (int i = 0; i < QX; i++) { if constexpr (decltype(end)::value) xreg[i] = lin_drop(xreg[i], over); *(intx4_t*)(st + BN * 128 + (wave * QX + i) * 1024) = xreg[i]; }
+            for (int i = 0; i < QX; i++) { if constexpr (decltype(end)::value) xreg[i] = lin_drop(xreg[i], over(wave * QX + i)); *(intx4_t*)(st + BN * 128 + (wave * QX + i) * 1024) = xreg[i]; }
         }
     };
     // ---- the products of a step in four phases (fragments of 32 rows: one for each 32 bytes of K; of 16 rows: one for each 64 bytes of K and each half of the wave's weight rows; 128-row tiles of
@@ -308,9 +319,8 @@ __global__ __launch_bounds__(64 * WN * WM) void lin_tile_kernel(LinearParams p) 
     int wall[MX ? FN : 1], xall[MX ? FM : 1], wsc[2][MX && HA == 1 ? GA : 1], xsc[2][MX ? FM : 1];   // scale bytes: of a lane's blocks of the step, and of the phase
     auto read = [&](int t, auto phase, bool masked) {
         constexpr int P = decltype(phase)::value, H = P / HA, A = P % HA, WB = P & 1, XB = H & 1;
-        // this lane's chunk of the row; of MX4 rows a lane takes neighbouring ones, whose scales are one 16- or 32-bit read a step (a byte read for each: 2.25 us a step of 256 x 256, against 1.9)
-        const int ch = MX ? g * (FR / 8) + H : H * (64 / FR) + g;
-        const char* st = lds + (t & 1) * S::STAGE + r * 128 + ((ch ^ (lane & 7)) << 4);
+        const int ch = H * (64 / FR) + g;                                           // this lane's chunk of the row
+        const char* st = lds + (t & 1) * S::STAGE + r * 128 + ((ch ^ (lane & 7) ^ swz(r)) << 4);
 #pragma unroll
         for (int a = 0; a < GA; a++) wf[WB][a] = *(const intx4_t*)(st + (wn * FN + A * GA + a) * (FR * 128));
         if constexpr (A == 0) {
