@@ -98,8 +98,8 @@ __device__ __forceinline__ LinTile lin_find_tile(const LinearParams& p, int BM, 
             const int at = __builtin_ctzll(past);
             const long long tl = t - r.total - (__shfl(sum, at) - __shfl(n, at));
             const long long l = __shfl(lo, at), h = __shfl(hi, at);
-            const long long row0 = l + tl * BM, left = h - row0;
-            r.e = base + at; r.row0 = lin_uniform(row0); r.rows = __builtin_amdgcn_readfirstlane((int)(left < BM ? left : BM));
+            const long long row0 = l + tl * BM, left = tl < 0 ? 0 : h - row0;         // (offsets that do not ascend may count more tiles than 32 bits hold)
+            r.e = base + at; r.row0 = lin_uniform(row0); r.rows = __builtin_amdgcn_readfirstlane((int)(left < 0 ? 0 : left < BM ? left : BM));
             if (!want_total) return r;
         }
         r.total += all;

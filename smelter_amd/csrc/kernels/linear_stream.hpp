@@ -144,11 +144,12 @@ template <int XK, int WK, int NB> __global__ __launch_bounds__(512) void lin_str
             for (int b = 0; b < NB; b++) { if constexpr (OWN) acc[b] += sum[b] * mul[b]; else acc[b] = sum[b]; }
         }
     }
-    // acc[b][i] = slot 4 g + i, weight row r of group b
+    // acc[b][i] = slot 4 g + i, weight row r of group b; a slot without a row of x: zero, also under weights that are infinite or NaN
+    const unsigned alive = (unsigned)__ballot(live) >> (4 * g);
 #pragma unroll
     for (int b = 0; b < NB; b++)
 #pragma unroll
-        for (int i = 0; i < 4; i++) part[((wave * NB + b) * 16 + 4 * g + i) * 17 + r] = acc[b][i];
+        for (int i = 0; i < 4; i++) part[((wave * NB + b) * 16 + 4 * g + i) * 17 + r] = alive >> i & 1 ? acc[b][i] : 0.f;
     __syncthreads();
     const float* bias = p.bias ? p.bias + (long long)tile.e * p.w_rows : nullptr;
     const int total = cols * tile.rows;

@@ -219,7 +219,7 @@ extern "C" int sm_moe_route(const void* scores, int32_t type, int64_t T, int32_t
     SM_REQUIRE(type == SM_F16 || type == SM_BF16 || type == SM_F32, "moe_route: type %d is not fp16, bf16 or fp32", type);
     SM_REQUIRE(E >= 1 && E <= MOE_MAX_E, "moe_route: %d experts (taken: 1 .. %d)", E, MOE_MAX_E);
     SM_REQUIRE(k >= 1 && k <= MOE_MAX_K && k <= E, "moe_route: %d of %d experts (taken: 1 .. min(%d, E))", k, E, MOE_MAX_K);
-    SM_REQUIRE(T >= 0 && T * k < (1ll << 31), "moe_route: %lld tokens x %d", (long long)T, k);
+    SM_REQUIRE(T >= 0 && T < (1ll << 31) && T * k < (1ll << 31), "moe_route: %lld tokens x %d", (long long)T, k);
     SM_REQUIRE(offsets && (T == 0 || (scores && weights && experts && rows && slots)), "moe_route: null operand");
     SM_REQUIRE(T <= 1 || ld >= E, "moe_route: row stride %lld below the %d scores", (long long)ld, E);
     SM_REQUIRE((size_t)scores % (type == SM_F32 ? 4 : 2) == 0, "moe_route: scores are not aligned to their element");

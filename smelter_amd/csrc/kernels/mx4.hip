@@ -103,9 +103,9 @@ extern "C" int sm_mx4_quantize(const void* x, int32_t x_type, int64_t rows, int3
     SM_REQUIRE(x_type == SM_F16 || x_type == SM_BF16 || x_type == SM_F32, "mx4_quantize: type %d is not fp16, bf16 or fp32", x_type);
     SM_REQUIRE(rows >= 0 && K >= 0, "mx4_quantize: negative size (%lld x %d)", (long long)rows, K);
     if (rows == 0 || K == 0) return SM_OK;
-    const int nb = (K + 31) / 32;
+    const int nb = K / 32 + (K % 32 != 0);
     SM_REQUIRE(x && codes && scales, "mx4_quantize: null operand");
-    SM_REQUIRE(rows < (1ll << 40), "mx4_quantize: %lld rows", (long long)rows);
+    SM_REQUIRE(rows <= (1ll << 40) / nb, "mx4_quantize: %lld x %d elements", (long long)rows, K);
     SM_REQUIRE(rows == 1 || x_ld >= K, "mx4_quantize: row stride %lld below the %d columns", (long long)x_ld, K);
     const int es = x_type == SM_F32 ? 4 : 2;
     SM_REQUIRE(((size_t)x % es) == 0 && ((size_t)codes & 15) == 0, "mx4_quantize: codes need 16-byte alignment, x its type's");
@@ -122,9 +122,9 @@ extern "C" int sm_mx4_dequantize(const void* codes, const void* scales, int64_t 
     SM_REQUIRE(y_type == SM_F16 || y_type == SM_BF16 || y_type == SM_F32, "mx4_dequantize: type %d is not fp16, bf16 or fp32", y_type);
     SM_REQUIRE(rows >= 0 && K >= 0, "mx4_dequantize: negative size (%lld x %d)", (long long)rows, K);
     if (rows == 0 || K == 0) return SM_OK;
-    const int nb = (K + 31) / 32;
+    const int nb = K / 32 + (K % 32 != 0);
     SM_REQUIRE(y && codes && scales, "mx4_dequantize: null operand");
-    SM_REQUIRE(rows < (1ll << 40), "mx4_dequantize: %lld rows", (long long)rows);
+    SM_REQUIRE(rows <= (1ll << 40) / nb, "mx4_dequantize: %lld x %d elements", (long long)rows, K);
     SM_REQUIRE(rows == 1 || y_ld >= K, "mx4_dequantize: row stride %lld below the %d columns", (long long)y_ld, K);
     const int es = y_type == SM_F32 ? 4 : 2;
     SM_REQUIRE(((size_t)y % es) == 0 && ((size_t)codes & 15) == 0, "mx4_dequantize: codes need 16-byte alignment, y its type's");

@@ -617,3 +617,78 @@ def test_groups_of_all_shapes(kind, k, gated, sizes, n):
             s = a * torch.sigmoid(a)
             z, lim = s * b, 1.1 * la * b.abs() + s.abs() * lb + 1.1 * la * lb + 2.0 ** -19 * (s * b).abs()
         assert ((got[off[i]:off[i + 1]] - z).abs() <= lim).all(), i
+
+
+# ---- what a caller may also do --------------------------------------------------------------------------------------------------------------
+
+WAYS = [(6, 40, 96), (90, 256, 512), (90, 256, 4096), (1500, 2048, 512), (4000, 4096, 256), (7000, 2048, 256)]     # slots, columns, K: streamed, few tiles, K split, the three tiles
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("m, n, k", WAYS)
+def test_weights_that_are_not_finite(kind, m, n, k):
+    """a weight row with an infinity or a NaN reaches its own column only, and no slot without a row of x (its product is zero, whatever the weights hold)"""
+    g = gen(m)
+    x, xv, w, wv, dt = operands(kind, g, m, k, (2, n, k))
+    rows = torch.arange(m, dtype=torch.int32)
+    rows[2::3] = -1
+    off = torch.tensor([0, m // 2 + 1, m], dtype=torch.int32, device="cuda")
+    bias = randn(g, 2, n)
+    fine = ops.expert_linear(x, w, off, rows.cuda(), bias.cuda())
+    if isinstance(w, ops.Mx4):
+        s = w.scales.clone()
+        s[:, 3, 0], s[:, 9, -1] = 255, 255
+        bad = ops.Mx4(w.codes, s, k)
+    else:
+        bad = w.clone()
+        bad[:, 3, 1], bad[:, 9, k - 1] = NAN, INF
+    got = ops.expert_linear(x, bad, off, rows.cuda(), bias.cuda())
+    cols = [j for j in range(n) if j not in (3, 9)]
+    assert torch.equal(got[:, cols], fine[:, cols])
+    none = rows.cuda() < 0
+    assert not torch.isfinite(got[~none][:, [3, 9]]).any()
+    want = bias.to(dt)[torch.bucketize(torch.arange(m), off.cpu()[1:], right=True)]
+    assert torch.equal(got[none].cpu(), want[rows < 0])
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f16-mx4", "mx4-mx4"])
+@pytest.mark.parametrize("m, n, k", WAYS[1:4])
+def test_two_calls_at_once(kind, m, n, k):
+    """the same layer on two streams at the same time, each with scratch of its own"""
+    g = gen(5)
+    x, xv, w, wv, dt = operands(kind, g, m, k, (1, n, k))
+    y, yv, _, _, _ = operands(kind, g, m, k, (1, 1, k))
+    off = torch.tensor([0, m], dtype=torch.int32, device="cuda")
+    want = [ops.expert_linear(v, w, off) for v in (x, y)]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(8):
+        for i, v in enumerate((x, y)):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(ops.expert_linear(v, w, off))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, want[i]) for i in range(2) for a in got[i])
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16-mx4", "mx4-mx4"])
+@pytest.mark.parametrize("m, n, k", WAYS[:5])
+def test_groups_that_overlap_or_descend(kind, m, n, k):
+    """offsets are meant to ascend; others cost nothing but the slots they name: nothing beside the slots is written"""
+    x, xv, w, wv, dt = operands(kind, gen(6), m, k, (4, n, k))
+    out = torch.full((m + 2, n), 7.0, dtype=dt, device="cuda")
+    for off in ([m, 0, m, 0, m], [0, m, 0, m, 0], [m, m, 0, 0, 0], [-(1 << 31), (1 << 31) - 1, -5, 3, 1 << 30]):
+        ops.expert_linear(x, w, torch.tensor(off, dtype=torch.int32, device="cuda"), out=out[1:m + 1])
+    assert out[0].eq(7).all() and out[m + 1].eq(7).all()
+
+
+def test_masked_scores_of_the_lowest_value():
+    """a mask of the type's lowest finite value is a score like any other: chosen last, with weight 0"""
+    for t in (F16, BF16, F32):
+        z = torch.full((70, 8), torch.finfo(t).min, dtype=t)
+        z[:, 5] = 1
+        p = ops.moe_route(z.cuda(), 2)
+        assert p.experts.cpu().eq(torch.tensor([5, 0])).all() and p.weights.cpu().eq(torch.tensor([1.0, 0.0])).all()
+        assert p.offsets.cpu().tolist() == [0, 70, 70, 70, 70, 70, 140, 140, 140]
+        p = ops.moe_route(torch.full((3, 8), torch.finfo(t).min, dtype=t).cuda(), 2)
+        assert p.experts.cpu().eq(torch.tensor([0, 1])).all() and p.weights.eq(0.5).all()

@@ -133,3 +133,13 @@ def test_plain_route_by_hand():
     r = mx4ref.route(torch.tensor([[1.0, 3.0, 3.0, 0.0], [-inf] * 4, [-inf, float("nan"), 2.0, -inf]]), 2, True)
     assert r["experts"].tolist() == [[1, 2], [-1, -1], [2, -1]] and r["weights"].tolist() == [[0.5, 0.5], [0, 0], [1, 0]]
     assert r["offsets"].tolist() == [0, 0, 1, 3, 3] and r["rows"].tolist() == [0, 0, 2, -1, -1, -1] and r["slots"].tolist() == [[0, 1], [-1, -1], [2, -1]]
+
+
+def test_sizes_that_would_overflow():
+    """products of sizes that pass 64 bits are refused, not wrapped"""
+    r = N.lib().sm_moe_route
+    refused(r(P, F32, (1 << 63) - 1, 8, 2, 8, 1, P, P, P, P, P, P, 1 << 62, None), "tokens")
+    refused(r(P, F32, 1 << 62, 8, 4, 8, 1, P, P, P, P, P, P, 1 << 62, None), "tokens")
+    q, dq = N.lib().sm_mx4_quantize, N.lib().sm_mx4_dequantize
+    refused(q(P, F16, 1 << 40, (1 << 31) - 1, (1 << 31) - 1, P, P, None), "elements")
+    refused(dq(P, P, 1 << 40, (1 << 31) - 1, P, F16, (1 << 31) - 1, None), "elements")
