@@ -565,8 +565,8 @@ def _refuse(msg, *args):
 
 def _on(index, call, *args):
     """run an enqueueing entry point on the current stream of device `index`"""
-    if index == torch.cuda.current_device():
-        rc = call(*args, torch._C._cuda_getCurrentRawStream(index))        # (torch.cuda.current_stream(index).cuda_stream without the Stream object: 2 us of a 4 us call)
+    if index == torch._C._cuda_getDevice():                                # (torch.cuda.current_device() and .current_stream(index).cuda_stream without their detours: 2 us of a 4 us call)
+        rc = call(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(index):
             rc = call(*args, torch._C._cuda_getCurrentRawStream(index))
@@ -603,12 +603,12 @@ def _rows2d(t, name):
 
 def _gpu(index, name, t, dtypes):
     """the device index of a tensor of one of `dtypes` (on device `index`, if given)"""
-    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+    at = t.get_device() if isinstance(t, torch.Tensor) and t.is_cuda else -1
+    if at < 0:
         _refuse("%s: a tensor on the GPU is wanted", name)
     if t.dtype not in dtypes:
         _refuse("%s: type %s is not taken", name, t.dtype)
-    at = t.get_device()
-    if index is not None and at != index:
+    if at != index and index is not None:
         _refuse("%s: tensors on devices %d and %d", name, index, at)
     return at
 
@@ -622,9 +622,11 @@ def _check_mx4(q, index, name):
     c, s, k = q
     index = _gpu(index, name, c, _BYTES)
     _gpu(index, name, s, _BYTES)
-    nb, cs, ss = (k + 31) // 32, c.shape, s.shape
-    if k < 0 or not cs or len(cs) != len(ss) or cs[-1] != 16 * nb or ss[-1] != nb or cs[:-1] != ss[:-1]:
-        _refuse("%s: codes %s and scales %s for %d columns", name, tuple(cs), tuple(ss), k)
+    nb = (k + 31) // 32
+    *cs, cb = c.shape or (-1,)
+    *ss, sb = s.shape or (-1,)
+    if k < 0 or sb != nb or cb != 16 * nb or cs != ss:
+        _refuse("%s: codes %s and scales %s for %d columns", name, tuple(c.shape), tuple(s.shape), k)
     if not c.is_contiguous() or not s.is_contiguous() or c.data_ptr() & 15:
         _refuse("%s: codes and scales must be contiguous, codes 16-byte aligned", name)
     return index
