@@ -35,7 +35,8 @@ __device__ __forceinline__ float lin_act(float v, int act, float slope) {
     if (act == SM_ACT_PRELU) return v < 0.f ? v * slope : v;
     return sm_act_other(v, act, slope);
 }
-__device__ __forceinline__ float lin_silu(float v) { return v / (1.f + __expf(-v)); }
+// the hardware's reciprocal (1 step; below v = -87 its result is 0): a division costs ten instructions a value, 11 us of the 94 of 8192 x 4096 gated columns with K = 2048 in MX4
+__device__ __forceinline__ float lin_silu(float v) { return v * __builtin_amdgcn_rcpf(1.f + __expf(-v)); }
 
 // one rounding to the output type (nearest even)
 __device__ __forceinline__ void lin_store1(void* y, long long i, float v, int type) {

@@ -90,7 +90,7 @@ template <int XK, int WK, int FM, int ST> __global__ __launch_bounds__(256) void
             for (int b = tid & 1; b < blocks; b += 2) top = top > row[b] ? top : row[b];
             const int o = __shfl_xor(top, 1); top = top > o ? top : o;
             for (int b = tid & 1; b < blocks; b += 2) { const int d = row[b] - top + 127; row[b] = row[b] == 255 ? 255 : d > 0 ? d : 0; }
-            if (!(tid & 1)) wmul[j] = mx4_scale(top);
+            if (!(tid & 1)) wmul[j] = mx4_scale(top < 255 ? top : 254);       // (finite also for a row with a NaN: its sums are NaN by themselves, those of slots without a row 0)
         }
     }
 
@@ -181,7 +181,7 @@ template <int XK, int WK, int FM, int ST> __global__ __launch_bounds__(256) void
 #pragma unroll 1
         for (; t < steps; t += 2) { tail(t, I0()); if (t + 1 < steps) tail(t + 1, I1()); }
     }
-    lin_finish<32, 2, 2, FN, FM, S::DUMP, DEQ && XK == SM_F16>(p, tile, split, n0, acc, dlds, wmul);
+    lin_finish<XK, 32, 2, 2, FN, FM, S::DUMP, DEQ && XK == SM_F16>(p, tile, split, n0, acc, dlds, wmul);
 }
 
 // a kernel's dynamic LDS may be the whole 160 KB on the current device; asked for once per kernel and device

@@ -46,10 +46,110 @@ __device__ __forceinline__ long long lin_slot_row(const LinearParams& p, const L
     return s;
 }
 
-// Epilogue of the tile kernels: acc[a][b][i] = tile row FR (wn FN + a) + 8 (i / 4) + 4 g + i % 4 of the weights, slot FR (wm FM + b) + r.  The fp32 tile goes through LDS (chunks of four columns, xor-ed with the slot) so that a
-// thread stores eight consecutive columns: whole 512-byte rows instead of 8-byte pieces.  BYTES of LDS, all of it free once every wave is here.  SCALED: wmul[row] = the factor of a weight row.
+// Epilogue of the tile kernels: acc[a][b][i] = tile row FR (wn FN + a) + 8 (i / 4) + 4 g + i % 4 of the weights, slot FR (wm FM + b) + r: quads of four consecutive columns of a slot, quad j of a
+// lane at column CW j + 4 g of its wave; gate and up row of a column lie in the same lane.  SCALED: wmul[row] = the factor of a weight row.
+template <int FR, int FN, int FM> struct LinQuads {
+    static constexpr int Q = FR * FR / 256, N = FN * Q, CW = 256 / FR, UP = 16 / CW;   // quads of a fragment, of a wave; columns from one to the next; quads from a gate row to its up row
+};
+template <int FR, int FN, int FM, bool SCALED, int J, class AccT> __device__ __forceinline__ floatx4 lin_quad(const AccT (&acc)[FN][FM], int b, const float* wmul) {
+    constexpr int Q = LinQuads<FR, FN, FM>::Q, q = J % Q;
+    const AccT& c = acc[J / Q][b];
+    floatx4 v = {c[4 * q], c[4 * q + 1], c[4 * q + 2], c[4 * q + 3]};
+    if constexpr (SCALED) v *= *(const floatx4*)(wmul + LinQuads<FR, FN, FM>::CW * J);
+    return v;
+}
+
+// The sums of a run of K, in the order of the weight rows; lin_join_kernel adds them.
+template <int FR, int FN, int FM, bool SCALED, class AccT>
+__device__ __forceinline__ void lin_finish_split(const LinearParams& p, const LinTile& tile, int split, int n0, int row0, const AccT (&acc)[FN][FM], const int (&slot)[FM], const float* wmul) {
+    typedef LinQuads<FR, FN, FM> L;
+    sm_static_for<0, L::N>([&](auto index) {
+        constexpr int j = decltype(index)::value;
+        const int row = row0 + L::CW * j, n = p.gated ? n0 + ((row >> 5) << 4) + (row & 15) : n0 + row;
+#pragma unroll
+        for (int b = 0; b < FM; b++) {
+            const floatx4 v = lin_quad<FR, FN, FM, SCALED, j>(acc, b, wmul);
+            if (slot[b] >= tile.rows || n >= p.N) continue;
+            float* dst = p.part + ((long long)split * p.M + tile.row0 + slot[b]) * p.part_ld + n + (p.gated && (row & 16) ? p.N : 0);
+            if (n + 4 <= p.N && (!p.gated || p.N % 4 == 0)) *(floatx4*)dst = v;
+            else {
+#pragma unroll
+                for (int i = 0; i < 4; i++) if (n + i < p.N) dst[i] = v[i];
+            }
+        }
+    });
+}
+
+// The outputs from the registers, where N is a multiple of 8 and rows of y are 16-byte aligned.  Of 16-bit outputs two lanes exchange a quad each, so that every lane stores 16 bytes and a slot's
+// columns come in pieces of 32 or 64.  Everything that is the same for the whole launch is decided outside.  ACT: an activation of the ReLU family.
+template <int FR, int WN, int WM, int FN, int FM, bool SCALED, int YT, bool GATED, bool ACT, class AccT>
+__device__ __forceinline__ void lin_finish_registers(const LinearParams& p, const LinTile& tile, int n0, int g, int wn, const AccT (&acc)[FN][FM], const int (&slot)[FM], const float* wmul) {
+    typedef LinQuads<FR, FN, FM> L;
+    constexpr int ZN = GATED ? L::N / 2 : L::N, CW = L::CW, ES = YT == SM_F32 ? 4 : 2;   // quads of outputs
+    const int first = n0 + ZN / L::Q * FR * wn;                                      // first column of this wave
+    const int lane_col = YT == SM_F32 ? 4 * g : CW * (g & 1) + 8 * (g >> 1);
+    const bool relu = p.act == SM_ACT_RELU;
+    floatx4 add[L::N];
+    if (p.bias) {
+        const float* bias = p.bias + (long long)tile.e * p.w_rows;
+        sm_static_for<0, ZN>([&](auto index) {
+            constexpr int j = decltype(index)::value;
+            const int n = first + CW * j + 4 * g, at = n < p.N ? n : p.N - 4;       // (behind the last column: not stored)
+            __builtin_memcpy(&add[j], bias + at, 16);
+            if constexpr (GATED) __builtin_memcpy(&add[ZN + j], bias + at + p.N, 16);
+        });
+    } else {
+#pragma unroll
+        for (int j = 0; j < L::N; j++) add[j] = floatx4{0, 0, 0, 0};
+    }
+    auto output = [&](auto index, int b) {                                          // quad j of the outputs
+        constexpr int j = decltype(index)::value;
+        if constexpr (GATED) {
+            constexpr int at = j / L::UP * 2 * L::UP + j % L::UP;
+            const floatx4 z = lin_quad<FR, FN, FM, SCALED, at>(acc, b, wmul) + add[j], u = lin_quad<FR, FN, FM, SCALED, at + L::UP>(acc, b, wmul) + add[ZN + j];
+            return floatx4{lin_silu(z[0]) * u[0], lin_silu(z[1]) * u[1], lin_silu(z[2]) * u[2], lin_silu(z[3]) * u[3]};
+        } else {
+            floatx4 z = lin_quad<FR, FN, FM, SCALED, j>(acc, b, wmul) + add[j];
+            if constexpr (ACT) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) z[i] = z[i] < 0.f ? (relu ? 0.f : z[i] * p.slope) : z[i];
+            }
+            return z;
+        }
+    };
+#pragma unroll
+    for (int b = 0; b < FM; b++) {
+        if (slot[b] >= tile.rows) continue;
+        char* dst = (char*)p.y + ((tile.row0 + slot[b]) * p.y_ld + first + lane_col) * ES;
+        const int left = p.N - first - lane_col;                                     // columns that exist from this lane's first on
+        if constexpr (YT == SM_F32) {
+            sm_static_for<0, ZN>([&](auto index) { constexpr int j = decltype(index)::value; const floatx4 v = output(index, b); if (CW * j < left) *(floatx4*)(dst + CW * j * 4) = v; });
+        } else {
+            sm_static_for<0, ZN / 2>([&](auto pair) {
+                constexpr int j = 2 * decltype(pair)::value;
+                unsigned h[2][2];
+                auto round = [&](floatx4 z, unsigned* to) {
+                    if constexpr (YT == SM_F16) { const half4_t t = {(half_t)z[0], (half_t)z[1], (half_t)z[2], (half_t)z[3]}; __builtin_memcpy(to, &t, 8); }
+                    else { const bf16x4_t t = {(bf16_t)z[0], (bf16_t)z[1], (bf16_t)z[2], (bf16_t)z[3]}; __builtin_memcpy(to, &t, 8); }
+                };
+                round(output(std::integral_constant<int, j>(), b), h[0]); round(output(std::integral_constant<int, j + 1>(), b), h[1]);
+                // odd lane groups give their quad j for the quad j + 1 of the group before: even ones then hold eight columns of the one, odd ones of the other
+                intx4_t v;
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    const auto s = FR == 16 ? __builtin_amdgcn_permlane16_swap(h[0][i], h[1][i], false, false) : __builtin_amdgcn_permlane32_swap(h[0][i], h[1][i], false, false);
+                    v[i] = (int)s[0]; v[2 + i] = (int)s[1];
+                }
+                if (CW * j < left) *(intx4_t*)(dst + CW * j * 2) = v;
+            });
+        }
+    }
+}
+
+// Other activations, other N, other rows of y: through LDS, the fp32 tile in chunks of four columns, xor-ed with the slot; a thread takes eight consecutive columns.  BYTES of LDS, all of it free
+// once every wave is here.  (8192 x 8192 outputs of K = 512 in MX4: 62 us this way, 48 from the registers, 30 without the stores.)
 template <int FR, int WN, int WM, int FN, int FM, int BYTES, bool SCALED, class AccT>
-__device__ __forceinline__ void lin_finish(const LinearParams& p, const LinTile& tile, int split, int n0, AccT (&acc)[FN][FM], char* lds, const float* wmul) {
+__device__ __forceinline__ void lin_finish_lds(const LinearParams& p, const LinTile& tile, int n0, AccT (&acc)[FN][FM], char* lds, const float* wmul) {
     constexpr int BN = FR * FN * WN, THREADS = 64 * WN * WM;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & (FR - 1), g = lane / FR, wn = wave % WN, wm = wave / WN;
     const int cols = p.gated ? BN / 2 : BN;
@@ -72,27 +172,6 @@ __device__ __forceinline__ void lin_finish(const LinearParams& p, const LinTile&
                 }
             }
         __syncthreads();
-        if (p.splits > 1) {                                                         // the sums of a run, in the order of the weight rows; lin_join_kernel adds them
-            constexpr int per = BN / 8;
-            for (int o = tid; o < PB * WM * FR * per; o += THREADS) {
-                const int l = o / per, j = (o - l * per) * 8;
-                const int slot = (l / (FR * PB) * FM + b0) * FR + l % (FR * PB);
-                const int n = p.gated ? n0 + ((j >> 5) << 4) + (j & 15) : n0 + j;
-                if (slot >= tile.rows || n >= p.N) continue;
-                const char* row = lds + l * BN * 4;
-                const int x = l & 15;
-                const bool dead = p.rows && lin_slot_row(p, tile, slot) < 0;
-                floatx4 v[2] = {*(const floatx4*)(row + ((j / 4 ^ x) << 4)), *(const floatx4*)(row + (((j / 4 + 1) ^ x) << 4))};
-                if (dead) v[0] = v[1] = floatx4{0, 0, 0, 0};
-                float* dst = p.part + ((long long)split * p.M + tile.row0 + slot) * p.part_ld + n + (p.gated && (j & 16) ? p.N : 0);
-                if (n + 8 <= p.N && (!p.gated || p.N % 4 == 0)) { *(floatx4*)dst = v[0]; *(floatx4*)(dst + 4) = v[1]; }
-                else {
-#pragma unroll
-                    for (int i = 0; i < 8; i++) if (n + i < p.N) dst[i] = v[i >> 2][i & 3];
-                }
-            }
-            continue;
-        }
         const int per = cols / 8;
         for (int o = tid; o < PB * WM * FR * per; o += THREADS) {
             const int l = o / per, c = o - l * per, n = n0 + c * 8;                 // LDS row, group of eight columns
@@ -105,7 +184,6 @@ __device__ __forceinline__ void lin_finish(const LinearParams& p, const LinTile&
                 const floatx4 q0 = *(const floatx4*)(row + ((ch ^ x) << 4)), q1 = *(const floatx4*)(row + (((ch + 1) ^ x) << 4));
 #pragma unroll
                 for (int i = 0; i < 4; i++) { q[i] = q0[i]; q[4 + i] = q1[i]; }
-                if (p.rows && lin_slot_row(p, tile, slot) < 0) for (int i = 0; i < 8; i++) q[i] = 0.f;
                 if (bias) {
                     if (n + 8 <= p.N) {
                         float t[8]; __builtin_memcpy(t, bias + n + up, 32);
@@ -130,6 +208,44 @@ __device__ __forceinline__ void lin_finish(const LinearParams& p, const LinTile&
             else for (int i = 0; i < 8; i++) if (n + i < p.N) lin_store1(p.y, out + i, v[i], p.y_type);
         }
     }
+}
+
+template <int XK, int FR, int WN, int WM, int FN, int FM, int BYTES, bool SCALED, class AccT>
+__device__ __forceinline__ void lin_finish(const LinearParams& p, const LinTile& tile, int split, int n0, AccT (&acc)[FN][FM], char* lds, const float* wmul) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), r = lane & (FR - 1), g = lane / FR, wn = wave % WN, wm = wave / WN;
+    if constexpr (SCALED) __syncthreads();                                          // (wmul, of a product without a step)
+    int slot[FM]; bool dead[FM], any = false;
+#pragma unroll
+    for (int b = 0; b < FM; b++) {
+        slot[b] = FR * (wm * FM + b) + r;
+        dead[b] = p.rows && lin_slot_row(p, tile, slot[b]) < 0;
+        any |= dead[b];
+    }
+    if (__any(any)) {                                                               // slots without a row of x: zero, also under weights that are infinite or NaN
+#pragma unroll
+        for (int a = 0; a < FN; a++)
+#pragma unroll
+            for (int b = 0; b < FM; b++)
+#pragma unroll
+                for (int i = 0; i < FR * FR / 64; i++) acc[a][b][i] = dead[b] ? 0.f : acc[a][b][i];
+    }
+    const int row0 = FR * wn * FN + 4 * g;
+    if constexpr (FR == 32 && FM == 1) if (p.splits > 1) { lin_finish_split<FR, FN, FM, SCALED>(p, tile, split, n0, row0, acc, slot, wmul + row0); return; }
+    if (p.y_vec && p.N % 8 == 0 && p.act <= SM_ACT_PRELU) {
+        if (wm * FM * FR >= tile.rows) return;
+        auto go = [&](auto type) {
+            constexpr int YT = decltype(type)::value;
+            if (p.gated) lin_finish_registers<FR, WN, WM, FN, FM, SCALED, YT, true, false>(p, tile, n0, g, wn, acc, slot, wmul + row0);
+            else if (p.act != SM_ACT_NONE) lin_finish_registers<FR, WN, WM, FN, FM, SCALED, YT, false, true>(p, tile, n0, g, wn, acc, slot, wmul + row0);
+            else lin_finish_registers<FR, WN, WM, FN, FM, SCALED, YT, false, false>(p, tile, n0, g, wn, acc, slot, wmul + row0);
+        };
+        if (p.y_type == SM_F32) go(std::integral_constant<int, SM_F32>());
+        else if constexpr (XK != SM_MX4) go(std::integral_constant<int, XK>());
+        else if (p.y_type == SM_F16) go(std::integral_constant<int, SM_F16>());
+        else go(std::integral_constant<int, SM_BF16>());
+        return;
+    }
+    lin_finish_lds<FR, WN, WM, FN, FM, BYTES, SCALED>(p, tile, n0, acc, lds, wmul);
 }
 
 // the eight 16-bit elements of v without the first n, zeros behind them
@@ -220,7 +336,7 @@ __global__ __launch_bounds__(64 * WN * WM) void lin_tile_kernel(LinearParams p) 
                 for (int b = 0; b < nb && nb < 16; b++) up(ssrc[i][b]);
                 const int o = __shfl_xor(top, 1); top = top > o ? top : o;
                 stop[i] = top;
-                if (!(tid & 1)) wmul[j] = mx4_scale(top);
+                if (!(tid & 1)) wmul[j] = mx4_scale(top < 255 ? top : 254);       // (finite also for a row with a NaN: its sums are NaN by themselves, those of slots without a row 0)
             }
         }
     }
@@ -440,7 +556,7 @@ __global__ __launch_bounds__(64 * WN * WM) void lin_tile_kernel(LinearParams p) 
     if (t + 1 < steps) { step(t, std::true_type(), std::false_type(), std::false_type()); t++; }
     if (t < steps) step(t, std::false_type(), std::false_type(), std::false_type());
 
-    lin_finish<FR, WN, WM, FN, FM, 2 * S::STAGE, DEQ && XK == SM_F16>(p, tile, split, n0, acc, lds, wmul);
+    lin_finish<XK, FR, WN, WM, FN, FM, 2 * S::STAGE, DEQ && XK == SM_F16>(p, tile, split, n0, acc, lds, wmul);
 }
 
 template <int XK, int WK, int FR, int WN, int WM, int FN, int FM, bool DMA> static int lin_tile(const LinearParams& q, hipStream_t s) {
