@@ -39,10 +39,28 @@ static LinearPlan lin_plan(const sm_linear_desc* d, bool grouped, bool gathered)
     const long long per = grouped ? (d->M + d->E - 1) / d->E : d->M;
     LinearPlan plan = {-1, 1, 0};
     if (per <= 16 || d->K < 8 || !lin_tile_fits(p)) return plan;
-    auto tiles = [&](int bn, int bm) { const int cols = p.gated ? bn / 2 : bn; return lin_row_tiles(p, bm) * ((p.N + cols - 1) / cols); };
+    // the tiles to expect: groups end anywhere inside their last tile (E = 1: of all slots)
+    auto tiles = [&](int bn, int bm) {
+        const int cols = p.gated ? bn / 2 : bn;
+        const long long groups = d->M < d->E ? d->M : d->E, most = lin_row_tiles(p, bm), half = d->M / bm + (groups + 1) / 2, row = half < groups ? groups : half;
+        return (groups == 1 || row > most ? most : row) * ((p.N + cols - 1) / cols);
+    };
+    // Times in units of a round of 512 tiles of 128 x 128, two on a CU (69 us of fp16 with K = 4096, 29 of MX4 by MX4).  A round that is not full costs less, but not in proportion, and differently
+    // for each tile: a CU that holds one tile of 128 x 128 needs 0.6 of the time it needs for two.  Measured on 4096 x 4096 weights in fp16 (us; tiles of 128 x 128 / 256 x 256 / 128 x 64):
+    // 512 rows 39 / 60 / 29, 640 rows 40 / 60 / 44, 1280 rows 55 / 61 / 56, 2048 rows 69 / 67 / 98, 2304 rows 109 / 80 / 101, 4096 rows 135 / 108 / 168; MX4 weights under them: 42 / 88 / 32,
+    // 43 / 87 / 52, 59 / 88 / 73, 79 / 91 / 127, 131 / 91 / 130, 152 / 109 / 218.
     const long long n0 = tiles(128, 128), n1 = tiles(256, 256), n2 = tiles(128, 64);
-    // times in units of a round of 512 tiles of 128 x 128, two on a CU
-    const double t0 = n0 <= 256 ? 0.65 : n0 <= 384 ? 0.75 : n0 / 512.0, t1 = (n1 + 255) / 256 * 1.24, t2 = n2 <= 256 ? 0.42 : n2 * 0.75 / 512.0 < 0.7 ? 0.7 : n2 * 0.75 / 512.0;
+    const bool w16 = d->w_type != SM_MX4;
+    auto time = [&](int shape, long long n) {
+        const long long round = shape == 0 ? 512 : shape == 1 ? 256 : 768, r = n % round;
+        const double full = shape == 0 ? 0.97 : shape == 1 ? (w16 ? 1.55 : 1.38) : 0.95;
+        const double part = r == 0 ? 0 : shape == 0 ? (r <= 256 ? 0.6 : 0.8 + 0.2 * (r - 256) / 256) : shape == 1 ? (w16 && r <= 128 ? 0.9 : r <= 192 ? 1.1 : full)    // (w16: the halves of lin_pick_tile)
+                          : r <= 256 ? 0.42 : r <= 512 ? 0.7 : w16 ? 0.82 : 0.95;
+        return n / round * full + part;
+    };
+    // the number of tiles of ragged groups may lie on either side of a whole round: the mean over a tenth more and less
+    auto mean = [&](int shape, long long n) { return !grouped || d->E == 1 ? time(shape, n) : (time(shape, n - n / 10) + time(shape, n) + time(shape, n + n / 10)) / 3; };
+    const double t0 = mean(0, n0), t1 = mean(1, n1), t2 = mean(2, n2);
     plan.shape = t2 <= t0 && t2 <= t1 ? 2 : t0 <= t1 ? 0 : 1;
     const long long n = plan.shape == 2 ? n2 : n0;
     plan.deep = d->x_type != SM_MX4 && plan.shape != 1 && n <= SM_NUM_CU;

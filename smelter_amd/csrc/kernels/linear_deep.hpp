@@ -28,7 +28,7 @@ template <int XK, int WK, int FM, int ST> __global__ __launch_bounds__(256) void
     extern __shared__ __align__(16) char dlds[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 31, g = lane >> 5;
     int split, nt;
-    const LinTile tile = lin_pick_tile(p, BM, &split, &nt);
+    const LinTile tile = lin_pick_tile<false>(p, BM, &split, &nt);
     if (tile.rows == 0) return;
     const int nb = (p.K + 31) >> 5, w_bytes = DEQ ? 16 * nb : 2 * p.K, x_bytes = 2 * p.K;
     const int every = (x_bytes + 127) >> 7, first = (int)((long long)every * split / p.splits), steps = (int)((long long)every * (split + 1) / p.splits);

@@ -19,19 +19,31 @@ __device__ __forceinline__ void lin_arrive() { asm volatile("s_waitcnt vmcnt(0) 
 
 // Which tile (and which run of K) this block has: consecutive tiles stay on one XCD (blocks are dealt to the 8 XCDs in turn), in squares of up to 8 row tiles, so that an XCD's L2 holds what its
 // CUs read together.  The number of row tiles is known on the device only; blocks to spare get an empty tile.
-__device__ __forceinline__ LinTile lin_pick_tile(const LinearParams& p, int BM, int* split, int* nt) {
+// HALVES (a tile to a CU): where the last round of an XCD's tiles fills at most half of its CUs, two blocks take the halves of each of these tiles.
+template <bool HALVES> __device__ __forceinline__ LinTile lin_pick_tile(const LinearParams& p, int BM, int* split, int* nt) {
     LinTile none; none.rows = 0;
     *split = p.splits > 1 ? (int)(blockIdx.x % (unsigned)p.splits) : 0;
     const LinTile all = lin_find_tile(p, BM, 0, true);
     const long long total = all.total * p.n_tiles;
     const long long b = p.splits > 1 ? blockIdx.x / (unsigned)p.splits : blockIdx.x, q = total >> 3;
     const int xcd = (int)(b & 7), rem = (int)(total & 7);
-    if ((b >> 3) >= q + (xcd < rem ? 1 : 0)) return none;
-    const long long id = xcd * q + (xcd < rem ? xcd : rem) + (b >> 3);
+    const long long mine = q + (xcd < rem ? 1 : 0);                                 // tiles of this XCD
+    long long at = b >> 3; int half = -1;
+    if constexpr (HALVES) {
+        const int over = (int)(mine % (SM_NUM_CU / 8));
+        if (over <= SM_NUM_CU / 16 && at >= mine - over) { const int j = (int)(at - (mine - over)); half = j & 1; at = mine - over + (j >> 1); }
+    }
+    if (at >= mine) return none;
+    const long long id = xcd * q + (xcd < rem ? xcd : rem) + at;
     const long long band = id / (8ll * p.n_tiles);
     const int in = (int)(id - band * 8 * p.n_tiles), high = (int)(all.total - band * 8 < 8 ? all.total - band * 8 : 8);
     *nt = in / high;
-    return lin_find_tile(p, BM, band * 8 + in - *nt * high, false);
+    LinTile tile = lin_find_tile(p, BM, band * 8 + in - *nt * high, false);
+    if (HALVES && half >= 0) {
+        if (half) { tile.row0 += BM / 2; tile.rows = tile.rows > BM / 2 ? tile.rows - BM / 2 : 0; }
+        else if (tile.rows > BM / 2) tile.rows = BM / 2;
+    }
+    return tile;
 }
 // weight row of tile row j: gated tiles alternate 16 gate rows and their 16 up rows
 __device__ __forceinline__ long long lin_weight_row(const LinearParams& p, int n0, int j) {
@@ -276,7 +288,8 @@ __global__ __launch_bounds__(64 * WN * WM) void lin_tile_kernel(LinearParams p) 
     const int r = lane & (FR - 1), g = lane / FR;
 
     int split, nt;
-    const LinTile tile = lin_pick_tile(p, BM, &split, &nt);
+    constexpr bool HALVES = FR == 16 && DMA && !DEQ && !MX;                         // (the others' waves have work for each other: a half takes as long)
+    const LinTile tile = lin_pick_tile<HALVES>(p, BM, &split, &nt);
     if (tile.rows == 0) return;
     const int row_bytes = MX || DEQ ? 16 * ((p.K + 31) >> 5) : 2 * p.K;             // of a weight row
     const int x_bytes = MX ? row_bytes : 2 * p.K;
@@ -565,7 +578,7 @@ template <int XK, int WK, int FR, int WN, int WM, int FN, int FM, bool DMA> stat
     const int cols = p.gated ? S::BN / 2 : S::BN;
     p.n_tiles = (p.N + cols - 1) / cols;
     p.m_tiles = lin_row_tiles(p, S::BM);
-    const long long blocks = (p.m_tiles * p.n_tiles + 7) / 8 * 8 * p.splits;
+    const long long blocks = (p.m_tiles * p.n_tiles + 7) / 8 * 8 * p.splits + (FR == 16 ? SM_NUM_CU / 2 : 0);   // (and the second halves of lin_pick_tile)
     SM_REQUIRE(blocks < (1ll << 31), "linear: %lld row tiles x %d column tiles exceed one launch", p.m_tiles, p.n_tiles);
     lin_tile_kernel<XK, WK, FR, WN, WM, FN, FM, DMA><<<dim3((unsigned)blocks), S::THREADS, 0, s>>>(p);
     SM_LAUNCH_CHECK();

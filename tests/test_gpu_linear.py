@@ -692,3 +692,17 @@ def test_masked_scores_of_the_lowest_value():
         assert p.offsets.cpu().tolist() == [0, 70, 70, 70, 70, 70, 140, 140, 140]
         p = ops.moe_route(torch.full((3, 8), torch.finfo(t).min, dtype=t).cuda(), 2)
         assert p.experts.cpu().eq(torch.tensor([0, 1])).all() and p.weights.eq(0.5).all()
+
+
+@pytest.mark.parametrize("kind, aligned", [(k, True) for k in KINDS] + [(k, False) for k in KINDS if k != "mx4-mx4"])
+@pytest.mark.parametrize("m, n, k", [(4400, 4096, 264), (1400, 4000, 200), (1100, 4000, 136), (2000, 4040, 72)])
+def test_products_between_whole_rounds(kind, aligned, m, n, k):
+    """numbers of tiles a little above what the card holds at once (the last ones are cut in half), one tile of 128 x 128 to some CUs and two to others"""
+    test_products_of_all_shapes(kind, m, n, k, aligned)
+
+
+@pytest.mark.parametrize("kind, k", [(k, 136) for k in KINDS] + [(k, 133) for k in KINDS if k != "mx4-mx4"])
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("sizes, n", [([1100, 0, 130, 90], 3900), ([257, 385, 128, 1, 640, 900, 300, 1500], 4000)])
+def test_groups_between_whole_rounds(kind, k, gated, sizes, n):
+    test_groups_of_all_shapes(kind, k, gated, sizes, n)
