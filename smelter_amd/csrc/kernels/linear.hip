@@ -65,11 +65,16 @@ static LinearPlan lin_plan(const sm_linear_desc* d, bool grouped, bool gathered)
     const long long n = plan.shape == 2 ? n2 : n0;
     plan.deep = d->x_type != SM_MX4 && plan.shape != 1 && n <= SM_NUM_CU;
     if (plan.shape == 2 && n * 2 <= SM_NUM_CU && d->E <= 64) {
+        // Runs of K, as many as fill the card: a step of a block that is alone on its CU takes 0.3 us (MX4 by MX4, four times as long a piece of K: 0.55), the sums go to memory and back, the
+        // joining launch costs 3.5 us.  bf16, us with 1 / 2 / 4 / 8 runs: 64 rows of 2048 x 8192 42 / 29 / 21 / 18, 100 rows of 4096 x 4096 25 / 22 / 18.5 / 26, 64 rows of 8192 x 2048 16.7 / 17.7 /
+        // 18.3 / 25.8; MX4 by MX4: 100 rows of 8192 x 8192 25.6 / 23.2 / 22 / 29, of 4096 x 4096 11.8 / 13.9 / 14.1.
         const int steps = (int)(((d->x_type == SM_MX4 ? xr : 2ll * d->K) + 127) / 128);
-        long long s = SM_NUM_CU / n;
-        if (s > steps / 8) s = steps / 8;
-        if (s > (d->M <= 32 ? 8 : 4)) s = d->M <= 32 ? 8 : 4;                       // (the sums that go through memory grow with M)
-        if (s > 2 || (s == 2 && steps >= 48)) plan.splits = (int)s;
+        const double step = d->x_type == SM_MX4 ? 0.55 : 0.3, sums = d->M * (double)d->N * (d->gated ? 2 : 1) * 8 / 4e6;
+        double best = steps * step;
+        for (int s = 2; s <= 8 && s * n <= SM_NUM_CU && s <= steps / 4; s++) {
+            const double t = (steps + s - 1) / s * step + 3.5 + s * sums;
+            if (t < best) { best = t; plan.splits = s; }
+        }
     }
     return plan;
 }
