@@ -1,19 +1,28 @@
 // smelter_amd/csrc/kernels/linear_stream.hpp — linear layers on FEW rows (decoding, small groups): the weights stream through the registers once, nothing is staged.
 //
 // A block owns 16 slots of one group and NB groups of 16 weight rows (16 NB output columns, or half as many gated ones: gate rows and up rows); its waves split K and join their sums in LDS, in a
-// fixed order.  Bound by the weights' bytes: a lane holds 32 consecutive k of one weight row (64 bytes of fp16, or two 16-byte MX4 blocks), so that a wave reads whole 128 / 256-byte pieces of 16
-// rows; which k a matrix instruction multiplies does not matter as long as both operands agree, so x is read in the same order and no operand is re-arranged.  What else goes through a CU's L1 is
-// kept small beside the weights: the scales come as one dword per lane for 16 blocks and are handed to their lanes by a shuffle (byte loads cost 8 of 28 us of a 5-row layer of 16384 x 8192),
+// fixed order.  Bound by the weights' bytes (MX4 by MX4 reads them at 4.5 TB/s, 16-bit weights at 4.3, MX4 under a 16-bit x at 3.8: 4 rows of 262144 x 2048): a wave reads 128 or 256 bytes of each of
+// its rows at once; which k a matrix instruction multiplies does not matter as long as both operands agree, so x is read in the same order and no operand is re-arranged.  What else goes through a
+// CU's L1 is kept small beside the weights: the scales come as one dword per lane for 16 blocks and are handed to their lanes by a shuffle (byte loads cost 8 of 28 us of a 5-row layer of 16384 x 8192),
 // lanes without a slot load no x, and where there are blocks enough a wave takes four groups of weight rows with the same x.
 // MX4 weights under 16-bit x become 16-bit values in the registers.  bf16: value times scale, exact.  fp16: the range of 2^-24 .. 65504 does not hold every scale, so the values are taken
 // relative to the largest scale of their row in these 512 k and the partial sum is multiplied by it in fp32 (a block 2^23 below that neighbour rounds, by less than the fp32 sum does).
 #pragma once
 #include "linear.hpp"
 
-// 32 consecutive k of a row starting at block `b` (k = 32 b): 16-bit = four loads of eight, MX4 = one of 32 codes
+// 32 k of a row for a lane of group g.  ROW (16-bit x and weights): eight k of each of the blocks b .. b + 3, so that a row's four lanes read 64 bytes side by side (16 rows of 8192 x 8192: 31.1 us
+// against 32.8 with a block for each); otherwise the lane's own block b: four loads of eight, or one of 32 MX4 codes.
 template <int KIND> struct LinBlk { static constexpr int NV = KIND == SM_MX4 ? 1 : 4; intx4_t v[NV]; };
-template <int KIND> __device__ __forceinline__ void lin_load_block(LinBlk<KIND>& f, const char* row, int b, int nb, int K) {
-    if constexpr (KIND == SM_MX4) {
+template <int KIND, bool ROW> __device__ __forceinline__ void lin_load_block(LinBlk<KIND>& f, const char* row, int b, int g, int nb, int K) {
+    if constexpr (ROW) {
+        if (32 * b + 128 <= K) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) __builtin_memcpy(&f.v[i], row + 64ll * (b + i) + 16 * g, 16);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; i++) f.v[i] = lin_load8(row, 32 * (b + i) + 8 * g, K);
+        }
+    } else if constexpr (KIND == SM_MX4) {
         f.v[0] = intx4_t{0, 0, 0, 0};
         if (b < nb) __builtin_memcpy(&f.v[0], row + 16ll * b, 16);
     } else {
@@ -79,7 +88,7 @@ template <int XK, int WK, int NB> __global__ __launch_bounds__(512) void lin_str
 #pragma unroll
             for (int b = 0; b < NB; b++)
 #pragma unroll
-                for (int j = 0; j < BL; j++) lin_load_block<WK>(w[u][b][j], wr[b], c + u * 4 * BL + g * BL + j, nb, p.K);
+                for (int j = 0; j < BL; j++) lin_load_block<WK, !MXW>(w[u][b][j], wr[b], MXW ? c + u * 4 * BL + g * BL + j : c, g, nb, p.K);
         // the scales of this lane's blocks c + 8 u + 2 g + {0, 1} lie in lane group 2 u + g / 2, bytes 2 (g & 1) + {0, 1}
         auto pair = [&](unsigned dw, int u) { return (unsigned)__shfl((int)dw, r + 16 * (2 * u + (g >> 1))) >> (16 * (g & 1)); };
         if constexpr (XK == SM_MX4) {
@@ -92,7 +101,7 @@ template <int XK, int WK, int NB> __global__ __launch_bounds__(512) void lin_str
 #pragma unroll
                 for (int j = 0; j < BL; j++) {
                     LinBlk<SM_MX4> x;
-                    lin_load_block<SM_MX4>(x, xr, c + u * 4 * BL + g * BL + j, xnb, p.K);
+                    lin_load_block<SM_MX4, false>(x, xr, c + u * 4 * BL + g * BL + j, g, xnb, p.K);
 #pragma unroll
                     for (int b = 0; b < NB; b++) acc[b] = lin_mma4<0>(x.v[0], (int)(sx >> (8 * j)), w[u][b][j].v[0], (int)(sw[b] >> (8 * j)), acc[b]);
                 }
@@ -122,7 +131,7 @@ template <int XK, int WK, int NB> __global__ __launch_bounds__(512) void lin_str
 #pragma unroll
                 for (int j = 0; j < BL; j++) {
                     LinBlk<XK> x;
-                    lin_load_block<XK>(x, xr, c + u * 4 * BL + g * BL + j, nb, xk);
+                    lin_load_block<XK, !MXW>(x, xr, MXW ? c + u * 4 * BL + g * BL + j : c, g, nb, xk);
 #pragma unroll
                     for (int b = 0; b < NB; b++) {
                         float rel = 0.f;
