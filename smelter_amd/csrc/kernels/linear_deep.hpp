@@ -1,10 +1,11 @@
 // smelter_amd/csrc/kernels/linear_deep.hpp — linear layers on some tens to some hundred rows: small tiles (128 weight rows x 64 or 128 slots, four waves) with several steps of K in flight.
 //
 // With few tiles a CU waits: for memory (the bytes that it has asked for, over the time they take, are its rate), and for LDS, whose latency is longer than the few products of a phase.  The tile
-// kernel asks for one step ahead and reads a quarter of a step ahead; here ST - 1 steps are on their way and the fragments of a whole step are read while the products of the one before run.  That needs every load of the loop to be an LDS-DMA (their completion is counted; a load into registers would make the compiler wait for all of them): MX4 weights under a
-// 16-bit x stay packed in LDS (32 bytes a row and step instead of 128) and become 16-bit values behind the fragment read, and the scale bytes of the whole run of K are put into LDS once, in
-// front of the loop.  For the packed weights a lane group takes the chunks 4 g .. 4 g + 3 of a row — one MX4 block, one scale — instead of 2 P + g; the order in which k are added is free as
-// long as both operands agree.
+// kernel asks for one step ahead and reads a quarter of a step ahead; here ST - 1 steps are on their way and the fragments of a whole step are read while the products of the one before run: 512 rows
+// of 4096 x 4096 in fp16 take 29 us, 64 rows 17.  That needs every load of the loop to be an LDS-DMA (their completion is counted; a load into registers would make the compiler wait for all of
+// them): MX4 weights under a 16-bit x stay packed in LDS (32 bytes a row and step instead of 128) and become 16-bit values behind the fragment read, and the scale bytes of the whole run of K are
+// put into LDS once, in front of the loop.  For the packed weights a lane group takes the chunks 4 g .. 4 g + 3 of a row — one MX4 block, one scale — instead of 2 P + g; the order in which k are
+// added is free as long as both operands agree.  (Both sides in MX4 gain nothing: their steps are four times as long in K, few, and their scales are a load of their own.)
 #pragma once
 #include "linear_tile.hpp"
 #include <atomic>
