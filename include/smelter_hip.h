@@ -348,7 +348,8 @@ size_t sm_float_array_count(int32_t N, int32_t C, int32_t H, int32_t W);
 
 /* ---- linear layers with 4-bit weights, and expert layers (csrc/kernels/mx4.hip, linear.hip, moe.hip) ----
  * Where an MPSCNNFullyConnectedNode (Converters.swift:297) holds fp16 weights [N][K], these hold fp16, bf16 or MX4 ones, for one layer or for E experts of the same shape.
- * No call allocates, synchronises or keeps anything between calls; every one can be captured into a graph. */
+ * No call allocates, synchronises or keeps anything between calls; every one can be captured into a graph.  Outputs and workspace must not overlap an operand; calls (or graphs) that may run at
+ * the same time need a workspace each. */
 enum { SM_F16 = 0, SM_BF16 = 1, SM_F32 = 2,
        SM_MX4 = 3 /* blocks of 32 e2m1 elements along the row (16 bytes, even column in the low nibble; columns behind the end hold code 0) + one e8m0 scale byte per block, 2^(b - 127), 255 = NaN:
                      codes [rows][ceil(K / 32)][16], 16-byte aligned, scales [rows][ceil(K / 32)], both dense */ };

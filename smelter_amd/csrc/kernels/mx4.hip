@@ -4,7 +4,8 @@
 //
 // |v| / scale lies below 8; what lies above 6 becomes 6 (the format's own rule: the scale is not raised).  Division by a power of two is exact, so the code of every value is decided without a
 // rounding before it.  A block that holds a NaN or an infinity gets scale byte 255 (NaN) and codes 0; a block of zeros scale byte 0.  The sign of a value that becomes zero is kept.
-// Both directions are bound by memory: 2 + 17/32 bytes per 16-bit element.
+// Both directions are bound by memory: 2 + 17/32 bytes per 16-bit element.  65536 x 4096 bf16: packed in 156 us (4.4 TB/s), read back in 117 (5.8 TB/s; a copy of 1 GiB: 5.1).  A thread packs a whole
+// block, so that no maximum crosses lanes; it reads back eight elements, so that it stores 16 bytes.
 #include "linear.hpp"
 
 template <int KIND> struct Mx4In;      // the 32 elements of one block in registers, and their largest magnitude as fp32 bits (>= 0x7f800000: an infinity or a NaN)

@@ -531,7 +531,7 @@ def mbconv_stem(x_nchw, w_stem_ohwi, b_stem, wd, bd, w2, b2, st_stride=2, st_pad
 
 # ---- linear layers with 4-bit weights, and expert layers ---------------------------------------------------------------------------------------
 # fp16 / bf16 row-major tensors [rows, K] instead of NHWC; arguments that do not fit raise SmelterError (invalidArgument) before anything is launched.  The work goes to the
-# current stream of the tensors' own device, whichever device is current.
+# current stream of the tensors' own device, whichever device is current.  No gradients; an `out` must not overlap an operand.
 
 _TYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
 _MX4 = 3
