@@ -12,7 +12,6 @@
 
 #define MOE_MAX_E 1024
 #define MOE_MAX_K 32
-#define MOE_WAVES 8
 
 struct RouteParams {
     const char* z; int type; long long T; int E, k; long long ld; int renorm;       // ld in elements
@@ -153,22 +152,22 @@ template <int EPL, bool ONE> __global__ __launch_bounds__(EPL <= 16 ? 1024 : 512
     }
 }
 
-__global__ void route_place_kernel(RouteParams p, int blocks) {
+__global__ __launch_bounds__(1024) void route_place_kernel(RouteParams p, int blocks) {
     extern __shared__ int lds[];
     int* total = lds; int* before = total + p.E; int* offs = before + p.E; int* wcount = offs + p.E + 1;
     for (int e = threadIdx.x; e < 2 * p.E; e += blockDim.x) lds[e] = 0;
     __syncthreads();
-    // counts of all blocks and of the blocks before this one (integer sums, the same in any order): a thread adds one expert's over every parts-th block, eight loads at a time
+    // counts of all blocks and of the blocks before this one (integer sums, the same in any order): a thread adds one expert's over every parts-th block, sixteen loads at a time
     const int parts = (int)blockDim.x / p.E > 0 ? (int)blockDim.x / p.E : 1;
     for (int i = threadIdx.x; i < parts * p.E; i += blockDim.x) {
         const int e = i % p.E, part = i / p.E;
         int all = 0, low = 0;
-        for (int b0 = part; b0 < blocks; b0 += 8 * parts) {
-            int c[8];
+        for (int b0 = part; b0 < blocks; b0 += 16 * parts) {
+            int c[16];
 #pragma unroll
-            for (int q = 0; q < 8; q++) { const int b = b0 + q * parts; c[q] = b < blocks ? p.counts[(long long)b * p.E + e] : 0; }
+            for (int q = 0; q < 16; q++) { const int b = b0 + q * parts; c[q] = b < blocks ? p.counts[(long long)b * p.E + e] : 0; }
 #pragma unroll
-            for (int q = 0; q < 8; q++) { all += c[q]; low += b0 + q * parts < (int)blockIdx.x ? c[q] : 0; }
+            for (int q = 0; q < 16; q++) { all += c[q]; low += b0 + q * parts < (int)blockIdx.x ? c[q] : 0; }
         }
         if (all) atomicAdd(&total[e], all);
         if (low) atomicAdd(&before[e], low);
@@ -201,7 +200,6 @@ extern "C" size_t sm_moe_route_workspace_bytes(int64_t T, int32_t E, int32_t k) 
 
 template <int EPL> static int route_launch(RouteParams p, hipStream_t s) {
     constexpr int WAVES = EPL <= 16 ? 16 : 8;                                     // of the selecting kernel: 64 tokens at once, 32 where a lane holds more scores
-    const size_t place = (size_t)(MOE_WAVES * p.E + p.E + 1) * sizeof(int);
     if (p.T <= ROUTE_SMALL) {
         p.per_block = (int)p.T;
         route_select_kernel<EPL, true><<<1, 64 * WAVES, p.E * sizeof(int) + (size_t)(WAVES * p.E + p.E + 1) * sizeof(int), s>>>(p);
@@ -209,7 +207,10 @@ template <int EPL> static int route_launch(RouteParams p, hipStream_t s) {
         const long long blocks = route_blocks(p.T, &p.per_block);
         route_select_kernel<EPL, false><<<dim3((unsigned)blocks), 64 * WAVES, p.E * sizeof(int), s>>>(p);
         SM_LAUNCH_CHECK();
-        route_place_kernel<<<dim3((unsigned)blocks), 64 * MOE_WAVES, 2 * p.E * sizeof(int) + place, s>>>(p, (int)blocks);
+        // waves of the placing one: more to add the counts of many blocks (16384 tokens of 256 scores: 26.4 us with 16, 30.6 with 8), fewer to count and join (1024 of 128: 15.1, 13.9); 8 is what
+        // LDS holds of more than 256 experts
+        const int place = EPL <= 16 && blocks >= 128 ? 16 : 8;
+        route_place_kernel<<<dim3((unsigned)blocks), 64 * place, (size_t)((place + 3) * p.E + 1) * sizeof(int), s>>>(p, (int)blocks);
     }
     SM_LAUNCH_CHECK();
     return SM_OK;
