@@ -373,12 +373,14 @@ typedef struct sm_linear_desc {
 } sm_linear_desc;
 int sm_linear_fwd(const sm_linear_desc* d, const void* x, const void* x_scales, const void* w, const void* w_scales, const float* bias /* [E][N or 2 N] or NULL */, const int32_t* offsets,
                   const int32_t* rows, void* y, void* workspace, size_t workspace_bytes, sm_stream_t stream);
-/* bytes of scratch sm_linear_fwd wants for these sizes (sums of a product whose K is cut because there are few tiles), 16-byte aligned; 0 if none.  grouped, gathered: offsets, rows are given */
+/* bytes of scratch sm_linear_fwd wants for these sizes (sums of a product whose K is cut because there are few tiles), 16-byte aligned; 0 if none, as always
+ * where M <= 16 E.  grouped, gathered: offsets, rows are given */
 size_t sm_linear_workspace_bytes(const sm_linear_desc* d, int32_t grouped, int32_t gathered);
 
 /* Routing: for each of T tokens the k <= 32 largest of its E <= 1024 scores (ties: the lower index first) and their softmax weights (over the chosen ones, or over all E when !renormalize),
  * and the assignments in the order of their expert (stable): offsets [E + 1], rows [T k] = token of each slot, slots [T][k] = slot of each assignment.  A score of -inf or NaN is never
- * chosen: what is missing to k gets expert -1, weight 0, slot -1, and rows behind offsets[E] hold -1.  Workspace: sm_moe_route_workspace_bytes. */
+ * chosen: what is missing to k gets expert -1, weight 0, slot -1, and rows behind offsets[E] hold -1.  Workspace: sm_moe_route_workspace_bytes, 4-byte
+ * aligned (none up to 64 tokens). */
 size_t sm_moe_route_workspace_bytes(int64_t T, int32_t E, int32_t k);
 int sm_moe_route(const void* scores, int32_t type, int64_t T, int32_t E, int32_t k, int64_t ld, int32_t renormalize, float* weights /* [T][k] */, int32_t* experts /* [T][k] */,
                  int32_t* offsets, int32_t* rows, int32_t* slots, void* workspace, size_t workspace_bytes, sm_stream_t stream);

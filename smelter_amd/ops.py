@@ -613,7 +613,7 @@ def _gpu(index, name, t, dtypes):
     return at
 
 
-_BYTES, _INTS, _HALVES, _FLOATS = (torch.uint8,), (torch.int32,), (torch.float16, torch.bfloat16), (torch.float32,)
+_U8, _BYTES, _INTS, _HALVES, _FLOATS = torch.uint8, (torch.uint8,), (torch.int32,), (torch.float16, torch.bfloat16), (torch.float32,)
 
 
 def _check_mx4(q, index, name):
@@ -621,12 +621,11 @@ def _check_mx4(q, index, name):
         _refuse("%s: an Mx4 tensor is wanted", name)
     c, s, k = q
     index = _gpu(index, name, c, _BYTES)
-    _gpu(index, name, s, _BYTES)
-    nb = (k + 31) // 32
-    *cs, cb = c.shape or (-1,)
-    *ss, sb = s.shape or (-1,)
-    if k < 0 or sb != nb or cb != 16 * nb or cs != ss:
-        _refuse("%s: codes %s and scales %s for %d columns", name, tuple(c.shape), tuple(s.shape), k)
+    if not isinstance(s, torch.Tensor) or s.dtype is not _U8 or s.get_device() != index:
+        _gpu(index, name, s, _BYTES)
+    nb, cs, ss, n = (k + 31) // 32, c.shape, s.shape, c.dim()
+    if k < 0 or n < 1 or n != s.dim() or cs[-1] != 16 * nb or ss[-1] != nb or (n > 1 and cs[0] != ss[0]) or (n > 2 and cs[1:-1] != ss[1:-1]):
+        _refuse("%s: codes %s and scales %s for %d columns", name, tuple(cs), tuple(ss), k)
     if not c.is_contiguous() or not s.is_contiguous() or c.data_ptr() & 15:
         _refuse("%s: codes and scales must be contiguous, codes 16-byte aligned", name)
     return index
@@ -659,19 +658,20 @@ def mx4_dequantize(q, dtype=torch.float16, out=None):
     return out
 
 
-def _linear(name, x, w, lead, offsets, rows, bias, act, slope, gated, out, dtype):
-    """the checks and the call that mx4_linear and expert_linear share; `lead` = leading axes of the weights (0 or 1)"""
+def _linear(name, index, x, w, lead, offsets, rows, bias, act, slope, gated, out, dtype):
+    """the checks and the call that mx4_linear and expert_linear share; `index` = the device of the offsets, `lead` = leading axes of the weights
+    (0 or 1)"""
     if isinstance(x, Mx4):
-        index = _check_mx4(x, None, name)
+        index = _check_mx4(x, index, name)
         xt, xs, x_type, xk, x_ld = x.codes, x.scales.data_ptr(), _MX4, x.k, 0
         if xt.dim() != 2:
             _refuse("%s: x must be [rows, K]", name)
     else:
-        index = _gpu(None, name, x, _HALVES)
+        index = _gpu(index, name, x, _HALVES)
         if x.dim() != 2:
             _refuse("%s: x must be [rows, K]", name)
-        xt, xs, x_type = x, None, _TYPES[x.dtype]
-        _, xk, x_ld = _rows2d(x, name)
+        xt, xs, x_type, xk = x, None, _TYPES[x.dtype], x.shape[1]
+        x_ld = xk if x.is_contiguous() else _rows2d(x, name)[2]
     if isinstance(w, Mx4):
         _check_mx4(w, index, name)
         wc, wsc, w_type, wk = w.codes, w.scales.data_ptr(), _MX4, w.k
@@ -690,7 +690,7 @@ def _linear(name, x, w, lead, offsets, rows, bias, act, slope, gated, out, dtype
     m = t if rows is None else rows.shape[0]
     if bias is not None:
         _gpu(index, name, bias, _FLOATS)
-        if not bias.is_contiguous() or bias.shape != wsh[:-1]:
+        if not bias.is_contiguous() or bias.dim() != lead + 1 or bias.shape[-1] != n or (lead and bias.shape[0] != e):
             _refuse("%s: bias %s for weights %s", name, tuple(bias.shape), tuple(w.shape))
     if gated:
         if n % 2:
@@ -711,7 +711,7 @@ def _linear(name, x, w, lead, offsets, rows, bias, act, slope, gated, out, dtype
         y_ld = _rows2d(out, name)[2]
     L = lib()
     d = C.byref(LinearDesc(m, t, n, xk, e, x_type, w_type, _TYPES[out.dtype], act, slope, 1 if gated else 0, x_ld, y_ld))
-    wsb = L.sm_linear_workspace_bytes(d, offsets is not None, rows is not None)
+    wsb = L.sm_linear_workspace_bytes(d, offsets is not None, rows is not None) if m > 16 * e else 0
     work = xt.new_empty((wsb,), dtype=torch.uint8) if wsb else None
     _on(index, L.sm_linear_fwd, d, xt.data_ptr(), xs, wc.data_ptr(), wsc, bias.data_ptr() if bias is not None else None, offsets.data_ptr() if offsets is not None else None,
         rows.data_ptr() if rows is not None else None, out.data_ptr(), work.data_ptr() if wsb else None, wsb)
@@ -723,7 +723,7 @@ def mx4_linear(x, w, bias=None, act=ACT_NONE, slope=0.0, gated=False, out=None, 
     sides in 4 bits; dtype fp16 (default), bf16 or fp32).  gated: w has 2 N rows and the result is silu(first N columns) * last N.  bias fp32 [rows of w]."""
     if not isinstance(w, Mx4):
         _refuse("mx4_linear: the weights must be an Mx4 tensor")
-    return _linear("mx4_linear", x, w, 0, None, None, bias, act, slope, gated, out, dtype)
+    return _linear("mx4_linear", None, x, w, 0, None, None, bias, act, slope, gated, out, dtype)
 
 
 def expert_linear(x, w, offsets, rows=None, bias=None, act=ACT_NONE, slope=0.0, gated=False, out=None, dtype=None):
@@ -732,15 +732,14 @@ def expert_linear(x, w, offsets, rows=None, bias=None, act=ACT_NONE, slope=0.0, 
     read back to the host.  Slots that no group covers are left as they were (in a new `out`: unspecified).  gated, bias [E, rows of w], dtype: as in mx4_linear."""
     index = _gpu(None, "expert_linear", offsets, _INTS)
     wc = w.codes if isinstance(w, Mx4) else w
-    _gpu(index, "expert_linear", x.codes if isinstance(x, Mx4) else x, (torch.float16, torch.bfloat16, torch.uint8))
     e = wc.shape[0] if isinstance(wc, torch.Tensor) and wc.dim() else 0
-    if e < 1 or not offsets.is_contiguous() or offsets.shape != (e + 1,):
+    if e < 1 or not offsets.is_contiguous() or offsets.dim() != 1 or offsets.shape[0] != e + 1:
         _refuse("expert_linear: offsets %s for %d experts", tuple(offsets.shape), e)
     if rows is not None:
         _gpu(index, "expert_linear", rows, _INTS)
         if rows.dim() != 1 or not rows.is_contiguous():
             _refuse("expert_linear: rows must be a contiguous vector")
-    return _linear("expert_linear", x, w, 1, offsets, rows, bias, act, slope, gated, out, dtype)
+    return _linear("expert_linear", index, x, w, 1, offsets, rows, bias, act, slope, gated, out, dtype)
 
 
 def moe_route(scores, k, renormalize=True):
@@ -754,7 +753,7 @@ def moe_route(scores, k, renormalize=True):
         _refuse("moe_route: %d of %d experts (taken: up to 1024 experts, 1 .. min(32, experts) of them)", k, e)
     ld = e if scores.is_contiguous() else _rows2d(scores, "moe_route")[2]
     L, n = lib(), t * k
-    ws = L.sm_moe_route_workspace_bytes(t, e, k)
+    ws = L.sm_moe_route_workspace_bytes(t, e, k) if t > 64 else 0
     weights = scores.new_empty((t, k), dtype=torch.float32)
     # the integers in one allocation, the workspace behind the results
     experts, slots, rows, offsets, work = scores.new_empty((3 * n + e + 1 + ws // 4,), dtype=torch.int32).split_with_sizes((n, n, n, e + 1, ws // 4))
