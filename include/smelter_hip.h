@@ -366,7 +366,8 @@ int sm_mx4_dequantize(const void* codes, const void* scales, int64_t rows, int32
 typedef struct sm_linear_desc {
     int64_t M, T;                   /* slots (rows of y); rows of x */
     int32_t N, K, E;                /* columns of y, inner size, groups (1 = an ordinary layer) */
-    int32_t x_type, w_type, y_type; /* fp16 | bf16 x on weights of the same type or MX4, y of x's type or fp32; MX4 x on MX4 weights, any y */
+    int32_t x_type, w_type, y_type; /* fp16 | bf16 x on weights of the same type or MX4, y of x's type, fp16 (three bits more for what a
+                                     next layer with MX4 weights takes) or fp32; MX4 x on MX4 weights, any y */
     int32_t act; float slope;       /* SM_ACT_* behind the bias (not with gated) */
     int32_t gated;
     int64_t x_ld, y_ld;             /* row strides in elements, 0 = dense (an MX4 x is dense) */

@@ -93,8 +93,8 @@ extern "C" int sm_linear_fwd(const sm_linear_desc* d, const void* x, const void*
     const bool x16 = d->x_type == SM_F16 || d->x_type == SM_BF16;
     SM_REQUIRE((x16 && (d->w_type == d->x_type || d->w_type == SM_MX4)) || (d->x_type == SM_MX4 && d->w_type == SM_MX4),
                "linear: x of type %d on weights of type %d (taken: fp16 or bf16 on weights of the same type or MX4, MX4 on MX4)", d->x_type, d->w_type);
-    SM_REQUIRE(d->y_type == SM_F32 || ((d->y_type == SM_F16 || d->y_type == SM_BF16) && (!x16 || d->y_type == d->x_type)),
-               "linear: output type %d for x of type %d (taken: x's own 16-bit type or fp32; any of the three for an MX4 x)", d->y_type, d->x_type);
+    SM_REQUIRE(d->y_type == SM_F32 || ((d->y_type == SM_F16 || d->y_type == SM_BF16) && (!x16 || d->y_type == SM_F16 || d->y_type == d->x_type)),
+               "linear: output type %d for x of type %d (taken: x's own 16-bit type, fp16 or fp32; any of the three for an MX4 x)", d->y_type, d->x_type);
     SM_REQUIRE(d->act >= SM_ACT_NONE && d->act <= SM_ACT_CLIP, "linear: unknown activation %d", d->act);
     SM_REQUIRE(!d->gated || d->act == SM_ACT_NONE, "linear: a gated layer takes no further activation");
     SM_REQUIRE(offsets || d->E == 1, "linear: %d experts without offsets", d->E);

@@ -252,9 +252,8 @@ __device__ __forceinline__ void lin_finish(const LinearParams& p, const LinTile&
             else lin_finish_registers<FR, WN, WM, FN, FM, SCALED, YT, false, false>(p, tile, n0, g, wn, acc, slot, wmul + row0);
         };
         if (p.y_type == SM_F32) go(std::integral_constant<int, SM_F32>());
-        else if constexpr (XK != SM_MX4) go(std::integral_constant<int, XK>());
         else if (p.y_type == SM_F16) go(std::integral_constant<int, SM_F16>());
-        else go(std::integral_constant<int, SM_BF16>());
+        else if constexpr (XK != SM_F16) go(std::integral_constant<int, SM_BF16>());
         return;
     }
     lin_finish_lds<FR, WN, WM, FN, FM, BYTES, SCALED>(p, tile, n0, acc, lds, wmul);

@@ -706,3 +706,28 @@ def test_products_between_whole_rounds(kind, aligned, m, n, k):
 @pytest.mark.parametrize("sizes, n", [([1100, 0, 130, 90], 3900), ([257, 385, 128, 1, 640, 900, 300, 1500], 4000)])
 def test_groups_between_whole_rounds(kind, k, gated, sizes, n):
     test_groups_of_all_shapes(kind, k, gated, sizes, n)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "bf16-mx4"])
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("m, n, k", WAYS + [(300, 1004, 520)])
+def test_fp16_answers_of_bf16_rows(kind, gated, m, n, k):
+    """a bf16 layer that hands fp16 to the next one: rounded once, to eleven bits"""
+    g = torch.Generator("cuda").manual_seed(m + n)
+    x = torch.randn((m, k), generator=g, device="cuda").to(BF16)
+    w = torch.randn((2 * n if gated else n, k), generator=g, device="cuda") * k ** -0.5
+    if kind == "bf16":
+        w = w.to(BF16)
+        got, wv = ops.expert_linear(x, w[None], torch.tensor([0, m], dtype=torch.int32, device="cuda"), gated=gated, dtype=F16), w.double()
+    else:
+        w = ops.mx4_quantize(w)
+        got, wv = ops.mx4_linear(x, w, gated=gated, dtype=F16), ops.mx4_dequantize(w, F32).double()
+    assert got.dtype == F16
+    z, mag = x.double() @ wv.t(), x.double().abs() @ wv.abs().t()
+    err = (k / 8 + 64) * 2.0 ** -23 * mag + 2.0 ** -23 * x.double().abs().sum(1, keepdim=True) * wv.abs().amax(1)
+    if gated:                                                            # as mx4ref.linear: |silu'| < 1.1; the exponential, division and products: below 2^-19 of the result
+        a, b, ea, eb = z[:, :n], z[:, n:], err[:, :n], err[:, n:]
+        s = a * torch.sigmoid(a)
+        z, err = s * b, 1.1 * ea * b.abs() + s.abs() * eb + 1.1 * ea * eb + 2.0 ** -19 * (s * b).abs()
+    lim = err + 2.0 ** -11 * (z.abs() + err) + 2.0 ** -25
+    assert ((got.double() - z).abs() <= lim).all()
