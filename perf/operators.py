@@ -269,7 +269,8 @@ def _own(s):
     if s["op"] == "combine":
         return ops.moe_combine(s["data"], s["plan"]["slots"], s["part"])
     r = ops.moe_route(s["score"], s["top"])
-    h = ops.expert_linear(s["data"], _own_weight(ops, s["hidden"], s["k"]), r.offsets, rows=r.rows, gated=True)
+    # what goes between the products under 4-bit weights in fp16 (bf16 would round it to eight bits, half of what the answer may be off by)
+    h = ops.expert_linear(s["data"], _own_weight(ops, s["hidden"], s["k"]), r.offsets, rows=r.rows, gated=True, dtype=torch.float16 if len(s["answer"]) == 2 else None)
     y = ops.expert_linear(h, _own_weight(ops, s["answer"], s["f"]), r.offsets, dtype=torch.float32)
     return ops.moe_combine(y, r.slots, r.weights, dtype=s["data"].dtype)
 
