@@ -367,7 +367,8 @@ typedef struct sm_linear_desc {
     int64_t M, T;                   /* slots (rows of y); rows of x */
     int32_t N, K, E;                /* columns of y, inner size, groups (1 = an ordinary layer) */
     int32_t x_type, w_type, y_type; /* fp16 | bf16 x on weights of the same type or MX4, y of x's type, fp16 (three bits more for what a
-                                     next layer with MX4 weights takes) or fp32; MX4 x on MX4 weights, any y */
+                                     next layer with MX4 weights takes) or fp32; MX4 x on MX4 weights, any y;
+                                     fp32 x on 16-bit or MX4 weights, any y: carried as two parts of bf16 (of fp16 under fp16 weights) on twice the rows */
     int32_t act; float slope;       /* SM_ACT_* behind the bias (not with gated) */
     int32_t gated;
     int64_t x_ld, y_ld;             /* row strides in elements, 0 = dense (an MX4 x is dense) */
@@ -375,7 +376,7 @@ typedef struct sm_linear_desc {
 int sm_linear_fwd(const sm_linear_desc* d, const void* x, const void* x_scales, const void* w, const void* w_scales, const float* bias /* [E][N or 2 N] or NULL */, const int32_t* offsets,
                   const int32_t* rows, void* y, void* workspace, size_t workspace_bytes, sm_stream_t stream);
 /* bytes of scratch sm_linear_fwd wants for these sizes (sums of a product whose K is cut because there are few tiles), 16-byte aligned; 0 if none, as always
- * where M <= 16 E.  grouped, gathered: offsets, rows are given */
+ * where M <= 16 E, but for fp32 rows (256-byte aligned).  grouped, gathered: offsets, rows are given */
 size_t sm_linear_workspace_bytes(const sm_linear_desc* d, int32_t grouped, int32_t gathered);
 
 /* Routing: for each of T tokens the k <= 32 largest of its E <= 1024 scores (ties: the lower index first) and their softmax weights (over the chosen ones, or over all E when !renormalize),

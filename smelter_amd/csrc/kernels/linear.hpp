@@ -26,6 +26,7 @@ struct LinearParams {
     int N, K, E, act; float slope;
     int gated, y_type, y_vec, w_rows;               // y_vec: eight consecutive outputs may be stored as 16-byte words;  w_rows = N or 2 N
     float* part; long long part_ld; int splits;     // fp32 sums [splits][M][part_ld] of a product whose K is cut into `splits` runs (1: none)
+    int pairs;                                      // (lin_join_kernel) the sums are [M][2][part_ld], of the two parts of fp32 rows
     long long m_tiles; int n_tiles;                 // launch grid: a bound on the row tiles (the real number is known on the device only) x column tiles
 };
 

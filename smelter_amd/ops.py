@@ -667,7 +667,7 @@ def _linear(name, index, x, w, lead, offsets, rows, bias, act, slope, gated, out
         if xt.dim() != 2:
             _refuse("%s: x must be [rows, K]", name)
     else:
-        index = _gpu(index, name, x, _HALVES)
+        index = _gpu(index, name, x, _TYPES)
         if x.dim() != 2:
             _refuse("%s: x must be [rows, K]", name)
         xt, xs, x_type, xk = x, None, _TYPES[x.dtype], x.shape[1]
@@ -678,7 +678,7 @@ def _linear(name, index, x, w, lead, offsets, rows, bias, act, slope, gated, out
     else:
         _gpu(index, name, w, _HALVES)
         wc, wsc, w_type = w, None, _TYPES[w.dtype]
-        if w_type != x_type:
+        if w_type != x_type and x_type != 2:
             _refuse("%s: weights of type %s under x of type %s", name, w.dtype, "MX4" if x_type == _MX4 else x.dtype)
         if not w.is_contiguous():
             _refuse("%s: weights must be contiguous", name)
@@ -711,7 +711,7 @@ def _linear(name, index, x, w, lead, offsets, rows, bias, act, slope, gated, out
         y_ld = _rows2d(out, name)[2]
     L = lib()
     d = C.byref(LinearDesc(m, t, n, xk, e, x_type, w_type, _TYPES[out.dtype], act, slope, 1 if gated else 0, x_ld, y_ld))
-    wsb = L.sm_linear_workspace_bytes(d, offsets is not None, rows is not None) if m > 16 * e else 0
+    wsb = L.sm_linear_workspace_bytes(d, offsets is not None, rows is not None) if m > 16 * e or x_type == 2 else 0
     work = xt.new_empty((wsb,), dtype=torch.uint8) if wsb else None
     _on(index, L.sm_linear_fwd, d, xt.data_ptr(), xs, wc.data_ptr(), wsc, bias.data_ptr() if bias is not None else None, offsets.data_ptr() if offsets is not None else None,
         rows.data_ptr() if rows is not None else None, out.data_ptr(), work.data_ptr() if wsb else None, wsb)
@@ -720,7 +720,8 @@ def _linear(name, index, x, w, lead, offsets, rows, bias, act, slope, gated, out
 
 def mx4_linear(x, w, bias=None, act=ACT_NONE, slope=0.0, gated=False, out=None, dtype=None):
     """act(x . w^T + bias) with MX4 weights w [N, K] (sm_linear_fwd).  x [M, K]: fp16 or bf16 (the weights are read as 16-bit values, the output has x's type, fp16 or fp32), or an Mx4 tensor
-    (both sides in 4 bits; dtype fp16 (default), bf16 or fp32).  What a bf16 layer hands to a next one with MX4 weights keeps three bits more as fp16 (beyond 65504: infinities).  gated: w has 2 N rows and the result is silu(first N columns) * last N.  bias fp32 [rows of w]."""
+    (both sides in 4 bits; dtype fp16 (default), bf16 or fp32).  What a bf16 layer hands to a next one with MX4 weights keeps three bits more as fp16 (beyond 65504: infinities).  fp32 x: carried as two
+    16-bit parts on twice the rows, any dtype (fp32 by default).  gated: w has 2 N rows and the result is silu(first N columns) * last N.  bias fp32 [rows of w]."""
     if not isinstance(w, Mx4):
         _refuse("mx4_linear: the weights must be an Mx4 tensor")
     return _linear("mx4_linear", None, x, w, 0, None, None, bias, act, slope, gated, out, dtype)
@@ -728,7 +729,7 @@ def mx4_linear(x, w, bias=None, act=ACT_NONE, slope=0.0, gated=False, out=None, 
 
 def expert_linear(x, w, offsets, rows=None, bias=None, act=ACT_NONE, slope=0.0, gated=False, out=None, dtype=None):
     """Products grouped by expert (sm_linear_fwd): slot s of group e (offsets[e] <= s < offsets[e + 1]) gets act(x[rows[s]] . w[e]^T + bias[e]); without `rows` slot s is row s of x.
-    x [T, K] and w [E, N, K]: both fp16, both bf16, 16-bit x on Mx4 weights, or both Mx4.  offsets int32 [E + 1], rows int32 [slots], both on the GPU (MoePlan holds them): nothing is
+    x [T, K] and w [E, N, K]: both fp16, both bf16, 16-bit x on Mx4 weights, both Mx4, or fp32 x on any.  offsets int32 [E + 1], rows int32 [slots], both on the GPU (MoePlan holds them): nothing is
     read back to the host.  Slots that no group covers are left as they were (in a new `out`: unspecified).  gated, bias [E, rows of w], dtype: as in mx4_linear."""
     index = _gpu(None, "expert_linear", offsets, _INTS)
     wc = w.codes if isinstance(w, Mx4) else w

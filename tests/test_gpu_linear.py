@@ -266,7 +266,7 @@ def test_python_refusals():
     x, xv, w, wv, dt = operands("f16-mx4", gen(2), 4, 64, (8, 64))
     off = torch.tensor([0, 4], dtype=torch.int32, device="cuda")
     w3 = ops.Mx4(w.codes[None], w.scales[None], 64)
-    for f in (lambda: ops.mx4_linear(x[:, :32], w), lambda: ops.mx4_linear(x.float(), w), lambda: ops.mx4_linear(x, w3), lambda: ops.mx4_linear(x, w, torch.zeros(7, device="cuda")),
+    for f in (lambda: ops.mx4_linear(x[:, :32], w), lambda: ops.mx4_linear(x.double(), w), lambda: ops.mx4_linear(x, w3), lambda: ops.mx4_linear(x, w, torch.zeros(7, device="cuda")),
               lambda: ops.mx4_linear(x, w, torch.zeros(8, device="cuda", dtype=F16)), lambda: ops.mx4_linear(x, w, dtype=BF16), lambda: ops.mx4_linear(x, w, out=torch.empty(4, 9, device="cuda", dtype=F16)),
               lambda: ops.mx4_linear(x, ops.Mx4(w.codes, w.scales, 40)), lambda: ops.mx4_linear(x, ops.Mx4(w.codes[:, ::2], w.scales, 64)), lambda: ops.mx4_linear(x, w, act=99),
               lambda: ops.expert_linear(x, w3, off.long()), lambda: ops.expert_linear(x, w3, off[:1]), lambda: ops.expert_linear(x, w3, off, torch.zeros(4, device="cuda")),
@@ -731,3 +731,80 @@ def test_fp16_answers_of_bf16_rows(kind, gated, m, n, k):
         z, err = s * b, 1.1 * ea * b.abs() + s.abs() * eb + 1.1 * ea * eb + 2.0 ** -19 * (s * b).abs()
     lim = err + 2.0 ** -11 * (z.abs() + err) + 2.0 ** -25
     assert ((got.double() - z).abs() <= lim).all()
+
+
+@pytest.mark.parametrize("weights", [F16, BF16, "mx4"])
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("m, n, k", [(1, 24, 1), (7, 40, 96), (33, 130, 261), (90, 256, 4096), (1500, 1000, 72)])
+def test_fp32_rows(weights, gated, m, n, k):
+    """fp32 rows in two parts: right to 2^-16 of the products' magnitudes (bf16 parts: what two roundings of half a step 2^-8 leave), 2^-22 under fp16 weights (2^-11 each)"""
+    g = torch.Generator("cuda").manual_seed(m + n + k)
+    t = m // 2 + 1
+    x = torch.randn((t, k + 3), generator=g, device="cuda")[:, 2:k + 2]
+    rows = torch.randint(-1, t + 1, (m,), generator=g, device="cuda").int()             # -1, t: no row of x
+    off = torch.tensor([0, m // 3, m // 3, m], dtype=torch.int32, device="cuda")
+    wn = 2 * n if gated else n
+    w = torch.randn((3, wn, k), generator=g, device="cuda") * k ** -0.5
+    bias = torch.randn((3, wn), generator=g, device="cuda")
+    if weights == "mx4":
+        w = ops.mx4_quantize(w)
+        wv = ops.mx4_dequantize(w, F32).double()
+    else:
+        w = w.to(weights)
+        wv = w.double()
+    got = ops.expert_linear(x, w, off, rows, bias, gated=gated)
+    assert got.dtype == F32 and got.shape == (m, n)
+    ok = ((rows >= 0) & (rows < t))[:, None]
+    xv = torch.where(ok, x.double()[rows.clamp(0, t - 1).long()], torch.zeros((), dtype=torch.float64, device="cuda"))
+    part = 2.0 ** -22 if weights == F16 else 2.0 ** -16
+    for e in range(3):
+        s = slice(int(off[e]), int(off[e + 1]))
+        z, mag = xv[s] @ wv[e].t(), xv[s].abs() @ wv[e].abs().t()
+        err = (k / 8 + 64) * 2.0 ** -22 * mag + 2.0 ** -22 * xv[s].abs().sum(1, keepdim=True) * wv[e].abs().amax(1) + part * mag + 2.0 ** -24 * wv[e].abs().sum(1)
+        z = z + bias[e].double()
+        err = err + 2.0 ** -23 * z.abs()
+        if gated:
+            a, b, ea, eb = z[:, :n], z[:, n:], err[:, :n], err[:, n:]
+            q = a * torch.sigmoid(a)
+            z, err = q * b, 1.1 * ea * b.abs() + q.abs() * eb + 1.1 * ea * eb + 2.0 ** -19 * (q * b).abs()
+        assert ((got[s].double() - z).abs() <= err + 2.0 ** -24 * z.abs()).all(), e
+    out = torch.full((m + 1, n + 8), 7.0, dtype=BF16, device="cuda")
+    ops.expert_linear(x, w, off, rows, bias, gated=gated, out=out[:m, :n])
+    assert torch.equal(out[:m, :n], got.to(BF16)) and out[m].eq(7).all() and out[:, n:].eq(7).all()
+
+
+def test_fp32_rows_of_nothing_and_infinities():
+    off = torch.tensor([0, 0, 2], dtype=torch.int32, device="cuda")
+    w = torch.ones((2, 8, 40), dtype=BF16, device="cuda")
+    bias = torch.full((2, 8), 3.0, device="cuda")
+    x = torch.ones((3, 40), device="cuda")
+    x[0, 4], x[1, 5] = INF, NAN
+    got = ops.expert_linear(x, w, off, torch.tensor([0, 2], dtype=torch.int32, device="cuda"), bias)
+    assert got[0].eq(INF).all() and got[1].eq(43).all()
+    assert ops.expert_linear(x, w, off, torch.tensor([1, 2], dtype=torch.int32, device="cuda"), bias)[0].isnan().all()
+    w[1, 3] = INF
+    got = ops.expert_linear(x, w, off, torch.tensor([-1, 2], dtype=torch.int32, device="cuda"), bias)
+    assert got[0].eq(3).all() and got[1, 3].eq(INF) and got[1, 2].eq(43)
+    assert ops.expert_linear(x[:0], w, off, torch.tensor([0, 0], dtype=torch.int32, device="cuda"), bias).eq(3).all()
+    assert ops.expert_linear(x[:, :0], w[:, :, :0], torch.tensor([0, 1, 3], dtype=torch.int32, device="cuda"), bias=bias).eq(3).all()
+    out = torch.full((4, 8), 7.0, device="cuda")
+    ops.expert_linear(torch.ones((4, 40), device="cuda"), w, torch.tensor([1, 2, 3], dtype=torch.int32, device="cuda"), out=out)
+    assert out[0].eq(7).all() and out[3].eq(7).all() and out[1].eq(40).all()
+
+
+def test_fp32_rows_in_a_graph():
+    g = torch.Generator("cuda").manual_seed(1)
+    x = torch.randn((70, 256), generator=g, device="cuda")
+    w = ops.mx4_quantize(torch.randn((2, 96, 256), generator=g, device="cuda"))
+    off = torch.tensor([0, 30, 70], dtype=torch.int32, device="cuda")
+    ops.expert_linear(x, w, off)
+    torch.cuda.synchronize()
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):
+        y = ops.expert_linear(x, w, off)
+    for turn in range(4):
+        x.mul_(1.5)
+        off.copy_(torch.tensor([0, 10 * turn + 5, 70], dtype=torch.int32))
+        gr.replay()
+        assert torch.equal(y, ops.expert_linear(x, w, off)), turn
+        torch.cuda.synchronize()

@@ -28,7 +28,7 @@ def refused(rc, word):
 
 @pytest.mark.parametrize("change, word", [
     (dict(M=-1), "sizes"), (dict(K=-1), "sizes"), (dict(E=0), "sizes"), (dict(M=1 << 31), "beyond"), (dict(N=1 << 30), "beyond"),
-    (dict(x_type=F32), "type"), (dict(w_type=BF16), "type"), (dict(x_type=MX4), "type"), (dict(x_type=7), "type"), (dict(y_type=BF16), "output type"), (dict(y_type=MX4), "output type"),
+    (dict(x_type=F32, w_type=F32), "type"), (dict(x_type=F32), "workspace"), (dict(w_type=BF16), "type"), (dict(x_type=MX4), "type"), (dict(x_type=7), "type"), (dict(y_type=BF16), "output type"), (dict(y_type=MX4), "output type"),
     (dict(act=13), "activation"), (dict(act=-1), "activation"), (dict(gated=1, act=1), "gated"), (dict(E=2), "offsets"), (dict(M=5), "row list"),
     (dict(x_ld=63), "stride"), (dict(y_ld=7), "stride"),
 ])
