@@ -362,7 +362,7 @@ int sm_mx4_dequantize(const void* codes, const void* scales, int64_t rows, int32
 /* y[s][n] = act(bias[e][n] + sum_k x[r(s)][k] * w[e][n][k]) for the slots s of group e: offsets[e] <= s < offsets[e + 1], r(s) = rows ? rows[s] : s.
  * gated: y[s][n] = silu(z[s][n]) * z[s][N + n], z = product + bias over the 2 N weight rows (gate rows first).
  * `offsets` (device, E + 1 ascending values) may be NULL when E = 1: all M slots then.  Slots that no group covers are left as they were.  Offsets are read as clamped to 0 .. M; a row index
- * outside 0 .. T - 1 reads as a row of zeros.  fp32 accumulation, one rounding to y_type. */
+ * outside 0 .. T - 1 gives a product of zero, whatever the weights hold.  fp32 accumulation, one rounding to y_type. */
 typedef struct sm_linear_desc {
     int64_t M, T;                   /* slots (rows of y); rows of x */
     int32_t N, K, E;                /* columns of y, inner size, groups (1 = an ordinary layer) */

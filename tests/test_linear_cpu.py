@@ -143,3 +143,16 @@ def test_sizes_that_would_overflow():
     q, dq = N.lib().sm_mx4_quantize, N.lib().sm_mx4_dequantize
     refused(q(P, F16, 1 << 40, (1 << 31) - 1, (1 << 31) - 1, P, P, None), "elements")
     refused(dq(P, P, 1 << 40, (1 << 31) - 1, P, F16, (1 << 31) - 1, None), "elements")
+
+
+def test_scratch_is_asked_for():
+    """a product whose K is cut into runs, and fp32 rows, want scratch; a call without it is refused; few rows want none"""
+    size = N.lib().sm_linear_workspace_bytes
+    cut = desc(M=64, T=64, N=2048, K=8192)
+    assert size(C.byref(cut), 0, 0) % (64 * 2048 * 4) == 0 and size(C.byref(cut), 0, 0) > 0
+    refused(linear(cut), "workspace")
+    assert size(C.byref(desc(M=16, T=16, N=2048, K=8192)), 0, 0) == 0
+    wide = desc(M=4, T=4, N=8, K=64, x_type=F32)
+    assert size(C.byref(wide), 1, 0) >= 2 * 4 * (64 * 2 + 8 * 4)
+    refused(linear(wide), "workspace")
+    refused(linear(desc(M=1 << 30, T=1 << 30, x_type=F32)), "fp32 rows")
