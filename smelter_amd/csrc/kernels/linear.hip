@@ -79,33 +79,82 @@ static LinearPlan lin_plan(const sm_linear_desc* d, bool grouped, bool gathered)
     return plan;
 }
 
-// fp32 rows: each becomes two 16-bit ones, its value rounded and what the rounding left (bf16: 16 bits together; fp16, under fp16 weights, 22 inside its range), the product runs on twice the rows —
-// the weights are read once — and lin_join_kernel adds the two sums.  192 slots on 32 experts of 2048 x 1024 in MX4: 25 us (3.5 + 12 + 5.6, three launches) against 13 of bf16 rows.
-template <class H> __global__ void lin_parts_kernel(const float* x, long long x_ld, const int* offsets, const int* rows, long long M, long long T, int K, int E, H* out, long long ld, int* twice) {
-    if (offsets && blockIdx.x == 0) for (int e = threadIdx.x; e <= E; e += blockDim.x) twice[e] = (int)(2 * lin_clamp(offsets[e], M));
-    const unsigned quads = ((unsigned)K + 3) >> 2;
-    const unsigned long long units = (unsigned long long)M * quads;
-    for (unsigned long long u = (unsigned long long)blockIdx.x * blockDim.x + threadIdx.x; u < units; u += (unsigned long long)gridDim.x * blockDim.x) {
-        const long long s = u < 0xffffffffull ? (long long)((unsigned)u / quads) : (long long)(u / quads);
-        const int k = (int)(u - (unsigned long long)s * quads) * 4;
+// fp32 rows: each becomes several 16-bit ones that add up to it, the product runs on all of them — the weights are read once — and lin_join_kernel adds their sums, bias and activation.
+// bf16 (under bf16 and MX4 weights): the value rounded and what the rounding left, 16 bits together.
+// fp16 (under fp16 weights): fp16 ends at 65504 and holds nothing below 2^-24, so a row is first scaled by a power of two that puts its largest value at 2^15 .. 2^16; then three parts, 2^-11 apart,
+// each cut (not rounded), so that none passes 65504.  They hold all 24 bits of every value down to 2^-38 of the largest.  A row with smaller ones, an infinity or a NaN is marked: its parts are zero,
+// the join leaves it out, and lin_stream_kernel multiplies it in fp32 (one launch more, 4 us where no row is marked).  4096 rows of 4096 x 4096: 511 us, 1870 where all are marked.
+// 192 slots on 32 experts of 2048 x 1024 in MX4: 25 us (3.5 + 12 + 5.6, three launches) against 13 of bf16 rows.
+__device__ __forceinline__ floatx4 lin_load4(const float* row, int k, int K) {       // zero behind the row's end
+    floatx4 v = {0, 0, 0, 0};
+    if (k + 4 <= K) __builtin_memcpy(&v, row + k, 16);
+    else for (int q = 0; q < 3; q++) if (k + q < K) v[q] = row[k + q];
+    return v;
+}
+template <class H> constexpr int LIN_PARTS = std::is_same_v<H, half_t> ? 3 : 2;
+template <class H> __global__ __launch_bounds__(256) void lin_parts_kernel(const float* x, long long x_ld, const int* offsets, const int* rows, long long M, long long T, int K, int E, H* out, long long ld,
+                                                                           int* more, int* power) {
+    constexpr int PARTS = LIN_PARTS<H>;
+    constexpr bool SCALED = std::is_same_v<H, half_t>;
+    if (offsets && blockIdx.x == 0) for (int e = threadIdx.x; e <= E; e += blockDim.x) more[e] = (int)(PARTS * lin_clamp(offsets[e], M));
+    __shared__ unsigned ends[2][4];                                                  // largest magnitude, smallest one that is not 0, of the waves
+    for (long long s = blockIdx.x; s < M; s += gridDim.x) {                          // a block to a slot
         const long long r = rows ? rows[s] : s;
         const bool live = r >= 0 && r < T;
-        for (int i = 0; i < 4 && k + i < K; i++) {
-            const float v = live ? x[r * x_ld + k + i] : 0.f;
-            const H hi = (H)v;
-            const float left = v - (float)hi;
-            out[2 * s * ld + k + i] = hi;
-            out[(2 * s + 1) * ld + k + i] = (H)(__builtin_fabsf((float)hi) < __builtin_inff() ? left : 0.f);    // (an infinity, a NaN: once)
+        const float* src = x + (live ? r : 0) * x_ld;
+        int up = 0; bool marked = false;
+        if constexpr (SCALED) {
+            unsigned hi = 0, lo = ~0u;
+            for (int k = 4 * threadIdx.x; k < K && live; k += 1024) {
+                const floatx4 v = lin_load4(src, k, K);
+#pragma unroll
+                for (int q = 0; q < 4; q++) { const float f = v[q]; const unsigned b = __builtin_bit_cast(unsigned, f) & 0x7fffffffu; hi = hi > b ? hi : b; if (b) lo = lo < b ? lo : b; }
+            }
+#pragma unroll
+            for (int d = 1; d < 64; d <<= 1) { const unsigned a = __shfl_xor(hi, d), c = __shfl_xor(lo, d); hi = hi > a ? hi : a; lo = lo < c ? lo : c; }
+            __syncthreads();                                                         // (of the slot before)
+            if ((threadIdx.x & 63) == 0) { ends[0][threadIdx.x >> 6] = hi; ends[1][threadIdx.x >> 6] = lo; }
+            __syncthreads();
+#pragma unroll
+            for (int w = 0; w < 4; w++) { const unsigned a = ends[0][w], c = ends[1][w]; hi = hi > a ? hi : a; lo = lo < c ? lo : c; }
+            if (hi) {
+                up = 16 - __builtin_amdgcn_frexp_expf(__builtin_bit_cast(float, hi));    // |v| < 2^(16 - up)
+                marked = hi >= 0x7f800000u || ldexpf(__builtin_bit_cast(float, lo), up) < 0x1p-23f;
+            }
+            if (threadIdx.x == 0) power[s] = marked ? LIN_MARKED : -up;
+        }
+        H* to = out + PARTS * s * ld;
+        typedef H H4 __attribute__((ext_vector_type(4)));
+        for (int k = 4 * threadIdx.x; k < K; k += 1024) {                           // (rows of the parts end behind a whole quad)
+            floatx4 v = {0, 0, 0, 0};
+            if (live && !marked) v = lin_load4(src, k, K);
+            H4 h[PARTS];
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                if constexpr (SCALED) {
+                    float left = ldexpf(v[q], up);
+#pragma unroll
+                    for (int i = 0; i < PARTS; i++) { h[i][q] = __builtin_bit_cast(half2_t, __builtin_amdgcn_cvt_pkrtz(left, left))[0]; left = (left - (float)h[i][q]) * 0x1p11f; }
+                } else {
+                    h[0][q] = (H)v[q];
+                    h[1][q] = (H)(__builtin_fabsf((float)h[0][q]) < __builtin_inff() ? v[q] - (float)h[0][q] : 0.f);    // (an infinity, a NaN: once)
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < PARTS; i++) *(H4*)(to + i * ld + k) = h[i];
         }
     }
 }
-struct LinearParts { sm_linear_desc in; size_t twice, sums, inner, total; };        // the product on the parts; where its offsets, its sums and its own workspace lie behind them
+struct LinearParts { sm_linear_desc in; int parts; size_t more, power, sums, inner, total; };   // the product on the parts of every row; where its offsets, the rows' powers of two, its sums and its own workspace lie behind them
 static LinearParts lin_parts(const sm_linear_desc* d, bool grouped) {
     LinearParts a; a.in = *d;
     auto up = [](size_t n) { return (n + 255) / 256 * 256; };
-    a.in.M = a.in.T = 2 * d->M; a.in.N = d->gated ? 2 * d->N : d->N; a.in.gated = 0; a.in.act = SM_ACT_NONE;
-    a.in.x_type = d->w_type == SM_F16 ? SM_F16 : SM_BF16; a.in.y_type = SM_F32; a.in.x_ld = (d->K + 7ll) / 8 * 8; a.in.y_ld = lin_part_ld(a.in.N);
-    a.twice = up((size_t)a.in.M * a.in.x_ld * 2); a.sums = a.twice + up(grouped ? (d->E + 1ll) * 4 : 0); a.inner = a.sums + up((size_t)a.in.M * a.in.y_ld * 4);
+    const bool scaled = d->w_type == SM_F16;
+    a.parts = scaled ? LIN_PARTS<half_t> : LIN_PARTS<bf16_t>;
+    a.in.M = a.in.T = a.parts * d->M; a.in.N = d->gated ? 2 * d->N : d->N; a.in.gated = 0; a.in.act = SM_ACT_NONE;
+    a.in.x_type = scaled ? SM_F16 : SM_BF16; a.in.y_type = SM_F32; a.in.x_ld = (d->K + 7ll) / 8 * 8; a.in.y_ld = lin_part_ld(a.in.N);
+    a.more = up((size_t)a.in.M * a.in.x_ld * 2); a.power = a.more + up(grouped ? (d->E + 1ll) * 4 : 0); a.sums = a.power + up(scaled ? (size_t)d->M * 4 : 0);
+    a.inner = a.sums + up((size_t)a.in.M * a.in.y_ld * 4);
     a.total = a.inner + sm_linear_workspace_bytes(&a.in, grouped, 0);
     return a;
 }
@@ -151,19 +200,23 @@ extern "C" int sm_linear_fwd(const sm_linear_desc* d, const void* x, const void*
     p.y_vec = (size_t)y % 16 == 0 && p.y_ld * ye % 16 == 0;
     hipStream_t s = sm_s(stream);
     if (x32) {
-        SM_REQUIRE(d->M < (1ll << 30) && d->M * ((d->N + 3ll) / 4) < (1ll << 31), "linear: %lld x %d outputs of fp32 rows exceed one launch", (long long)d->M, d->N);
+        SM_REQUIRE(d->M < (1ll << 31) / 3 && d->M * ((d->N + 3ll) / 4) < (1ll << 31), "linear: %lld x %d outputs of fp32 rows exceed one launch", (long long)d->M, d->N);
         const LinearParts a = lin_parts(d, offsets != nullptr);
         SM_REQUIRE(workspace && (size_t)workspace % 256 == 0 && workspace_bytes >= a.total, "linear: workspace of %zu bytes (256-byte aligned), %zu wanted", workspace_bytes, a.total);
         char* at = (char*)workspace;
-        int* twice = offsets ? (int*)(at + a.twice) : nullptr;
-        const long long blocks = (d->M * ((d->K + 3ll) / 4) + 255) / 256, cap = (long long)SM_NUM_CU * 32;
-        const dim3 grid((unsigned)(blocks < 1 ? 1 : blocks < cap ? blocks : cap));
-        if (a.in.x_type == SM_F16) lin_parts_kernel<half_t><<<grid, 256, 0, s>>>((const float*)x, p.x_ld / 4, offsets, rows, d->M, d->T, d->K, d->E, (half_t*)at, a.in.x_ld, twice);
-        else lin_parts_kernel<bf16_t><<<grid, 256, 0, s>>>((const float*)x, p.x_ld / 4, offsets, rows, d->M, d->T, d->K, d->E, (bf16_t*)at, a.in.x_ld, twice);
+        int* more = offsets ? (int*)(at + a.more) : nullptr;
+        int* power = a.in.x_type == SM_F16 ? (int*)(at + a.power) : nullptr;
+        const dim3 grid((unsigned)(d->M < SM_NUM_CU * 64 ? d->M : SM_NUM_CU * 64));
+        if (power) lin_parts_kernel<half_t><<<grid, 256, 0, s>>>((const float*)x, p.x_ld / 4, offsets, rows, d->M, d->T, p.K, d->E, (half_t*)at, a.in.x_ld, more, power);
+        else lin_parts_kernel<bf16_t><<<grid, 256, 0, s>>>((const float*)x, p.x_ld / 4, offsets, rows, d->M, d->T, p.K, d->E, (bf16_t*)at, a.in.x_ld, more, nullptr);
         SM_LAUNCH_CHECK();
-        if (int rc = sm_linear_fwd(&a.in, at, nullptr, w, w_scales, nullptr, twice, nullptr, at + a.sums, at + a.inner, workspace_bytes - a.inner, stream)) return rc;
-        p.part = (float*)(at + a.sums); p.part_ld = a.in.y_ld; p.splits = 2; p.pairs = 1;
-        return lin_join_launch(p, s);
+        sm_linear_desc in = a.in; in.K = p.K;                                        // (without a row of x nothing of w is read)
+        if (int rc = sm_linear_fwd(&in, at, nullptr, w, w_scales, nullptr, more, nullptr, at + a.sums, at + a.inner, workspace_bytes - a.inner, stream)) return rc;
+        LinearParams j = p;
+        j.part = (float*)(at + a.sums); j.part_ld = a.in.y_ld; j.splits = j.parts = a.parts; j.power = power;
+        if (int rc = lin_join_launch(j, s)) return rc;
+        p.power = power;
+        return power ? lin_stream<SM_F32, SM_F16>(p, s) : SM_OK;
     }
     LinearPlan plan = lin_plan(d, offsets != nullptr, rows != nullptr);
     if (plan.shape >= 0) {

@@ -15,6 +15,7 @@ typedef int intx4_t __attribute__((ext_vector_type(4)));
 typedef int intx8_t __attribute__((ext_vector_type(8)));
 typedef float floatx2_t __attribute__((ext_vector_type(2)));
 
+#define LIN_MARKED (-(1 << 30))
 struct LinearParams {
     const char* x; const unsigned char* xs;         // x rows; scales of an MX4 x
     const char* w; const unsigned char* ws;
@@ -26,7 +27,8 @@ struct LinearParams {
     int N, K, E, act; float slope;
     int gated, y_type, y_vec, w_rows;               // y_vec: eight consecutive outputs may be stored as 16-byte words;  w_rows = N or 2 N
     float* part; long long part_ld; int splits;     // fp32 sums [splits][M][part_ld] of a product whose K is cut into `splits` runs (1: none)
-    int pairs;                                      // (lin_join_kernel) the sums are [M][2][part_ld], of the two parts of fp32 rows
+    int parts;                                      // (lin_join_kernel) not 0: the sums are [M][parts][part_ld], of the parts of fp32 rows
+    const int* power;                               // fp32 rows in fp16 parts: the power of two of each slot's row, or LIN_MARKED: multiplied in fp32
     long long m_tiles; int n_tiles;                 // launch grid: a bound on the row tiles (the real number is known on the device only) x column tiles
 };
 
@@ -146,6 +148,8 @@ template <int KIND> __device__ __forceinline__ floatx16 lin_mma16(intx4_t a, int
     if constexpr (KIND == SM_F16) return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8_t, a), __builtin_bit_cast(half8_t, b), c, 0, 0, 0);
     else return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
 }
+// 16 x 16 x 4 product of fp32 elements: lane l holds row l & 15 and one k, l >> 4; the result lies as that of 16 x 16 x 32
+__device__ __forceinline__ floatx4 lin_mma32(float a, float b, floatx4 c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
 // 16 x 16 x 128 (32 x 32 x 64) product of MX4 fragments: lane l holds row l % 16 (32) and one block of 32, with its scale in byte SEL of sa, in the low byte of sb
 template <int SEL> __device__ __forceinline__ floatx4 lin_mma4(intx4_t a, int sa, intx4_t b, int sb, floatx4 c) {
     const intx8_t va = __builtin_shufflevector(a, a, 0, 1, 2, 3, -1, -1, -1, -1), vb = __builtin_shufflevector(b, b, 0, 1, 2, 3, -1, -1, -1, -1);   // (a 4-bit operand is four registers)

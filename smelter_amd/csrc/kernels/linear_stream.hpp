@@ -7,14 +7,25 @@
 // lanes without a slot load no x, and where there are blocks enough a wave takes four groups of weight rows with the same x.
 // MX4 weights under 16-bit x become 16-bit values in the registers.  bf16: value times scale, exact.  fp16: the range of 2^-24 .. 65504 does not hold every scale, so the values are taken
 // relative to the largest scale of their row in these 512 k and the partial sum is multiplied by it in fp32 (a block 2^23 below that neighbour rounds, by less than the fp32 sum does).
+// fp32 x on fp16 weights (the rows that fp16 parts do not hold, linear.hip): the weights become fp32 values and the products are those of the fp32 matrix instruction, 1/16 of the fp16 rate.
 #pragma once
 #include "linear.hpp"
 
 // 32 k of a row for a lane of group g.  ROW (16-bit x and weights): eight k of each of the blocks b .. b + 3, so that a row's four lanes read 64 bytes side by side (16 rows of 8192 x 8192: 31.1 us
 // against 32.8 with a block for each); otherwise the lane's own block b: four loads of eight, or one of 32 MX4 codes.
-template <int KIND> struct LinBlk { static constexpr int NV = KIND == SM_MX4 ? 1 : 4; intx4_t v[NV]; };
+template <int KIND> struct LinBlk { static constexpr int NV = KIND == SM_MX4 ? 1 : KIND == SM_F32 ? 8 : 4; intx4_t v[NV]; };
 template <int KIND, bool ROW> __device__ __forceinline__ void lin_load_block(LinBlk<KIND>& f, const char* row, int b, int g, int nb, int K) {
-    if constexpr (ROW) {
+    if constexpr (KIND == SM_F32) {                                     // the same k as of a 16-bit operand with ROW
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int k = 32 * (b + i) + 8 * g;
+            if (k + 8 <= K) { __builtin_memcpy(&f.v[2 * i], row + 4ll * k, 16); __builtin_memcpy(&f.v[2 * i + 1], row + 4ll * k + 16, 16); }
+            else {
+#pragma unroll
+                for (int q = 0; q < 8; q++) { int e = 0; if (k + q < K) __builtin_memcpy(&e, row + 4ll * (k + q), 4); f.v[2 * i + (q >> 2)][q & 3] = e; }
+            }
+        }
+    } else if constexpr (ROW) {
         if (32 * b + 128 <= K) {
 #pragma unroll
             for (int i = 0; i < 4; i++) __builtin_memcpy(&f.v[i], row + 64ll * (b + i) + 16 * g, 16);
@@ -61,7 +72,13 @@ template <int XK, int WK, int NB> __global__ __launch_bounds__(512) void lin_str
     const int cols = p.gated ? 16 * G : 16 * NB, n0 = nt * cols;
     long long xrow = tile.row0 + (r < tile.rows ? r : 0);
     if (p.rows) xrow = p.rows[xrow];
-    const bool live = r < tile.rows && xrow >= 0 && xrow < p.T;         // lanes without a slot, and row indices outside x: zeros
+    bool live = r < tile.rows;
+    if constexpr (XK == SM_F32) {                                       // the marked rows only
+        live = live && p.power[tile.row0 + r] == LIN_MARKED;
+        if (!__any(live)) return;
+    }
+    const unsigned wanted = (unsigned)__ballot(live);
+    live = live && xrow >= 0 && xrow < p.T;         // lanes without a slot, and row indices outside x: zeros
     if (!live) xrow = 0;
     const char* xr = p.x + xrow * p.x_ld; const unsigned char* xsr = p.xs + xrow * p.xs_ld;
     const int xk = live ? p.K : 0, xnb = live ? nb : 0;
@@ -106,6 +123,18 @@ template <int XK, int WK, int NB> __global__ __launch_bounds__(512) void lin_str
                     for (int b = 0; b < NB; b++) acc[b] = lin_mma4<0>(x.v[0], (int)(sx >> (8 * j)), w[u][b][j].v[0], (int)(sw[b] >> (8 * j)), acc[b]);
                 }
             }
+        } else if constexpr (XK == SM_F32) {
+            static_assert(WK == SM_F16, "fp32 rows: fp16 weights (others take bf16 parts of them)");
+            LinBlk<XK> x;
+            lin_load_block<XK, true>(x, xr, c, g, nb, xk);
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+#pragma unroll
+                for (int q = 0; q < 8; q++) {
+                    const float xe = __builtin_bit_cast(float, (int)x.v[2 * i + (q >> 2)][q & 3]);
+#pragma unroll
+                    for (int b = 0; b < NB; b++) acc[b] = lin_mma32(xe, (float)__builtin_bit_cast(half8_t, w[0][b][0].v[i])[q], acc[b]);
+                }
         } else {
             constexpr bool OWN = MXW && XK == SM_F16;                   // sums of their own, multiplied by `mul`
             float mul[NB]; int top[NB]; floatx4 sum[NB];
@@ -164,7 +193,7 @@ template <int XK, int WK, int NB> __global__ __launch_bounds__(512) void lin_str
     const int total = cols * tile.rows;
     for (int o = threadIdx.x; o < total; o += blockDim.x) {
         const int i = o / cols, c = o - i * cols, n = n0 + c;
-        if (n >= p.N) continue;
+        if (n >= p.N || (XK == SM_F32 && !(wanted >> i & 1))) continue;
         float v[2] = {0.f, 0.f};
         for (int h = 0; h < (p.gated ? 2 : 1); h++) {
             const int b = (c >> 4) + h * G;

@@ -13,7 +13,7 @@ int lin_tile_launch(const LinearParams& p, int x_kind, int w_kind, int shape, bo
     return x_kind == SM_F16 ? lin_tile_shape<SM_F16, SM_F16>(p, shape, dma, s) : lin_tile_shape<SM_BF16, SM_BF16>(p, shape, dma, s);
 }
 
-// Joins the runs of a split product, or the products of the two parts of fp32 rows: y = act(sum of the runs, in their order, + bias).  One thread per four
+// Joins the runs of a split product, or the products of the parts of fp32 rows: y = act(sum of the runs, in their order, + bias).  One thread per four
 // columns of a slot; the group of a slot (for its bias) is found in the offsets.  Bound by the reading of the sums and its own launch: 3 - 6 us.
 __global__ void lin_join_kernel(LinearParams p) {
     const int quads = (p.N + 3) >> 2;
@@ -26,21 +26,25 @@ __global__ void lin_join_kernel(LinearParams p) {
             for (int b = p.E; e < b;) { const int mid = (e + b + 1) >> 1; if (lin_clamp(p.offsets[mid], p.M) <= s) e = mid; else b = mid - 1; }
             if (e == p.E || lin_clamp(p.offsets[e], p.M) > s || lin_clamp(p.offsets[e + 1], p.M) <= s) continue;
         }
+        const int power = p.power ? p.power[s] : 0;
+        if (power == LIN_MARKED) continue;
+        const float apart = p.power ? 0x1p-11f : 1.f;                                // a part against the one before it
         floatx4 z[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
         for (int h = 0; h <= p.gated; h++) {
             const int c = n + (h ? p.N : 0);
-            const float* src = p.part + (p.pairs ? 2ll : 1ll) * s * p.part_ld + c;
+            const float* src = p.part + (p.parts ? (long long)p.parts : 1ll) * s * p.part_ld + c;
+            const long long step = p.parts ? p.part_ld : p.M * p.part_ld;
+            float scale = 1.f;
             if (vec) {
 #pragma unroll 4
-                for (int q = 0; q < p.splits; q++) z[h] += *(const floatx4*)(src + q * (p.pairs ? p.part_ld : p.M * p.part_ld));
+                for (int q = 0; q < p.splits; q++) { z[h] += *(const floatx4*)(src + q * step) * scale; scale *= apart; }
             } else {
-                for (int q = 0; q < p.splits; q++)
-                    for (int i = 0; i < 4; i++) if (n + i < p.N) z[h][i] += src[q * (p.pairs ? p.part_ld : p.M * p.part_ld) + i];
+                for (int q = 0; q < p.splits; q++) { for (int i = 0; i < 4; i++) if (n + i < p.N) z[h][i] += src[q * step + i] * scale; scale *= apart; }
             }
-            if (p.pairs) {
-                // under an infinite weight the second part's sum may be 0 times infinity: an infinity of the first stands; a slot without a row of x is zero (of runs, the sums are already)
+            if (p.parts) {
+                // under an infinite weight a later part's sum may be 0 times infinity: an infinity of the first stands; a slot without a row of x is zero (of runs, the sums are already)
                 const bool none = p.rows && (p.rows[s] < 0 || p.rows[s] >= p.T);
-                for (int i = 0; i < 4; i++) { const float first = n + i < p.N ? src[i] : 0.f; z[h][i] = none ? 0.f : __builtin_fabsf(first) == __builtin_inff() ? first : z[h][i]; }
+                for (int i = 0; i < 4; i++) { const float first = n + i < p.N ? src[i] : 0.f; z[h][i] = none ? 0.f : __builtin_fabsf(first) == __builtin_inff() ? first : ldexpf(z[h][i], power); }
             }
             if (p.bias) for (int i = 0; i < 4; i++) if (n + i < p.N) z[h][i] += p.bias[(long long)e * p.w_rows + c + i];
         }

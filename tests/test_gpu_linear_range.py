@@ -1,0 +1,123 @@
+"""Linear and expert layers over the whole range of their operands: rows of very large, very small and mixed values, weights whose scales lie far apart.
+Every limit here is relative to the sum of the products' own magnitudes: nothing is allowed for values that a product does not hold."""
+import pytest
+import torch
+
+from smelter_amd import ops
+
+pytestmark = pytest.mark.gpu
+F16, BF16, F32, F64 = torch.float16, torch.bfloat16, torch.float32, torch.float64
+INF, NAN = float("inf"), float("nan")
+
+
+def gen(seed):
+    return torch.Generator("cuda").manual_seed(seed)
+
+
+def randn(g, *shape):
+    return torch.randn(shape, generator=g, device="cuda")
+
+
+def chain(k):
+    """An fp32 sum of k exact products, in any order: at most k + 16 additions (16: partial sums of waves, lane groups, runs and parts) that round by half a step, 2^-24, or are cut, 2^-23"""
+    return (k + 16) * 2.0 ** -23
+
+
+def inside(got, want, lim, what=""):
+    """|got - want| <= lim + half a step of got's type (its smallest value's half below its range); the same infinities and NaN"""
+    assert torch.equal(torch.isnan(got), torch.isnan(want)), what
+    inf = torch.isinf(want)
+    assert torch.equal(got.double()[inf], want[inf]), what
+    info = torch.finfo(got.dtype)
+    fine = torch.isfinite(want) & (want.abs() + lim < info.max)         # (near the end of the range a value may round to an infinity)
+    off = (got.double() - want).abs() - lim - info.eps / 2 * (want.abs() + lim) - info.smallest_normal * info.eps / 2
+    bad = fine & ~(off <= 0)
+    assert not bad.any(), "%s: off by %.3g of %.3g where %.3g is allowed, at %s" % (what, (got.double() - want).abs()[bad][0], want[bad][0], lim.expand_as(want)[bad][0], bad.nonzero()[0].tolist())
+
+
+def gate(z, lim, n):
+    """silu(a) * b of the halves: |silu'| < 1.1; the exponential, the reciprocal and the products below 2^-19 of the result"""
+    a, b, la, lb = z[:, :n], z[:, n:], lim[:, :n], lim[:, n:]
+    s = a * torch.sigmoid(a)
+    return s * b, 1.1 * la * b.abs() + s.abs() * lb + 1.1 * la * lb + 2.0 ** -19 * (s * b).abs()
+
+
+def fp32_rows(g, m, k):
+    """rows whose magnitudes differ: all near 1e5, 1e-5, 1e-8, 1e30, 1e-30, of one magnitude for each element, with loud columns, behind a loud first column"""
+    x = randn(g, m, k)
+    scale = torch.tensor([1e5, 1e-5, 1e-8, 1e30, 1e-30, 1.0, 1.0, 1e-8], device="cuda")[torch.arange(m, device="cuda") % 8]
+    x = x * scale[:, None]
+    mixed = torch.arange(m, device="cuda") % 8 == 5
+    x = torch.where(mixed[:, None], x * 10.0 ** torch.randint(-9, 6, (m, k), generator=g, device="cuda").float(), x)
+    loud = torch.arange(m, device="cuda") % 8 >= 6
+    x[:, 0] = torch.where(loud, torch.full_like(x[:, 0], 7e4), x[:, 0])
+    return x
+
+
+def same_as_fp64(x, w, wv, off, rows, bias, gated, dtype, more=0.0):
+    """fp32 rows on weights [2, N, K]; `more`: of the products' magnitudes, allowed beside the sum's own error"""
+    got = ops.expert_linear(x, w, off, rows, bias, gated=gated, dtype=dtype)
+    t, k = x.shape
+    n = wv.shape[1] // (2 if gated else 1)
+    ok = ((rows >= 0) & (rows < t))[:, None]
+    xv = torch.where(ok, x.double()[rows.clamp(0, t - 1).long()], torch.zeros((), dtype=F64, device="cuda"))
+    for e in range(2):
+        s = slice(int(off[e]), int(off[e + 1]))
+        z, mag = xv[s] @ wv[e].t() + bias[e].double(), xv[s].abs() @ wv[e].abs().t()
+        lim = (chain(k) + more) * mag + 2.0 ** -23 * z.abs() + 2.0 ** -126
+        if gated:
+            z, lim = gate(z, lim, n)
+        inside(got[s], z, lim, "group %d" % e)
+    return got
+
+
+@pytest.mark.parametrize("gated, dtype", [(False, F32), (True, F32), (False, BF16), (True, F16)])
+@pytest.mark.parametrize("m, n, k", [(1, 24, 1), (8, 40, 96), (40, 130, 261), (96, 256, 4096), (64, 2048, 2048), (1500, 1000, 72)])
+def test_fp32_rows_on_fp16_weights(gated, dtype, m, n, k):
+    """no row is too large, too small or too mixed (some are multiplied in other ways than others).  Some weight rows are zero where the loud column is"""
+    g = gen(m + n + k)
+    x = torch.full((m, k + 3), NAN, device="cuda")[:, 2:k + 2]
+    x.copy_(fp32_rows(g, m, k))
+    w = (randn(g, 2, 2 * n if gated else n, k) * k ** -0.5).to(F16)
+    w[:, ::3, 0] = 0
+    rows = torch.randint(-1, m + 1, (m + 5,), generator=g, device="cuda").int()          # -1, m: no row of x
+    off = torch.tensor([0, m // 3 + 1, m + 5], dtype=torch.int32, device="cuda")
+    same_as_fp64(x, w, w.double(), off, rows, randn(g, 2, w.shape[1]) * 1e-8, gated, dtype)
+
+
+def test_fp32_rows_on_fp16_weights_one_by_one():
+    """values whose fp16 form is an infinity, coarse or zero"""
+    off = torch.tensor([0, 5], dtype=torch.int32, device="cuda")
+    x = torch.tensor([[7e4], [3e-5], [1e-6], [2e-8], [1e-9]], device="cuda")
+    w = torch.tensor([[[0.1], [1.0]]], device="cuda").to(F16)
+    want = x.double() * w[0, :, 0].double()
+    inside(ops.expert_linear(x, w, off), want, 2.0 ** -23 * want.abs())
+    w[0, 1] = INF
+    got = ops.expert_linear(x, w, off)
+    assert got[:, 1].eq(INF).all() and torch.isfinite(got[:, 0]).all()
+    assert torch.equal(ops.expert_linear(-x, w, off), -got)
+    # two large terms of opposite signs
+    pair = torch.tensor([[7e4, -7e4]] * 5, device="cuda")
+    assert ops.expert_linear(pair, torch.ones((1, 8, 2), dtype=F16, device="cuda"), off).eq(0).all()
+    # an infinity and a NaN beside small values
+    odd = torch.tensor([[INF, 1e-9], [-INF, 1e-9], [NAN, 1.0], [INF, -INF], [1e-9, 1.0]], device="cuda")
+    got = ops.expert_linear(odd, torch.ones((1, 8, 2), dtype=F16, device="cuda"), off)
+    assert got[0].eq(INF).all() and got[1].eq(-INF).all() and got[2:4].isnan().all() and got[4].eq(1).all()
+
+
+def test_fp32_rows_on_fp16_weights_in_a_graph():
+    """which rows are multiplied in another way is decided on the device: a replay goes by the present rows"""
+    g = gen(3)
+    fine, odd = randn(g, 70, 256), fp32_rows(g, 70, 256)
+    x, w = fine.clone(), (randn(g, 2, 96, 256) / 16).to(F16)
+    off = torch.tensor([0, 30, 70], dtype=torch.int32, device="cuda")
+    ops.expert_linear(x, w, off)
+    torch.cuda.synchronize()
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):
+        y = ops.expert_linear(x, w, off)
+    for turn in range(4):
+        x.copy_(odd.roll(turn, 0) if turn % 2 else fine)
+        gr.replay()
+        assert torch.equal(y, ops.expert_linear(x, w, off)), turn
+        torch.cuda.synchronize()
