@@ -368,8 +368,8 @@ typedef struct sm_linear_desc {
     int32_t N, K, E;                /* columns of y, inner size, groups (1 = an ordinary layer) */
     int32_t x_type, w_type, y_type; /* fp16 | bf16 x on weights of the same type or MX4, y of x's type, fp16 (three bits more for what a
                                      next layer with MX4 weights takes) or fp32; MX4 x on MX4 weights, any y;
-                                     fp32 x on 16-bit or MX4 weights, any y: on fp16 weights every row keeps its 24 bits (three parts of fp16
-                                     and a power of two of its own; rows that reach further than 2^38 are multiplied in fp32), on others it is carried as two parts of bf16 */
+                                     fp32 x on 16-bit or MX4 weights, any y: every row keeps its 24 bits (three parts of bf16; of fp16 under fp16 weights, with
+                                     a power of two of the row's own; rows that reach further than 2^38 are multiplied in fp32) */
     int32_t act; float slope;       /* SM_ACT_* behind the bias (not with gated) */
     int32_t gated;
     int64_t x_ld, y_ld;             /* row strides in elements, 0 = dense (an MX4 x is dense) */

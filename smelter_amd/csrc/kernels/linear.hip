@@ -80,21 +80,21 @@ static LinearPlan lin_plan(const sm_linear_desc* d, bool grouped, bool gathered)
 }
 
 // fp32 rows: each becomes several 16-bit ones that add up to it, the product runs on all of them — the weights are read once — and lin_join_kernel adds their sums, bias and activation.
-// bf16 (under bf16 and MX4 weights): the value rounded and what the rounding left, 16 bits together.
+// bf16 (under bf16 and MX4 weights): three parts of eight bits, each cut, not rounded: all 24 bits, and no part is infinite where the value is not.
 // fp16 (under fp16 weights): fp16 ends at 65504 and holds nothing below 2^-24, so a row is first scaled by a power of two that puts its largest value at 2^15 .. 2^16; then three parts, 2^-11 apart,
 // each cut (not rounded), so that none passes 65504.  They hold all 24 bits of every value down to 2^-38 of the largest.  A row with smaller ones, an infinity or a NaN is marked: its parts are zero,
-// the join leaves it out, and lin_stream_kernel multiplies it in fp32 (one launch more, 4 us where no row is marked).  4096 rows of 4096 x 4096: 511 us, 1870 where all are marked.
-// 192 slots on 32 experts of 2048 x 1024 in MX4: 25 us (3.5 + 12 + 5.6, three launches) against 13 of bf16 rows.
+// the join leaves it out, and lin_stream_kernel multiplies it in fp32 (one launch more, 4 us where no row is marked).  4096 rows of 4096 x 4096: 523 us, 1870 where all are marked.
+// 192 slots on 32 experts of 2048 x 1024 in MX4: 29 us (three launches) against 13 of bf16 rows; 4096 rows of 4096 x 4096: 464.
 __device__ __forceinline__ floatx4 lin_load4(const float* row, int k, int K) {       // zero behind the row's end
     floatx4 v = {0, 0, 0, 0};
     if (k + 4 <= K) __builtin_memcpy(&v, row + k, 16);
     else for (int q = 0; q < 3; q++) if (k + q < K) v[q] = row[k + q];
     return v;
 }
-template <class H> constexpr int LIN_PARTS = std::is_same_v<H, half_t> ? 3 : 2;
+#define LIN_PARTS 3
 template <class H> __global__ __launch_bounds__(256) void lin_parts_kernel(const float* x, long long x_ld, const int* offsets, const int* rows, long long M, long long T, int K, int E, H* out, long long ld,
                                                                            int* more, int* power) {
-    constexpr int PARTS = LIN_PARTS<H>;
+    constexpr int PARTS = LIN_PARTS;
     constexpr bool SCALED = std::is_same_v<H, half_t>;
     if (offsets && blockIdx.x == 0) for (int e = threadIdx.x; e <= E; e += blockDim.x) more[e] = (int)(PARTS * lin_clamp(offsets[e], M));
     __shared__ unsigned ends[2][4];                                                  // largest magnitude, smallest one that is not 0, of the waves
@@ -136,8 +136,13 @@ template <class H> __global__ __launch_bounds__(256) void lin_parts_kernel(const
 #pragma unroll
                     for (int i = 0; i < PARTS; i++) { h[i][q] = __builtin_bit_cast(half2_t, __builtin_amdgcn_cvt_pkrtz(left, left))[0]; left = (left - (float)h[i][q]) * 0x1p11f; }
                 } else {
-                    h[0][q] = (H)v[q];
-                    h[1][q] = (H)(__builtin_fabsf((float)h[0][q]) < __builtin_inff() ? v[q] - (float)h[0][q] : 0.f);    // (an infinity, a NaN: once)
+                    float left = v[q];
+#pragma unroll
+                    for (int i = 0; i < PARTS; i++) {
+                        const bool fine = __builtin_fabsf(left) < __builtin_inff();
+                        h[i][q] = fine ? (H)__builtin_bit_cast(float, __builtin_bit_cast(unsigned, left) & 0xffff0000u) : (H)left;
+                        left = fine ? left - (float)h[i][q] : 0.f;                   // (an infinity, a NaN: once)
+                    }
                 }
             }
 #pragma unroll
@@ -145,13 +150,12 @@ template <class H> __global__ __launch_bounds__(256) void lin_parts_kernel(const
         }
     }
 }
-struct LinearParts { sm_linear_desc in; int parts; size_t more, power, sums, inner, total; };   // the product on the parts of every row; where its offsets, the rows' powers of two, its sums and its own workspace lie behind them
+struct LinearParts { sm_linear_desc in; size_t more, power, sums, inner, total; };   // the product on the parts of every row; where its offsets, the rows' powers of two, its sums and its own workspace lie behind them
 static LinearParts lin_parts(const sm_linear_desc* d, bool grouped) {
     LinearParts a; a.in = *d;
     auto up = [](size_t n) { return (n + 255) / 256 * 256; };
     const bool scaled = d->w_type == SM_F16;
-    a.parts = scaled ? LIN_PARTS<half_t> : LIN_PARTS<bf16_t>;
-    a.in.M = a.in.T = a.parts * d->M; a.in.N = d->gated ? 2 * d->N : d->N; a.in.gated = 0; a.in.act = SM_ACT_NONE;
+    a.in.M = a.in.T = LIN_PARTS * d->M; a.in.N = d->gated ? 2 * d->N : d->N; a.in.gated = 0; a.in.act = SM_ACT_NONE;
     a.in.x_type = scaled ? SM_F16 : SM_BF16; a.in.y_type = SM_F32; a.in.x_ld = (d->K + 7ll) / 8 * 8; a.in.y_ld = lin_part_ld(a.in.N);
     a.more = up((size_t)a.in.M * a.in.x_ld * 2); a.power = a.more + up(grouped ? (d->E + 1ll) * 4 : 0); a.sums = a.power + up(scaled ? (size_t)d->M * 4 : 0);
     a.inner = a.sums + up((size_t)a.in.M * a.in.y_ld * 4);
@@ -200,7 +204,7 @@ extern "C" int sm_linear_fwd(const sm_linear_desc* d, const void* x, const void*
     p.y_vec = (size_t)y % 16 == 0 && p.y_ld * ye % 16 == 0;
     hipStream_t s = sm_s(stream);
     if (x32) {
-        SM_REQUIRE(d->M < (1ll << 31) / 3 && d->M * ((d->N + 3ll) / 4) < (1ll << 31), "linear: %lld x %d outputs of fp32 rows exceed one launch", (long long)d->M, d->N);
+        SM_REQUIRE(d->M < (1ll << 31) / LIN_PARTS && d->M * ((d->N + 3ll) / 4) < (1ll << 31), "linear: %lld x %d outputs of fp32 rows exceed one launch", (long long)d->M, d->N);
         const LinearParts a = lin_parts(d, offsets != nullptr);
         SM_REQUIRE(workspace && (size_t)workspace % 256 == 0 && workspace_bytes >= a.total, "linear: workspace of %zu bytes (256-byte aligned), %zu wanted", workspace_bytes, a.total);
         char* at = (char*)workspace;
@@ -213,7 +217,7 @@ extern "C" int sm_linear_fwd(const sm_linear_desc* d, const void* x, const void*
         sm_linear_desc in = a.in; in.K = p.K;                                        // (without a row of x nothing of w is read)
         if (int rc = sm_linear_fwd(&in, at, nullptr, w, w_scales, nullptr, more, nullptr, at + a.sums, at + a.inner, workspace_bytes - a.inner, stream)) return rc;
         LinearParams j = p;
-        j.part = (float*)(at + a.sums); j.part_ld = a.in.y_ld; j.splits = j.parts = a.parts; j.power = power;
+        j.part = (float*)(at + a.sums); j.part_ld = a.in.y_ld; j.splits = j.parts = LIN_PARTS; j.power = power;
         if (int rc = lin_join_launch(j, s)) return rc;
         p.power = power;
         return power ? lin_stream<SM_F32, SM_F16>(p, s) : SM_OK;

@@ -720,8 +720,8 @@ def _linear(name, index, x, w, lead, offsets, rows, bias, act, slope, gated, out
 
 def mx4_linear(x, w, bias=None, act=ACT_NONE, slope=0.0, gated=False, out=None, dtype=None):
     """act(x . w^T + bias) with MX4 weights w [N, K] (sm_linear_fwd).  x [M, K]: fp16 or bf16 (the weights are read as 16-bit values, the output has x's type, fp16 or fp32), or an Mx4 tensor
-    (both sides in 4 bits; dtype fp16 (default), bf16 or fp32).  What a bf16 layer hands to a next one with MX4 weights keeps three bits more as fp16 (beyond 65504: infinities).  fp32 x: carried as two
-    bf16 parts on twice the rows, any dtype (fp32 by default).  gated: w has 2 N rows and the result is silu(first N columns) * last N.  bias fp32 [rows of w]."""
+    (both sides in 4 bits; dtype fp16 (default), bf16 or fp32).  What a bf16 layer hands to a next one with MX4 weights keeps three bits more as fp16 (beyond 65504: infinities).  fp32 x: with all its
+    24 bits (three parts, on three times the rows), any dtype (fp32 by default).  gated: w has 2 N rows and the result is silu(first N columns) * last N.  bias fp32 [rows of w]."""
     if not isinstance(w, Mx4):
         _refuse("mx4_linear: the weights must be an Mx4 tensor")
     return _linear("mx4_linear", None, x, w, 0, None, None, bias, act, slope, gated, out, dtype)
@@ -729,7 +729,7 @@ def mx4_linear(x, w, bias=None, act=ACT_NONE, slope=0.0, gated=False, out=None, 
 
 def expert_linear(x, w, offsets, rows=None, bias=None, act=ACT_NONE, slope=0.0, gated=False, out=None, dtype=None):
     """Products grouped by expert (sm_linear_fwd): slot s of group e (offsets[e] <= s < offsets[e + 1]) gets act(x[rows[s]] . w[e]^T + bias[e]); without `rows` slot s is row s of x.
-    x [T, K] and w [E, N, K]: both fp16, both bf16, 16-bit x on Mx4 weights, both Mx4, or fp32 x on any (on fp16 weights with all its 24 bits).  offsets int32 [E + 1], rows int32 [slots], both on the GPU (MoePlan holds them): nothing is
+    x [T, K] and w [E, N, K]: both fp16, both bf16, 16-bit x on Mx4 weights, both Mx4, or fp32 x on any.  offsets int32 [E + 1], rows int32 [slots], both on the GPU (MoePlan holds them): nothing is
     read back to the host.  Slots that no group covers are left as they were (in a new `out`: unspecified).  gated, bias [E, rows of w], dtype: as in mx4_linear."""
     index = _gpu(None, "expert_linear", offsets, _INTS)
     wc = w.codes if isinstance(w, Mx4) else w

@@ -85,6 +85,38 @@ def test_fp32_rows_on_fp16_weights(gated, dtype, m, n, k):
     same_as_fp64(x, w, w.double(), off, rows, randn(g, 2, w.shape[1]) * 1e-8, gated, dtype)
 
 
+@pytest.mark.parametrize("weights", [BF16, "mx4"])
+@pytest.mark.parametrize("gated, dtype", [(False, F32), (True, F32), (False, BF16)])
+@pytest.mark.parametrize("m, n, k", [(1, 24, 1), (8, 40, 96), (40, 130, 261), (96, 256, 4096), (64, 2048, 2048), (1500, 1000, 72)])
+def test_fp32_rows_keep_their_bits(weights, gated, dtype, m, n, k):
+    """under bf16 and MX4 weights an fp32 row is not rounded to 16 bits on its way"""
+    g = gen(m + n + k)
+    x = torch.full((m, k + 3), NAN, device="cuda")[:, 2:k + 2]
+    x.copy_(fp32_rows(g, m, k))
+    w = randn(g, 2, 2 * n if gated else n, k) * k ** -0.5
+    w[:, ::3, 0] = 0
+    if weights == "mx4":
+        w = ops.mx4_quantize(w)
+        wv = ops.mx4_dequantize(w, F32).double()
+    else:
+        w = w.to(weights)
+        wv = w.double()
+    rows = torch.randint(-1, m + 1, (m + 5,), generator=g, device="cuda").int()
+    off = torch.tensor([0, m // 3 + 1, m + 5], dtype=torch.int32, device="cuda")
+    same_as_fp64(x, w, wv, off, rows, randn(g, 2, wv.shape[1]) * 1e-8, gated, dtype)
+
+
+def test_fp32_rows_at_the_end_of_the_range():
+    """values that bf16 would round to an infinity, under weights of 1, and each of them under an infinite weight"""
+    off = torch.tensor([0, 4], dtype=torch.int32, device="cuda")
+    x = torch.tensor([[3.4028235e38], [-3.4e38], [1.1754944e-38], [1 + 2.0 ** -23]], device="cuda")
+    for w in (torch.ones((1, 8, 1), dtype=BF16, device="cuda"), ops.mx4_quantize(torch.ones((1, 8, 1), device="cuda")), torch.ones((1, 8, 1), dtype=F16, device="cuda")):
+        assert torch.equal(ops.expert_linear(x, w, off), x.expand(4, 8))
+    for t in (BF16, F16):
+        got = ops.expert_linear(x, torch.full((1, 8, 1), INF, dtype=t, device="cuda"), off)
+        assert torch.equal(got, torch.tensor([[INF], [-INF], [INF], [INF]], device="cuda").expand(4, 8))
+
+
 def test_fp32_rows_on_fp16_weights_one_by_one():
     """values whose fp16 form is an infinity, coarse or zero"""
     off = torch.tensor([0, 5], dtype=torch.int32, device="cuda")
