@@ -138,6 +138,43 @@ template <int KIND> __device__ __forceinline__ intx4_t mx4_to16(int codes, float
 }
 __device__ __forceinline__ float mx4_scale(int byte) { return __builtin_bit_cast(float, byte << 23); }   // as an operand of the MX4 conversions, which read the exponent field alone (0 = 2^-127)
 
+// fp16 x on MX4 weights: a weight as an fp16 operand of the matrix instruction is taken relative to the largest scale `top` of its row (or run), which becomes 2^13: 6 * 2^13 is below 65504, and the
+// code .5 is exact down to 2^-24, so that scales 2^36 apart are exact together.  The sum is multiplied by lin_top_scale.  Where a row holds a block further below (and not all of it 0) the rows
+// of its fragments are multiplied by lin_exact_blocks.  top >= 14.
+#define LIN_REACH 36
+__device__ __forceinline__ int lin_relative(int byte, int top) { const int d = byte - top + 140; return byte == 255 ? 255 : d > 0 ? d : 0; }
+__device__ __forceinline__ float lin_top_scale(int top) { return mx4_scale(top - 13); }
+__device__ __forceinline__ int lin_top_of(int top, int byte) { return byte != 255 && byte > top ? byte : top; }       // (a NaN block is one under every scale)
+
+// largest and smallest of scale bytes, four at a time (lin_top_of takes three instructions a byte: 4 us of the 49 of 1024 x 4096 x 4096)
+typedef unsigned short ushortx2_t __attribute__((ext_vector_type(2)));
+struct LinSpread {
+    ushortx2_t hi = {0, 0}, lo = {255, 255};
+    __device__ __forceinline__ void look(unsigned v) {
+        const ushortx2_t a = __builtin_bit_cast(ushortx2_t, v & 0x00ff00ffu), b = __builtin_bit_cast(ushortx2_t, v >> 8 & 0x00ff00ffu);
+        hi = __builtin_elementwise_max(hi, __builtin_elementwise_max(a, b)); lo = __builtin_elementwise_min(lo, __builtin_elementwise_min(a, b));
+    }
+    __device__ __forceinline__ int top() const { return hi[0] > hi[1] ? hi[0] : hi[1]; }
+    __device__ __forceinline__ int low() const { return lo[0] < lo[1] ? lo[0] : lo[1]; }
+};
+
+// eight fp16 values as sums of two bf16 ones: eight bits cut off, three left (an infinity, a NaN: once)
+__device__ __forceinline__ void lin_halves(intx4_t v, intx4_t& hi, intx4_t& lo) {
+    const half8_t h = __builtin_bit_cast(half8_t, v);
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        unsigned a[2], b[2];
+#pragma unroll
+        for (int q = 0; q < 2; q++) {
+            const float f = (float)h[2 * i + q];
+            a[q] = __builtin_bit_cast(unsigned, f) >> 16;
+            const float left = __builtin_fabsf(f) < __builtin_inff() ? f - __builtin_bit_cast(float, a[q] << 16) : 0.f;
+            b[q] = __builtin_bit_cast(unsigned, left) >> 16;
+        }
+        hi[i] = (int)(a[0] | a[1] << 16); lo[i] = (int)(b[0] | b[1] << 16);
+    }
+}
+
 // 16 x 16 x 32 product of 16-bit fragments: lane l holds row l & 15, k = 8 (l >> 4) .. + 7 of either operand; result rows (first operand) 4 (l >> 4) + i, column l & 15
 template <int KIND> __device__ __forceinline__ floatx4 lin_mma16(intx4_t a, intx4_t b, floatx4 c) {
     if constexpr (KIND == SM_F16) return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, a), __builtin_bit_cast(half8_t, b), c, 0, 0, 0);
@@ -158,4 +195,24 @@ template <int SEL> __device__ __forceinline__ floatx4 lin_mma4(intx4_t a, int sa
 template <int SEL> __device__ __forceinline__ floatx16 lin_mma4(intx4_t a, int sa, intx4_t b, int sb, floatx16 c) {
     const intx8_t va = __builtin_shufflevector(a, a, 0, 1, 2, 3, -1, -1, -1, -1), vb = __builtin_shufflevector(b, b, 0, 1, 2, 3, -1, -1, -1, -1);
     return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(va, vb, c, 4, 4, SEL, sa, 0, sb);
+}
+
+// fp16 x on MX4 weights with bf16 instructions, straight from memory: any scale is exact there, x becomes two bf16 fragments.  For the rare fragments whose rows hold scales more than 2^36 apart,
+// where it is right and slow (us with such a row in every fragment: 5 rows of 16384 x 8192 140 against 20, 512 of 4096 x 4096 210 / 29, 4001 of 8192 x 4096 3446 / 210); the blocks first .. last - 1 of one fragment of FR weight rows.  w, scales, x[b] = this lane's rows, xk[b] = K, or 0: none;  add(b, w, x): the product.
+template <int FR, int FM, class F>
+__device__ __forceinline__ void lin_exact_blocks(const char* w, const unsigned char* scales, const char* const (&x)[FM], const int (&xk)[FM], int first, int last, F add) {
+    const int g = (threadIdx.x & 63) / FR;
+#pragma unroll 1
+    for (int block = first; block < last; block++)
+#pragma unroll 1
+        for (int h = 0; h < FR / 16; h++) {
+            const int q = h * (64 / FR) + g;                                         // a lane's eight k of the block
+            int code; __builtin_memcpy(&code, w + 16ll * block + 4 * q, 4);
+            const intx4_t wf = mx4_to16<SM_BF16>(code, mx4_scale(scales[block]));
+#pragma unroll
+            for (int b = 0; b < FM; b++) {
+                intx4_t hi, lo; lin_halves(lin_load8(x[b], 32 * block + 8 * q, xk[b]), hi, lo);
+                add(b, wf, hi); add(b, wf, lo);
+            }
+        }
 }

@@ -83,15 +83,38 @@ template <int XK, int WK, int FM, int ST> __global__ __launch_bounds__(256) void
             }
             *(intx4_t*)(scale + j * pitch + 16 * q) = v;
         }
-        if constexpr (XK == SM_F16) {                                               // relative to the row's largest scale of the run: inside fp16's range whatever the scales are
+        if constexpr (XK == SM_F16) {                                               // relative to the row's largest scale of the run; a row that reaches too far is marked by a negative factor
             asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
             const int j = tid >> 1;
             unsigned char* row = scale + j * pitch;
-            int top = 1;
-            for (int b = tid & 1; b < blocks; b += 2) top = top > row[b] ? top : row[b];
-            const int o = __shfl_xor(top, 1); top = top > o ? top : o;
-            for (int b = tid & 1; b < blocks; b += 2) { const int d = row[b] - top + 127; row[b] = row[b] == 255 ? 255 : d > 0 ? d : 0; }
-            if (!(tid & 1)) wmul[j] = mx4_scale(top < 255 ? top : 254);       // (finite also for a row with a NaN: its sums are NaN by themselves, those of slots without a row 0)
+            unsigned* words = (unsigned*)row;                                        // (what lies behind the run's last block are scales too)
+            const int count = (blocks + 3) >> 2;
+            LinSpread all;
+            for (int q = tid & 1; q < count; q += 2) all.look(words[q]);
+            int top = all.top(), low = all.low();
+            int o = __shfl_xor(top, 1); top = top > o ? top : o;
+            o = __shfl_xor(low, 1); low = low < o ? low : o;
+            const bool nan = top == 255;                                             // a NaN block: the largest of the others, its own byte stays
+            if (nan) { top = 0; for (int b = 0; b < blocks; b++) top = lin_top_of(top, row[b]); }
+            if (top < 14) top = 14;
+            int far = 0;
+            if (top - low > LIN_REACH) {
+                const char* codes = wexp + lin_weight_row(p, n0, j) * p.w_ld + 16ll * b0;
+                for (int b = tid & 1; b < blocks; b += 2)
+                    if (lin_relative(row[b], top) < 140 - LIN_REACH) { intx4_t c; __builtin_memcpy(&c, codes + 16ll * b, 16); far |= (c[0] | c[1] | c[2] | c[3]) & 0x77777777; }
+            }
+            __builtin_amdgcn_wave_barrier();                                         // (the two threads of a row have read all of it)
+            const ushortx2_t up = {140, 140}, down = {(unsigned short)top, (unsigned short)top};
+            for (int q = tid & 1; q < count; q += 2) {
+                const unsigned v = words[q];
+                if (nan) { for (int i = 0; i < 4; i++) row[4 * q + i] = lin_relative(v >> (8 * i) & 255, top); }
+                else {
+                    const ushortx2_t a = __builtin_bit_cast(ushortx2_t, v & 0x00ff00ffu) + up, b = __builtin_bit_cast(ushortx2_t, v >> 8 & 0x00ff00ffu) + up;
+                    words[q] = __builtin_bit_cast(unsigned, __builtin_elementwise_sub_sat(a, down)) | __builtin_bit_cast(unsigned, __builtin_elementwise_sub_sat(b, down)) << 8;
+                }
+            }
+            far |= __shfl_xor(far, 1);
+            if (!(tid & 1)) wmul[j] = far ? -1.f : lin_top_scale(top);
         }
     }
 
@@ -175,8 +198,24 @@ template <int XK, int WK, int FM, int ST> __global__ __launch_bounds__(256) void
     };
     if (steps > first) {
         if (ahead == ST) lin_arrive_n<(ST - 1) * QT>(); else lin_arrive_n<0>();
-        read(first, 0, I0(), ragged && steps == first + 1);
         int t = first;
+        if constexpr (DEQ && XK == SM_F16) {
+            if (__any(wmul[lane] < 0.f || wmul[64 + lane] < 0.f)) {                 // (every wave sees the same)
+                lin_arrive_n<0>();
+                if (tid < BN) wmul[tid] = 1.f;
+                const char* xr[FM]; int xk[FM];
+#pragma unroll
+                for (int b = 0; b < FM; b++) { const long long row = lin_slot_row(p, tile, 32 * (wm * FM + b) + r); xr[b] = p.x + (row < 0 ? 0 : row) * p.x_ld; xk[b] = row < 0 ? 0 : p.K; }
+#pragma unroll
+                for (int a = 0; a < FN; a++) {
+                    const long long row = lin_weight_row(p, n0, 32 * (wn * FN + a) + r);
+                    lin_exact_blocks<32, FM>(wexp + row * p.w_ld, p.ws + tile.e * p.ws_es + row * p.ws_ld, xr, xk, b0, b0 + blocks,
+                                             [&](int b, intx4_t w, intx4_t x) { acc[a][b] = lin_mma16<SM_BF16>(w, x, acc[a][b]); });
+                }
+                t = steps;
+            }
+        }
+        if (t < steps) read(first, 0, I0(), ragged && steps == first + 1);
 #pragma unroll 1
         for (; t + 1 + ST < steps; t += 2) { step(t, I0(), std::true_type(), std::true_type()); step(t + 1, I1(), std::true_type(), std::true_type()); }
 #pragma unroll 1

@@ -6,7 +6,8 @@
 // CU's L1 is kept small beside the weights: the scales come as one dword per lane for 16 blocks and are handed to their lanes by a shuffle (byte loads cost 8 of 28 us of a 5-row layer of 16384 x 8192),
 // lanes without a slot load no x, and where there are blocks enough a wave takes four groups of weight rows with the same x.
 // MX4 weights under 16-bit x become 16-bit values in the registers.  bf16: value times scale, exact.  fp16: the range of 2^-24 .. 65504 does not hold every scale, so the values are taken
-// relative to the largest scale of their row in these 512 k and the partial sum is multiplied by it in fp32 (a block 2^23 below that neighbour rounds, by less than the fp32 sum does).
+// relative to the largest scale of their row in these 512 k, exact where the scales are less than 2^36 apart, and the partial sum is multiplied by it in fp32; a wave that met others multiplies its
+// share of K again as bf16 (lin_exact_blocks).
 // fp32 x on fp16 weights (the rows that fp16 parts do not hold, linear.hip): the weights become fp32 values and the products are those of the fp32 matrix instruction, 1/16 of the fp16 rate.
 #pragma once
 #include "linear.hpp"
@@ -94,6 +95,7 @@ template <int XK, int WK, int NB> __global__ __launch_bounds__(512) void lin_str
 #pragma unroll
     for (int b = 0; b < NB; b++) acc[b] = floatx4{0, 0, 0, 0};
 
+    int low = 255;                                                      // fp16 x on MX4: the smallest scale, relative to the largest of its row and chunk
     for (int c = wave * CB; c < nb; c += waves * CB) {
         // the weights of a chunk are asked for at once: a wave's share of K is short, what counts is how much of it is under way
         LinBlk<WK> w[U][NB][BL]; unsigned wsc[NB], xsc = 0;
@@ -142,12 +144,12 @@ template <int XK, int WK, int NB> __global__ __launch_bounds__(512) void lin_str
             for (int b = 0; b < NB; b++) {
                 sum[b] = OWN ? floatx4{0, 0, 0, 0} : acc[b];
                 if constexpr (OWN) {
-                    int t = 1;
+                    int t = 14;
 #pragma unroll
-                    for (int i = 0; i < 4; i++) { const int v = wsc[b] >> (8 * i) & 255; t = t > v ? t : v; }
+                    for (int i = 0; i < 4; i++) t = lin_top_of(t, wsc[b] >> (8 * i) & 255);
                     int o = __shfl_xor(t, 16); t = t > o ? t : o;
                     o = __shfl_xor(t, 32); top[b] = t > o ? t : o;
-                    mul[b] = mx4_scale(top[b]);                         // >= 2^-126
+                    mul[b] = lin_top_scale(top[b]);
                 }
             }
 #pragma unroll
@@ -166,7 +168,7 @@ template <int XK, int WK, int NB> __global__ __launch_bounds__(512) void lin_str
                         float rel = 0.f;
                         if constexpr (MXW) {
                             int byte = sw[b] >> (8 * j) & 255;
-                            if constexpr (OWN) { const int d = byte - top[b] + 127; byte = byte == 255 ? 255 : d > 0 ? d : 0; }
+                            if constexpr (OWN) { byte = lin_relative(byte, top[b]); if (c + u * 4 * BL + g * BL + j < nb) low = low < byte ? low : byte; }
                             rel = mx4_scale(byte);
                         }
 #pragma unroll
@@ -180,6 +182,26 @@ template <int XK, int WK, int NB> __global__ __launch_bounds__(512) void lin_str
             }
 #pragma unroll
             for (int b = 0; b < NB; b++) { if constexpr (OWN) acc[b] += sum[b] * mul[b]; else acc[b] = sum[b]; }
+        }
+    }
+    if constexpr (MXW && XK == SM_F16) if (__any(low < 140 - LIN_REACH)) {   // blocks that fp16 does not hold beside the largest of their chunk: are they all zero?
+        int far = 0;
+        for (int c = wave * CB; c < nb; c += waves * CB)
+#pragma unroll
+            for (int b = 0; b < NB; b++) {
+                int top = 14;
+                for (int i = 0; i < CB && c + i < nb; i++) top = lin_top_of(top, wsr[b][c + i]);
+                for (int i = g; i < CB && c + i < nb; i += 4)
+                    if (lin_relative(wsr[b][c + i], top) < 140 - LIN_REACH) { intx4_t code; __builtin_memcpy(&code, wr[b] + 16ll * (c + i), 16); far |= (code[0] | code[1] | code[2] | code[3]) & 0x77777777; }
+            }
+        if (__any(far)) {
+            const char* const xrow[1] = {xr}; const int xks[1] = {xk};
+#pragma unroll
+            for (int b = 0; b < NB; b++) {
+                acc[b] = floatx4{0, 0, 0, 0};
+                for (int c = wave * CB; c < nb; c += waves * CB)
+                    lin_exact_blocks<16, 1>(wr[b], wsr[b], xrow, xks, c, c + CB < nb ? c + CB : nb, [&](int, intx4_t wf, intx4_t xf) { acc[b] = lin_mma16<SM_BF16>(xf, wf, acc[b]); });
+            }
         }
     }
     // acc[b][i] = slot 4 g + i, weight row r of group b; a slot without a row of x: zero, also under weights that are infinite or NaN

@@ -335,20 +335,24 @@ __global__ __launch_bounds__(64 * WN * WM) void lin_tile_kernel(LinearParams p) 
             const long long row = weight_row(j);
             csrc[i] = wexp + row * p.w_ld; ssrc[i] = p.ws + tile.e * p.ws_es + row * p.ws_ld;
             stop[i] = 127;
-            if constexpr (XK == SM_F16) {                                           // values relative to the row's largest scale: inside fp16's range whatever the scales are
-                int top = 1;
-                auto up = [&](unsigned v) {
-#pragma unroll
-                    for (int k = 0; k < 32; k += 8) { const int s = v >> k & 255; top = top > s ? top : s; }
-                };
+            if constexpr (XK == SM_F16) {                                           // relative to the row's largest scale; a row that reaches too far is marked by a negative factor
+                LinSpread all;
                 for (int b = 16 * (tid & 1); b < nb && nb >= 16; b += 32) {
                     intx4_t v; __builtin_memcpy(&v, ssrc[i] + (b < nb - 16 ? b : nb - 16), 16);
-                    up(v[0]); up(v[1]); up(v[2]); up(v[3]);
+                    all.look(v[0]); all.look(v[1]); all.look(v[2]); all.look(v[3]);
                 }
-                for (int b = 0; b < nb && nb < 16; b++) up(ssrc[i][b]);
+                for (int b = 0; b < nb && nb < 16; b++) all.look(ssrc[i][b] * 0x01010101u);
+                int top = all.top(); const int low = all.low();
                 const int o = __shfl_xor(top, 1); top = top > o ? top : o;
+                if (top == 255) { top = 0; for (int b = 0; b < nb; b++) top = lin_top_of(top, ssrc[i][b]); }   // a NaN block: the largest of the others
+                if (top < 14) top = 14;
+                int far = 0;
+                if (top - low > LIN_REACH)
+                    for (int b = 0; b < nb; b++)
+                        if (lin_relative(ssrc[i][b], top) < 140 - LIN_REACH) { intx4_t c; __builtin_memcpy(&c, csrc[i] + 16ll * b, 16); far |= (c[0] | c[1] | c[2] | c[3]) & 0x77777777; }
+                far |= __shfl_xor(far, 1);                                          // (each of the two threads has seen half of the scales)
                 stop[i] = top;
-                if (!(tid & 1)) wmul[j] = mx4_scale(top < 255 ? top : 254);       // (finite also for a row with a NaN: its sums are NaN by themselves, those of slots without a row 0)
+                if (!(tid & 1)) wmul[j] = far ? -1.f : lin_top_scale(top);
             }
         }
     }
@@ -414,7 +418,7 @@ __global__ __launch_bounds__(64 * WN * WM) void lin_tile_kernel(LinearParams p) 
             for (int i = 0; i < DB; i++) {
                 const int j = i * (THREADS / 2) + (tid >> 1);
                 int byte = sbyte[i];
-                if constexpr (XK == SM_F16) { const int d = byte - stop[i] + 127; byte = byte == 255 ? 255 : d > 0 ? d : 0; }
+                if constexpr (XK == SM_F16) byte = lin_relative(byte, stop[i]);
                 const float s = mx4_scale(byte);
 #pragma unroll
                 for (int q = 0; q < 4; q++) *(intx4_t*)(st + j * 128 + ((((tid & 1) * 4 + q) ^ (j & 7) ^ swz(j)) << 4)) = mx4_to16<XK>(code[i][q], s);
@@ -503,6 +507,7 @@ __global__ __launch_bounds__(64 * WN * WM) void lin_tile_kernel(LinearParams p) 
     };
     typedef std::integral_constant<int, 0> First; typedef std::integral_constant<int, PH - 1> Last;
     const bool ragged = DMA && (x_bytes & 127) && steps == every;
+    int t = first;
     if (steps > first) {
         if constexpr (DMA) {
 #pragma unroll
@@ -518,7 +523,26 @@ __global__ __launch_bounds__(64 * WN * WM) void lin_tile_kernel(LinearParams p) 
         }
         if (steps > first + 2) load_staged(first + 2, std::false_type());
         lin_arrive();
-        read(first, First(), ragged && steps == first + 1);
+        if constexpr (DEQ && XK == SM_F16) {
+            float least = 0.f;
+#pragma unroll
+            for (int j = 0; j < BN; j += 64) { const float m = wmul[j + lane]; least = m < least ? m : least; }
+            if (__any(least < 0.f)) {                                               // (every wave sees the same)
+                lin_arrive();
+                if (tid < BN) wmul[tid] = 1.f;
+                const char* xr[FM]; int xk[FM];
+#pragma unroll
+                for (int b = 0; b < FM; b++) { const long long row = slot_row(FR * (wm * FM + b) + r); xr[b] = p.x + (row < 0 ? 0 : row) * p.x_ld; xk[b] = row < 0 ? 0 : p.K; }
+#pragma unroll
+                for (int a = 0; a < FN; a++) {
+                    const long long row = weight_row(FR * (wn * FN + a) + r);
+                    lin_exact_blocks<FR, FM>(wexp + row * p.w_ld, p.ws + tile.e * p.ws_es + row * p.ws_ld, xr, xk, 2 * first, 2 * steps < nb ? 2 * steps : nb,
+                                             [&](int b, intx4_t w, intx4_t x) { acc[a][b] = lin_mma16<SM_BF16>(w, x, acc[a][b]); });
+                }
+                t = steps;
+            }
+        }
+        if (t < steps) read(first, First(), ragged && steps == first + 1);
     }
     auto step = [&](int t, auto has1, auto has2, auto end2) {                       // has1, has2: steps t + 1, t + 2 exist; end2: t + 2 may be the last
         constexpr bool MORE = decltype(has1)::value, MORE2 = decltype(has2)::value;
@@ -546,7 +570,6 @@ __global__ __launch_bounds__(64 * WN * WM) void lin_tile_kernel(LinearParams p) 
         });
         __builtin_amdgcn_sched_barrier(0);
     };
-    int t = first;
     if constexpr (DMA && !DEQ && !MX) {
         // a wave whose slots lie behind the tile's last one (the end of a group) only fills; the four SIMDs hold waves of all parts, so that the others run faster
         if (wm * FM * FR >= tile.rows) {

@@ -153,3 +153,97 @@ def test_fp32_rows_on_fp16_weights_in_a_graph():
         gr.replay()
         assert torch.equal(y, ops.expert_linear(x, w, off)), turn
         torch.cuda.synchronize()
+
+
+# ---- MX4 weights whose scales lie far apart ----------------------------------------------------------------------------------------------------
+
+KINDS = [F16, BF16, "mx4"]
+WAYS = [(1, 40, 96), (6, 1000, 1500), (16, 200, 2088), (90, 256, 512), (90, 256, 4096), (90, 300, 264), (90, 300, 261), (300, 1000, 333), (1500, 2048, 512), (2304, 4096, 256), (2304, 4096, 251)]
+
+
+def wide_weights(g, n, k):
+    """rows of blocks up to 2^80 apart; ordinary rows; rows with one huge value in a block that is zero otherwise, with blocks of zeros, with a block just inside and just outside fp16's reach"""
+    nb = -(-k // 32)
+    blocks = lambda v: v.repeat_interleave(32, -1)[:, :k]  # noqa: E731
+    w = randn(g, n, k)
+    kind = torch.arange(n, device="cuda") % 6
+    far = torch.exp2(torch.randint(-40, 41, (n, nb), generator=g, device="cuda").float())
+    w = torch.where((kind == 0)[:, None], w * blocks(far), w)
+    w = torch.where((kind == 2)[:, None] & blocks(torch.rand((n, nb), generator=g, device="cuda") < 0.3), torch.zeros_like(w), w)
+    edge = torch.exp2(-torch.randint(33, 41, (n, nb), generator=g, device="cuda").float())
+    w = torch.where((kind == 3)[:, None], w * blocks(edge), w)
+    huge = (kind == 1) | (kind == 3)
+    w[:, :32] = torch.where(huge[:, None], torch.zeros_like(w[:, :32]), w[:, :32])
+    w[:, 0] = torch.where(huge, torch.where(kind == 1, 2.0 ** 60, 1.0), w[:, 0])
+    return w
+
+
+def rows_of(kind, x):
+    """(x as handed over, its values in 64 bits, type of the output)"""
+    if kind == "mx4":
+        q = ops.mx4_quantize(x)
+        return q, ops.mx4_dequantize(q, F32).double(), F16
+    return x.to(kind), x.to(kind).double(), kind
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("loud", [False, True])
+@pytest.mark.parametrize("m, n, k", WAYS)
+def test_scales_far_apart(kind, loud, m, n, k):
+    """a block of weights counts for what it is, however large the others of its row are: every other row of x is zero where they are"""
+    g = gen(m + n + k)
+    w = ops.mx4_quantize(wide_weights(g, n, k))
+    wv = ops.mx4_dequantize(w, F32).double()
+    x = randn(g, m, k) * (3e4 if loud else 1.0) / (4 if loud else 1)
+    x[::2, 0] = 0
+    if loud:
+        x[1::4, 32:] = 0
+    x, xv, dt = rows_of(kind, x)
+    z, mag = xv @ wv.t(), xv.abs() @ wv.abs().t()
+    inside(ops.mx4_linear(x, w, dtype=F32), z, chain(2 * k) * mag + 2.0 ** -126)
+    rows = torch.randint(-1, m + 1, (m + 5,), generator=g, device="cuda").int()
+    off = torch.tensor([0, m // 3 + 1, m + 5], dtype=torch.int32, device="cuda")
+    both = ops.Mx4(torch.stack((w.codes, w.codes.flip(0))), torch.stack((w.scales, w.scales.flip(0))), k)
+    ok = ((rows >= 0) & (rows < m))[:, None]
+    got = ops.expert_linear(x, both, off, rows, dtype=F32)
+    for e in range(2):
+        s = slice(int(off[e]), int(off[e + 1]))
+        zero, at = torch.zeros((), dtype=F64, device="cuda"), rows[s].clamp(0, m - 1).long()
+        want, lim = torch.where(ok[s], z[at], zero), torch.where(ok[s], mag[at], zero)
+        if e:
+            want, lim = want.flip(1), lim.flip(1)
+        inside(got[s], want, chain(2 * k) * lim + 2.0 ** -126, "group %d" % e)
+
+
+@pytest.mark.parametrize("m", [1, 16, 17, 90, 1500])
+def test_one_far_block(m):
+    """two blocks, 2^30 apart and further, x zero in the larger one"""
+    for apart in (0, 22, 24, 30, 36, 37, 60, 126):
+        scales = torch.tensor([[127, 127 - apart]], dtype=torch.uint8, device="cuda").repeat(24, 1)
+        w = ops.Mx4(torch.full((24, 32), 0x22, dtype=torch.uint8, device="cuda"), scales, 64)        # every code 1
+        x = torch.zeros((m, 64), dtype=F16, device="cuda")
+        x[:, 40] = 30000
+        got = ops.mx4_linear(x, w, dtype=F32)
+        assert got.eq(30000 * 2.0 ** -apart).all(), apart
+        x[:, 41] = INF
+        assert ops.mx4_linear(x, w, dtype=F32).eq(INF).all(), apart
+
+
+@pytest.mark.parametrize("m", [5, 90])
+def test_scales_that_change_between_replays(m):
+    """which weights are multiplied in another way is decided on the device"""
+    g = gen(2)
+    fine, far = ops.mx4_quantize(randn(g, 200, 1024)), ops.mx4_quantize(wide_weights(g, 200, 1024))
+    w = ops.Mx4(fine.codes.clone(), fine.scales.clone(), 1024)
+    x = randn(g, m, 1024).to(F16)
+    ops.mx4_linear(x, w)
+    torch.cuda.synchronize()
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):
+        y = ops.mx4_linear(x, w, dtype=F32)
+    for turn in range(4):
+        now = far if turn % 2 else fine
+        w.codes.copy_(now.codes), w.scales.copy_(now.scales)
+        gr.replay()
+        assert torch.equal(y, ops.mx4_linear(x, now, dtype=F32)), turn
+        torch.cuda.synchronize()
