@@ -198,21 +198,30 @@ template <int SEL> __device__ __forceinline__ floatx16 lin_mma4(intx4_t a, int s
 }
 
 // fp16 x on MX4 weights with bf16 instructions, straight from memory: any scale is exact there, x becomes two bf16 fragments.  For the rare fragments whose rows hold scales more than 2^36 apart,
-// where it is right and slow (us with such a row in every fragment: 5 rows of 16384 x 8192 140 against 20, 512 of 4096 x 4096 210 / 29, 4001 of 8192 x 4096 3446 / 210); the blocks first .. last - 1 of one fragment of FR weight rows.  w, scales, x[b] = this lane's rows, xk[b] = K, or 0: none;  add(b, w, x): the product.
-template <int FR, int FM, class F>
-__device__ __forceinline__ void lin_exact_blocks(const char* w, const unsigned char* scales, const char* const (&x)[FM], const int (&xk)[FM], int first, int last, F add) {
+// where it is right and slow (us with such a row in every fragment: 5 rows of 16384 x 8192 140 against 20, 512 of 4096 x 4096 210 / 29, 4001 of 8192 x 4096 3446 / 210); the blocks first .. last - 1 of one fragment of FR weight rows.  w, scales, x[b] = this lane's rows, xk[b] = K, or 0: none;  add(b, w, x): the product,
+// raise(): the sums so far times 2^128.  Blocks at the upper end of the range come first, 2^128 smaller, so that no weight is an infinity in bf16 (a second part that is 0 times it: a NaN).
+template <int FR, int FM, class F, class R>
+__device__ __forceinline__ void lin_exact_blocks(const char* w, const unsigned char* scales, const char* const (&x)[FM], const int (&xk)[FM], int first, int last, F add, R raise) {
     const int g = (threadIdx.x & 63) / FR;
+    auto high = [](int byte) { return byte >= 200 && byte != 255; };
+    bool upper = false;
+    for (int block = first; block < last; block++) upper |= high(scales[block]);
 #pragma unroll 1
-    for (int block = first; block < last; block++)
+    for (int pass = __any(upper) ? 0 : 1; pass < 2; pass++) {
 #pragma unroll 1
-        for (int h = 0; h < FR / 16; h++) {
-            const int q = h * (64 / FR) + g;                                         // a lane's eight k of the block
-            int code; __builtin_memcpy(&code, w + 16ll * block + 4 * q, 4);
-            const intx4_t wf = mx4_to16<SM_BF16>(code, mx4_scale(scales[block]));
+        for (int block = first; block < last; block++)
+#pragma unroll 1
+            for (int h = 0; h < FR / 16; h++) {
+                const int q = h * (64 / FR) + g, byte = scales[block];               // a lane's eight k of the block
+                const bool now = high(byte) == (pass == 0);
+                int code; __builtin_memcpy(&code, w + 16ll * block + 4 * q, 4);
+                const intx4_t wf = mx4_to16<SM_BF16>(now ? code : 0, mx4_scale(now ? byte - (pass == 0 ? 128 : 0) : 127));
 #pragma unroll
-            for (int b = 0; b < FM; b++) {
-                intx4_t hi, lo; lin_halves(lin_load8(x[b], 32 * block + 8 * q, xk[b]), hi, lo);
-                add(b, wf, hi); add(b, wf, lo);
+                for (int b = 0; b < FM; b++) {
+                    intx4_t hi, lo; lin_halves(lin_load8(x[b], 32 * block + 8 * q, xk[b]), hi, lo);
+                    add(b, wf, hi); add(b, wf, lo);
+                }
             }
-        }
+        if (pass == 0) raise();
+    }
 }

@@ -210,7 +210,11 @@ template <int XK, int WK, int FM, int ST> __global__ __launch_bounds__(256) void
                 for (int a = 0; a < FN; a++) {
                     const long long row = lin_weight_row(p, n0, 32 * (wn * FN + a) + r);
                     lin_exact_blocks<32, FM>(wexp + row * p.w_ld, p.ws + tile.e * p.ws_es + row * p.ws_ld, xr, xk, b0, b0 + blocks,
-                                             [&](int b, intx4_t w, intx4_t x) { acc[a][b] = lin_mma16<SM_BF16>(w, x, acc[a][b]); });
+                                             [&](int b, intx4_t w, intx4_t x) { acc[a][b] = lin_mma16<SM_BF16>(w, x, acc[a][b]); },
+                                             [&] {
+#pragma unroll
+                                                 for (int b = 0; b < FM; b++) acc[a][b] = acc[a][b] * 0x1p64f * 0x1p64f;
+                                             });
                 }
                 t = steps;
             }

@@ -198,9 +198,14 @@ template <int XK, int WK, int NB> __global__ __launch_bounds__(512) void lin_str
             const char* const xrow[1] = {xr}; const int xks[1] = {xk};
 #pragma unroll
             for (int b = 0; b < NB; b++) {
-                acc[b] = floatx4{0, 0, 0, 0};
-                for (int c = wave * CB; c < nb; c += waves * CB)
-                    lin_exact_blocks<16, 1>(wr[b], wsr[b], xrow, xks, c, c + CB < nb ? c + CB : nb, [&](int, intx4_t wf, intx4_t xf) { acc[b] = lin_mma16<SM_BF16>(xf, wf, acc[b]); });
+                floatx4 sum = {0, 0, 0, 0};
+                for (int c = wave * CB; c < nb; c += waves * CB) {
+                    floatx4 own = {0, 0, 0, 0};                         // (of these blocks: raised by itself)
+                    lin_exact_blocks<16, 1>(wr[b], wsr[b], xrow, xks, c, c + CB < nb ? c + CB : nb, [&](int, intx4_t wf, intx4_t xf) { own = lin_mma16<SM_BF16>(xf, wf, own); },
+                                            [&] { own = own * 0x1p64f * 0x1p64f; });
+                    sum += own;
+                }
+                acc[b] = sum;
             }
         }
     }

@@ -537,7 +537,11 @@ __global__ __launch_bounds__(64 * WN * WM) void lin_tile_kernel(LinearParams p) 
                 for (int a = 0; a < FN; a++) {
                     const long long row = weight_row(FR * (wn * FN + a) + r);
                     lin_exact_blocks<FR, FM>(wexp + row * p.w_ld, p.ws + tile.e * p.ws_es + row * p.ws_ld, xr, xk, 2 * first, 2 * steps < nb ? 2 * steps : nb,
-                                             [&](int b, intx4_t w, intx4_t x) { acc[a][b] = lin_mma16<SM_BF16>(w, x, acc[a][b]); });
+                                             [&](int b, intx4_t w, intx4_t x) { acc[a][b] = lin_mma16<SM_BF16>(w, x, acc[a][b]); },
+                                             [&] {
+#pragma unroll
+                                                 for (int b = 0; b < FM; b++) acc[a][b] = acc[a][b] * 0x1p64f * 0x1p64f;
+                                             });
                 }
                 t = steps;
             }

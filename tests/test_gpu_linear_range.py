@@ -178,6 +178,13 @@ def wide_weights(g, n, k):
     return w
 
 
+def mx4ref_values(q):
+    """the values of an MX4 tensor in 64 bits (fp32 does not hold the largest)"""
+    low = q.scales.clamp(max=200)
+    up = torch.exp2((q.scales - low).double()).repeat_interleave(32, -1)[..., :q.k]
+    return ops.mx4_dequantize(ops.Mx4(q.codes, low, q.k), F32).double() * up
+
+
 def rows_of(kind, x):
     """(x as handed over, its values in 64 bits, type of the output)"""
     if kind == "mx4":
@@ -227,6 +234,25 @@ def test_one_far_block(m):
         assert got.eq(30000 * 2.0 ** -apart).all(), apart
         x[:, 41] = INF
         assert ops.mx4_linear(x, w, dtype=F32).eq(INF).all(), apart
+
+
+@pytest.mark.parametrize("m, n, k", [(1, 40, 96), (17, 40, 96), (90, 256, 4128), (300, 1000, 64), (1500, 2048, 288), (2304, 4096, 288), (2304, 4096, 261)])
+def test_both_ends_of_the_scales(m, n, k):
+    """blocks of the largest scales beside the smallest ones, x zero where they are or not: as in 64 bits (an infinity behind fp32's range)"""
+    g = gen(k)
+    q = ops.mx4_quantize(randn(g, n, k))
+    q.scales[1::2] = torch.randint(200, 255, q.scales[1::2].shape, generator=g, device="cuda").byte()
+    q.scales[1::2, ::2] = torch.randint(0, 60, q.scales[1::2, ::2].shape, generator=g, device="cuda").byte()
+    x = (randn(g, m, k) * 2.0 ** -12).to(F16)
+    cols = torch.arange(k, device="cuda") // 32 % 2 == 1
+    x[::3, cols] = 0
+    x[1::3, ~cols] = 0
+    w = mx4ref_values(q)
+    z, mag = x.double() @ w.t(), x.double().abs() @ w.abs().t()
+    got = ops.mx4_linear(x, q, dtype=F32)
+    big = z.abs() > 3.3e38
+    assert (got.isinf() == (z.abs() > 3.4028235e38))[~big | (z.abs() > 3.5e38)].all() and not got.isnan().any()
+    inside(torch.where(big, 0, got), torch.where(big, 0, z), chain(2 * k) * torch.where(mag > 3.3e38, 1e300, mag) + 2.0 ** -126)
 
 
 @pytest.mark.parametrize("m", [5, 90])
