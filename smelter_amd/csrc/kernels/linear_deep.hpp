@@ -139,6 +139,7 @@ template <int XK, int WK, int FM, int ST> __global__ __launch_bounds__(256) void
             for (int a = 0; a < FN; a++) {
                 wf[B][a][0] = *(const intx4_t*)(st + (wn * FN + a) * 32 * S::WB + g * 16);
                 wsc[B][a] = scale[((wn * FN + a) * 32 + r) * pitch + (q < blocks ? q : blocks - 1)];
+                if (masked && q >= blocks) wsc[B][a] = 0;                           // (behind the end: finite, under zeros of x)
             }
         }
 #pragma unroll

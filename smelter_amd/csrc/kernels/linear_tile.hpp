@@ -386,7 +386,7 @@ __global__ __launch_bounds__(64 * WN * WM) void lin_tile_kernel(LinearParams p) 
 #pragma unroll
             for (int i = 0; i < DB; i++) {
                 const int b = 2 * t + (tid & 1), at = b < nb ? b : nb - 1;
-                code[i] = *(const intx4_t*)(csrc[i] + 16ll * at); sbyte[i] = ssrc[i][at];
+                code[i] = *(const intx4_t*)(csrc[i] + 16ll * at); sbyte[i] = b < nb ? ssrc[i][at] : 0;   // (behind the end: finite, under zeros of x)
             }
         }
         if constexpr (!DMA) {

@@ -255,6 +255,23 @@ def test_both_ends_of_the_scales(m, n, k):
     inside(torch.where(big, 0, got), torch.where(big, 0, z), chain(2 * k) * torch.where(mag > 3.3e38, 1e300, mag) + 2.0 ** -126)
 
 
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("m, n, k", [(1, 40, 96), (17, 40, 96), (90, 256, 4128), (300, 1000, 32), (1500, 2048, 288), (2304, 4096, 288), (2304, 4096, 260)])
+def test_largest_scales_in_the_last_block(kind, m, n, k):
+    """weights behind fp32's range in the last block of an odd number of blocks: infinities, not NaN"""
+    q = ops.mx4_quantize(randn(gen(k), n, k))
+    q.scales[1, -1], q.scales[2, -1] = 254, 254
+    last = slice(-16, (k - 1) % 32 // 2 - 15 or None)                    # (columns behind the end hold code 0)
+    q.codes[1, last], q.codes[2, last] = 0x77, 0xff
+    x, xv, _ = rows_of(kind, torch.ones((m, k), device="cuda"))
+    got = ops.mx4_linear(x, q, dtype=F32)
+    assert got[:, 1].eq(INF).all() and got[:, 2].eq(-INF).all()
+    got[:, 1:3] = 0
+    wv = ops.mx4_dequantize(q, F32).double()
+    wv[1:3] = 0
+    inside(got, xv @ wv.t(), chain(2 * k) * (xv.abs() @ wv.abs().t()))
+
+
 @pytest.mark.parametrize("m", [5, 90])
 def test_scales_that_change_between_replays(m):
     """which weights are multiplied in another way is decided on the device"""
