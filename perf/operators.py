@@ -269,9 +269,8 @@ def _own(s):
     if s["op"] == "combine":
         return ops.moe_combine(s["data"], s["plan"]["slots"], s["part"])
     r = ops.moe_route(s["score"], s["top"])
-    # between the products three bits more than the answer has (fp16 for bf16 under 4-bit weights), otherwise fp32: rounded like the answer, the hidden values would double what it is off by
-    h = ops.expert_linear(s["data"], _own_weight(ops, s["hidden"], s["k"]), r.offsets, rows=r.rows, gated=True,
-                          dtype=torch.float16 if s["x"] == BF16 and len(s["answer"]) == 2 else torch.float32)
+    # fp32 between the products: rounded like the answer, the hidden values would double what it is off by, and a product of two unbounded values fits no 16-bit type with more bits than bf16
+    h = ops.expert_linear(s["data"], _own_weight(ops, s["hidden"], s["k"]), r.offsets, rows=r.rows, gated=True, dtype=torch.float32)
     y = ops.expert_linear(h, _own_weight(ops, s["answer"], s["f"]), r.offsets, dtype=torch.float32)
     return ops.moe_combine(y, r.slots, r.weights, dtype=s["data"].dtype)
 
