@@ -366,8 +366,8 @@ int sm_mx4_dequantize(const void* codes, const void* scales, int64_t rows, int32
 typedef struct sm_linear_desc {
     int64_t M, T;                   /* slots (rows of y); rows of x */
     int32_t N, K, E;                /* columns of y, inner size, groups (1 = an ordinary layer) */
-    int32_t x_type, w_type, y_type; /* fp16 | bf16 x on weights of the same type or MX4, y of x's type, fp16 (three bits more for what a
-                                     next layer with MX4 weights takes) or fp32; MX4 x on MX4 weights, any y;
+    int32_t x_type, w_type, y_type; /* fp16 | bf16 x on weights of the same type or MX4, y of x's type, fp16 (three bits more than bf16 between
+                                     2^-14 and 65504, fewer below, infinities above) or fp32; MX4 x on MX4 weights, any y;
                                      fp32 x on 16-bit or MX4 weights, any y: every row keeps its 24 bits (three parts of bf16; of fp16 under fp16 weights, with
                                      a power of two of the row's own; rows that reach further than 2^38 are multiplied in fp32) */
     int32_t act; float slope;       /* SM_ACT_* behind the bias (not with gated) */

@@ -720,8 +720,8 @@ def _linear(name, index, x, w, lead, offsets, rows, bias, act, slope, gated, out
 
 def mx4_linear(x, w, bias=None, act=ACT_NONE, slope=0.0, gated=False, out=None, dtype=None):
     """act(x . w^T + bias) with MX4 weights w [N, K] (sm_linear_fwd).  x [M, K]: fp16 or bf16 (the weights are read as 16-bit values, the output has x's type, fp16 or fp32), or an Mx4 tensor
-    (both sides in 4 bits; dtype fp16 (default), bf16 or fp32).  What a bf16 layer hands to a next one with MX4 weights keeps three bits more as fp16 (beyond 65504: infinities).  fp32 x: with all its
-    24 bits (three parts, on three times the rows), any dtype (fp32 by default).  gated: w has 2 N rows and the result is silu(first N columns) * last N.  bias fp32 [rows of w]."""
+    (both sides in 4 bits; dtype fp16 (default), bf16 or fp32).  fp32 x: with all its 24 bits (three parts, on three times the
+    rows), any dtype (fp32 by default): what one layer hands to the next.  fp16 out of bf16 rows is faster for the next one and ends at 65504 (then: infinities) and 2^-14 (then: fewer bits).  gated: w has 2 N rows and the result is silu(first N columns) * last N.  bias fp32 [rows of w]."""
     if not isinstance(w, Mx4):
         _refuse("mx4_linear: the weights must be an Mx4 tensor")
     return _linear("mx4_linear", None, x, w, 0, None, None, bias, act, slope, gated, out, dtype)

@@ -290,3 +290,45 @@ def test_scales_that_change_between_replays(m):
         gr.replay()
         assert torch.equal(y, ops.mx4_linear(x, now, dtype=F32)), turn
         torch.cuda.synchronize()
+
+
+# ---- a layer whose hidden values fit no 16-bit type ----------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16", "f16-mx4", "bf16-mx4"])
+@pytest.mark.parametrize("tokens", [1, 48, 500])
+@pytest.mark.parametrize("size", [2.0 ** 6, 2.0 ** -8])
+def test_layer_hands_fp32_over(kind, tokens, size):
+    """gated hidden values beyond 65504 in some rows (size 2^6: silu(gate) * up of about 2^6 * 2^6 * 2^6) and below 2^-17 in others, handed over in fp32: only the answer's own rounding is left"""
+    g = gen(tokens)
+    e, k, f, top = 6, 128, 96, 2
+    dt = BF16 if kind.startswith("bf16") else F16
+    x = (randn(g, tokens, k) * size).to(dt)
+    hidden, answer = randn(g, e, 2 * f, k) * k ** -0.5, randn(g, e, k, f) * f ** -0.5
+    hidden[:, f:] *= size
+    answer *= size ** -3 if size > 1 else 1
+    if kind.endswith("mx4"):
+        hidden, answer = ops.mx4_quantize(hidden), ops.mx4_quantize(answer)
+        hv, av = ops.mx4_dequantize(hidden, F32).double(), ops.mx4_dequantize(answer, F32).double()
+    else:
+        hidden, answer = hidden.to(dt), answer.to(dt)
+        hv, av = hidden.double(), answer.double()
+    scores = randn(g, tokens, e)
+    plan = ops.moe_route(scores, top)
+    h = ops.expert_linear(x, hidden, plan.offsets, plan.rows, gated=True, dtype=F32)
+    got = ops.moe_combine(ops.expert_linear(h, answer, plan.offsets, dtype=F32), plan.slots, plan.weights, dtype=dt)
+    want, err = torch.zeros((2, tokens, k), dtype=F64, device="cuda")
+    reach = 0.0
+    for i in range(e):
+        tok, j = (plan.experts == i).nonzero(as_tuple=True)
+        v = x[tok].double()
+        hh, he = gate(v @ hv[i].t(), chain(k) * (v.abs() @ hv[i].abs().t()) + 2.0 ** -126, f)
+        he = he + 2.0 ** -24 * hh.abs()
+        y, ye = hh @ av[i].t(), chain(3 * f) * ((hh.abs() + he) @ av[i].abs().t()) + he @ av[i].abs().t() + 2.0 ** -126
+        part = plan.weights[tok, j].double()[:, None]
+        want.index_add_(0, tok, part * y)
+        err.index_add_(0, tok, part * (ye + 2.0 ** -21 * (y.abs() + ye)))
+        reach = max(reach, hh.abs().max().item() if len(tok) else 0.0)
+    if tokens > 1:
+        assert reach > 65504 if size > 1 else reach < 2.0 ** -10
+    inside(got, want, err)
