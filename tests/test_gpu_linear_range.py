@@ -222,6 +222,26 @@ def test_scales_far_apart(kind, loud, m, n, k):
         inside(got[s], want, chain(2 * k) * lim + 2.0 ** -126, "group %d" % e)
 
 
+@pytest.mark.parametrize("kind", [F16, BF16])
+@pytest.mark.parametrize("m, n, k", WAYS)
+def test_16_bit_weights_of_mixed_magnitudes(kind, m, n, k):
+    """a product's limit is its own sum of magnitudes, not the largest weight of its row"""
+    g = gen(m + n + k)
+    w = randn(g, 2, n, k) * torch.exp2(torch.randint(-14, 9, (2, n, k), generator=g, device="cuda").float())
+    w[:, ::3, :32] = 0
+    w[:, 1::3, 0] = 6e4
+    w = w.to(kind)
+    x = randn(g, m, k) * torch.exp2(torch.randint(-14, 9, (m, k), generator=g, device="cuda").float())
+    x[::2, 0] = 0
+    x = x.to(kind)
+    off = torch.tensor([0, m // 3 + 1, m], dtype=torch.int32, device="cuda")
+    got = ops.expert_linear(x, w, off, dtype=F32)
+    for e in range(2):
+        s = slice(int(off[e]), int(off[e + 1]))
+        xv, wv = x[s].double(), w[e].double()
+        inside(got[s], xv @ wv.t(), chain(k) * (xv.abs() @ wv.abs().t()) + 2.0 ** -126, "group %d" % e)
+
+
 @pytest.mark.parametrize("m", [1, 16, 17, 90, 1500])
 def test_one_far_block(m):
     """two blocks, 2^30 apart and further, x zero in the larger one"""
