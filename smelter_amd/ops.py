@@ -613,6 +613,13 @@ def _gpu(index, name, t, dtypes):
     return at
 
 
+def _int32(name, *sizes):
+    """sizes that the C interface takes as 32-bit integers: ctypes would cut larger ones without a word"""
+    for n in sizes:
+        if n > 0x7fffffff:
+            _refuse("%s: %d columns exceed 32 bits", name, n)
+
+
 _U8, _BYTES, _INTS, _HALVES, _FLOATS = torch.uint8, (torch.uint8,), (torch.int32,), (torch.float16, torch.bfloat16), (torch.float32,)
 
 
@@ -636,6 +643,7 @@ def mx4_quantize(x):
     A block with a NaN or an infinity becomes NaN."""
     index = _gpu(None, "mx4_quantize", x, _TYPES)
     rows, k, ld = _rows2d(x, "mx4_quantize")
+    _int32("mx4_quantize", k)
     nb, lead = (k + 31) // 32, x.shape[:-1]
     codes, scales = x.new_empty((*lead, 16 * nb), dtype=torch.uint8), x.new_empty((*lead, nb), dtype=torch.uint8)
     _on(index, lib().sm_mx4_quantize, x.data_ptr(), _TYPES[x.dtype], rows, k, ld, codes.data_ptr(), scales.data_ptr())
@@ -654,6 +662,7 @@ def mx4_dequantize(q, dtype=torch.float16, out=None):
         if tuple(out.shape) != q.shape:
             _refuse("mx4_dequantize: output %s for %s", tuple(out.shape), q.shape)
     rows, k, ld = _rows2d(out, "mx4_dequantize")
+    _int32("mx4_dequantize", k)
     _on(index, lib().sm_mx4_dequantize, q.codes.data_ptr(), q.scales.data_ptr(), rows, k, out.data_ptr(), _TYPES[out.dtype], ld)
     return out
 
@@ -687,6 +696,8 @@ def _linear(name, index, x, w, lead, offsets, rows, bias, act, slope, gated, out
     if len(wsh) != lead + 2 or wk != xk:
         _refuse("%s: weights %s for x with %d columns", name, tuple(w.shape), xk)
     t, n, e = xt.shape[0], wsh[-2], wsh[0] if lead else 1
+    if xk > 0x7fffffff or n > 0x7fffffff or e > 0x7fffffff:
+        _int32(name, xk, n, e)
     m = t if rows is None else rows.shape[0]
     if bias is not None:
         _gpu(index, name, bias, _FLOATS)
@@ -773,6 +784,7 @@ def moe_combine(y, slots, weights, out=None, dtype=None):
         _refuse("moe_combine: y %s, slots %s, weights %s", tuple(y.shape), tuple(slots.shape), tuple(weights.shape))
     m, n = y.shape
     t, k = slots.shape
+    _int32("moe_combine", n, k)
     if out is None:
         if dtype is not None and dtype not in _TYPES:
             _refuse("moe_combine: type %s is not taken", dtype)

@@ -3,6 +3,7 @@ Every limit here is relative to the sum of the products' own magnitudes: nothing
 import pytest
 import torch
 
+from smelter_amd import _native as N
 from smelter_amd import ops
 
 pytestmark = pytest.mark.gpu
@@ -352,3 +353,19 @@ def test_layer_hands_fp32_over(kind, tokens, size):
     if tokens > 1:
         assert reach > 65504 if size > 1 else reach < 2.0 ** -10
     inside(got, want, err)
+
+
+# ---- sizes that the C interface does not hold ----------------------------------------------------------------------------------------------------
+
+
+def test_columns_behind_32_bits_are_refused():
+    """not cut to their low 32 bits"""
+    k = (1 << 32) + 32
+    x = torch.empty((1, k), dtype=F16, device="cuda")
+    w = torch.empty((1, k // 2), dtype=torch.uint8, device="cuda")
+    q = ops.Mx4(w, torch.empty((1, k // 32), dtype=torch.uint8, device="cuda"), k)
+    one = torch.zeros((1, 1), device="cuda")
+    for f in (lambda: ops.mx4_quantize(x), lambda: ops.mx4_dequantize(q), lambda: ops.mx4_linear(x, q), lambda: ops.moe_combine(x, one.int(), one)):
+        with pytest.raises(N.SmelterError) as e:
+            f()
+        assert e.value.kind == "invalidArgument"
