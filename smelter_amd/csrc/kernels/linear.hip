@@ -6,10 +6,10 @@ template <int XK, int WK, int NB> static int lin_stream_nb(LinearParams p, hipSt
     p.n_tiles = (p.N + cols - 1) / cols;
     p.m_tiles = lin_row_tiles(p, 16);
     const long long blocks = p.m_tiles * p.n_tiles;
-    SM_REQUIRE(blocks < (1ll << 31), "linear: %lld row tiles x %d column tiles exceed one launch", p.m_tiles, p.n_tiles);
     const int chunks = ((p.K + 31) / 32 + (WK == SM_MX4 ? 15 : 3)) / (WK == SM_MX4 ? 16 : 4);
     int waves = blocks >= 4 * SM_NUM_CU ? 4 : 8;                                    // many blocks: fewer sums to join (16 experts bf16 2048 x 2048: 13.2 us with 4 waves, 15.4 with 8; one 4096 x 4096: 15.0, 13.6)
     while (waves > 1 && waves > chunks) waves /= 2;
+    SM_REQUIRE(lin_one_launch(blocks, 64 * waves), "linear: %lld row tiles x %d column tiles exceed one launch", p.m_tiles, p.n_tiles);
     lin_stream_kernel<XK, WK, NB><<<dim3((unsigned)blocks), 64 * waves, (size_t)waves * NB * 16 * 17 * 4, s>>>(p);
     SM_LAUNCH_CHECK();
     return SM_OK;

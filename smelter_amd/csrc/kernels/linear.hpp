@@ -63,6 +63,7 @@ inline long long lin_row_tiles(const LinearParams& p, int BM) {
     const long long groups = p.offsets ? (p.M < p.E ? p.M : p.E) : 1;
     return (p.M + (BM - 1ll) * groups) / BM;
 }
+inline bool lin_one_launch(long long blocks, int threads) { return blocks < (1ll << 32) / threads; }   // a launch counts its threads in 32 bits
 // the tile kernels hold byte offsets inside an expert's weights, and inside x (gathered rows) or the rows of a tile, in 32 bits
 inline bool lin_tile_fits(const LinearParams& p) { return p.w_es < (1ll << 32) && (p.rows ? p.T * p.x_ld : 256 * p.x_ld) < (1ll << 32); }
 // linear_tile.hip: the tile kernels; shape 0 = 128 x 128, 1 = 256 x 256, 2 = 128 columns x 64 slots;  dma = both operands have rows of whole, 16-byte aligned chunks

@@ -251,7 +251,7 @@ template <int XK, int WK, int FM, int ST> static int lin_deep(const LinearParams
     p.n_tiles = (p.N + cols - 1) / cols;
     p.m_tiles = lin_row_tiles(p, S::BM);
     const long long blocks = (p.m_tiles * p.n_tiles + 7) / 8 * 8 * p.splits;
-    SM_REQUIRE(blocks < (1ll << 31), "linear: %lld row tiles x %d column tiles exceed one launch", p.m_tiles, p.n_tiles);
+    SM_REQUIRE(lin_one_launch(blocks, S::THREADS), "linear: %lld row tiles x %d column tiles exceed one launch", p.m_tiles, p.n_tiles);
     const int every = (int)((2ll * p.K + 127) / 128), most = (every + p.splits - 1) / p.splits * 2;
     const auto kernel = lin_deep_kernel<XK, WK, FM, ST>;
     if (int rc = lin_allow_lds_once<S>((const void*)kernel)) return rc;

@@ -605,7 +605,7 @@ template <int XK, int WK, int FR, int WN, int WM, int FN, int FM, bool DMA> stat
     p.n_tiles = (p.N + cols - 1) / cols;
     p.m_tiles = lin_row_tiles(p, S::BM);
     const long long blocks = (p.m_tiles * p.n_tiles + 7) / 8 * 8 * p.splits + (FR == 16 ? SM_NUM_CU / 2 : 0);   // (and the second halves of lin_pick_tile)
-    SM_REQUIRE(blocks < (1ll << 31), "linear: %lld row tiles x %d column tiles exceed one launch", p.m_tiles, p.n_tiles);
+    SM_REQUIRE(lin_one_launch(blocks, S::THREADS), "linear: %lld row tiles x %d column tiles exceed one launch", p.m_tiles, p.n_tiles);
     lin_tile_kernel<XK, WK, FR, WN, WM, FN, FM, DMA><<<dim3((unsigned)blocks), S::THREADS, 0, s>>>(p);
     SM_LAUNCH_CHECK();
     return SM_OK;

@@ -156,3 +156,10 @@ def test_scratch_is_asked_for():
     assert size(C.byref(wide), 1, 0) >= 2 * 4 * (64 * 2 + 8 * 4)
     refused(linear(wide), "workspace")
     refused(linear(desc(M=1 << 30, T=1 << 30, x_type=F32)), "fp32 rows")
+
+
+def test_more_threads_than_one_launch_holds():
+    """2^32 threads and more: refused by name before anything is launched"""
+    refused(linear(desc(M=1 << 20, T=1 << 20, N=1 << 24, K=8)), "one launch")
+    refused(linear(desc(M=1 << 20, T=1 << 20, N=1 << 16, K=8, E=1 << 17), offsets=P), "one launch")
+    refused(linear(desc(M=1 << 20, T=1 << 20, N=1 << 24, K=7)), "one launch")
