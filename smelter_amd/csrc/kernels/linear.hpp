@@ -38,7 +38,9 @@ __device__ __forceinline__ float lin_act(float v, int act, float slope) {
     if (act == SM_ACT_PRELU) return v < 0.f ? v * slope : v;
     return sm_act_other(v, act, slope);
 }
-// the hardware's reciprocal (1 step; below v = -87 its result is 0): a division costs ten instructions a value, 11 us of the 94 of 8192 x 4096 gated columns with K = 2048 in MX4
+// v / (1 + e^-v) by the hardware's reciprocal: a division costs ten instructions a value, 11 us of the 94 of 8192 x 4096 gated columns with K = 2048 in MX4.  What it is off by, relative to the result:
+// the reciprocal 2^-23, the product 2^-24, and 2^-24 |v| of the exponential's argument (v log2(e) rounded once; e^-v is that sensitive to the rounding of v itself).  Below v = -87.3 the result is 0
+// (there |silu| < 2^-119), as the reciprocal of more than 2^126 is.
 __device__ __forceinline__ float lin_silu(float v) { return v * __builtin_amdgcn_rcpf(1.f + __expf(-v)); }
 
 // one rounding to the output type (nearest even)
@@ -72,7 +74,7 @@ int lin_tile_launch(const LinearParams& p, int x_kind, int w_kind, int shape, bo
 int lin_deep_launch(const LinearParams& p, int x_kind, int w_kind, int shape, hipStream_t s);
 int lin_join_launch(const LinearParams& p, hipStream_t s);
 
-struct LinTile { int e; long long row0; int rows; long long index, total; };   // group, first slot, rows of the tile (<= BM); index of the row tile and number of row tiles
+struct LinTile { int e; long long row0; int rows; long long total; };            // group, first slot, rows of the tile (<= BM); number of row tiles
 
 // Row tile `t` of the group list.  Every group is cut into tiles of BM slots; the offsets live on the device, so each wave counts the tiles of 64 groups at a time (prefix sum over the
 // lanes) until it has passed `t`.  Offsets are clamped to 0 .. M, a group that ends before it begins is empty: nothing outside the M slots is ever addressed, whatever they hold.
@@ -82,7 +84,7 @@ __device__ __forceinline__ long long lin_uniform(long long v) {                 
     return ((long long)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32) | (unsigned)__builtin_amdgcn_readfirstlane((int)v);
 }
 __device__ __forceinline__ LinTile lin_find_tile(const LinearParams& p, int BM, long long t, bool want_total) {
-    LinTile r; r.e = 0; r.row0 = 0; r.rows = 0; r.index = t; r.total = 0;
+    LinTile r; r.e = 0; r.row0 = 0; r.rows = 0; r.total = 0;
     if (!p.offsets) {
         r.total = (p.M + BM - 1) / BM;
         if (t < r.total) { r.row0 = t * BM; long long left = p.M - r.row0; r.rows = (int)(left < BM ? left : BM); }
