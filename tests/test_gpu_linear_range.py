@@ -138,6 +138,51 @@ def test_fp32_rows_on_fp16_weights_one_by_one():
     assert got[0].eq(INF).all() and got[1].eq(-INF).all() and got[2:4].isnan().all() and got[4].eq(1).all()
 
 
+@pytest.mark.parametrize("weights", [F16, BF16])
+def test_fp32_rows_more_than_blocks(weights):
+    """a block takes several slots, ordinary and odd ones after one another"""
+    g = gen(8)
+    m, n, k = 40000, 24, 72
+    x, w = fp32_rows(g, m, k), (randn(g, 2, n, k) / 8).to(weights)
+    rows = torch.randperm(m, generator=g, device="cuda").int()
+    rows[5::7] = -1
+    off = torch.tensor([0, 15000, m], dtype=torch.int32, device="cuda")
+    same_as_fp64(x, w, w.double(), off, rows, randn(g, 2, n), False, F32)
+
+
+@pytest.mark.parametrize("weights", [F16, BF16])
+@pytest.mark.parametrize("m", [4, 700])
+def test_fp32_rows_beside_their_outputs(weights, m):
+    """slots that no group covers, and what lies beside the outputs, stay as they were, whichever way a row is multiplied"""
+    g = gen(9)
+    n, k = 40, 96
+    x, w = fp32_rows(g, m, k), (randn(g, 2, n, k) / 8).to(weights)
+    for dtype in (F32, F16):
+        out = torch.full((m + 2, n + 7), 7.0, dtype=dtype, device="cuda")
+        off = torch.tensor([1, m // 2, m - 1], dtype=torch.int32, device="cuda")
+        ops.expert_linear(x, w, off, out=out[1:m + 1, 2:n + 2])
+        whole = ops.expert_linear(x, w, torch.tensor([0, m // 2, m], dtype=torch.int32, device="cuda"), dtype=dtype)
+        assert torch.equal(out[2:m, 2:n + 2], whole[1:m - 1])
+        out[2:m, 2:n + 2] = 7
+        assert out.eq(7).all()
+
+
+def test_fp32_rows_on_two_streams():
+    """two calls at once, each with scratch of its own"""
+    g = gen(10)
+    xs, w = [fp32_rows(g, 300, 520) for _ in range(2)], (randn(g, 1, 264, 520) / 16).to(F16)
+    off = torch.tensor([0, 300], dtype=torch.int32, device="cuda")
+    want = [ops.expert_linear(x, w, off) for x in xs]
+    streams, got = [torch.cuda.Stream(), torch.cuda.Stream()], [[], []]
+    torch.cuda.synchronize()
+    for _ in range(8):
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(ops.expert_linear(xs[i], w, off))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, want[i]) for i in range(2) for a in got[i])
+
+
 def test_fp32_rows_on_fp16_weights_in_a_graph():
     """which rows are multiplied in another way is decided on the device: a replay goes by the present rows"""
     g = gen(3)
