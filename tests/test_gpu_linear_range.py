@@ -118,6 +118,23 @@ def test_fp32_rows_at_the_end_of_the_range():
         assert torch.equal(got, torch.tensor([[INF], [-INF], [INF], [INF]], device="cuda").expand(4, 8))
 
 
+@pytest.mark.parametrize("reach", [20, 37, 38, 39, 60])
+@pytest.mark.parametrize("m, n, k", [(6, 40, 96), (90, 256, 520), (700, 1000, 264)])
+def test_fp32_rows_at_the_edge_of_fp16_parts(reach, m, n, k):
+    """elements down to 2^-reach of the first, which meets weights of zero: each is there with all its bits"""
+    g = gen(reach)
+    x = (1 + torch.rand((m, k), generator=g, device="cuda")) * torch.exp2(-torch.randint(0, reach + 1, (m, k), generator=g, device="cuda").float())
+    x = x * torch.exp2(torch.randint(-60, 60, (m, 1), generator=g, device="cuda").float())
+    x[::3] *= 2.0 ** -(reach - 1)
+    x[:, 0] = x[:, 1:].amax(1) * (2.0 ** reach if reach < 38 else 1.0)
+    w = (randn(g, 1, n, k) / 8).to(F16)
+    w[..., 0] = 0
+    w[:, ::2, 1:] *= (x[0, 1:] < x[0, 1:].amax() * 2.0 ** -(reach // 2)).half()       # rows of weights that meet small elements only
+    off = torch.tensor([0, m], dtype=torch.int32, device="cuda")
+    xv, wv = x.double(), w[0].double()
+    inside(ops.expert_linear(x, w, off), xv @ wv.t(), chain(3 * k) * (xv.abs() @ wv.abs().t()) + 2.0 ** -126)
+
+
 def test_fp32_rows_on_fp16_weights_one_by_one():
     """values whose fp16 form is an infinity, coarse or zero"""
     off = torch.tensor([0, 5], dtype=torch.int32, device="cuda")
