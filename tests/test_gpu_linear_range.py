@@ -1,5 +1,7 @@
 """Linear and expert layers over the whole range of their operands: rows of very large, very small and mixed values, weights whose scales lie far apart.
 Every limit here is relative to the sum of the products' own magnitudes: nothing is allowed for values that a product does not hold."""
+import ctypes as C
+
 import pytest
 import torch
 
@@ -153,6 +155,29 @@ def test_fp32_rows_on_fp16_weights_one_by_one():
     odd = torch.tensor([[INF, 1e-9], [-INF, 1e-9], [NAN, 1.0], [INF, -INF], [1e-9, 1.0]], device="cuda")
     got = ops.expert_linear(odd, torch.ones((1, 8, 2), dtype=F16, device="cuda"), off)
     assert got[0].eq(INF).all() and got[1].eq(-INF).all() and got[2:4].isnan().all() and got[4].eq(1).all()
+
+
+@pytest.mark.parametrize("weights", [F16, "mx4"])
+@pytest.mark.parametrize("act, slope, f", [(ops.ACT_RELU, 0.0, lambda z: z.clamp(min=0)), (ops.ACT_PRELU, 0.25, lambda z: torch.where(z < 0, 0.25 * z, z)), (ops.ACT_CLIP, 0.5, lambda z: z.clamp(0, 0.5))])
+@pytest.mark.parametrize("m", [5, 200])
+def test_fp32_rows_without_groups(weights, act, slope, f, m):
+    """one layer without offsets, with activations (their slopes are at most 1): from Python, and through the C interface for fp16 weights"""
+    g = gen(m)
+    n, k = 72, 200
+    x, w, bias = fp32_rows(g, m, k), randn(g, n, k) * k ** -0.5, randn(g, n)
+    if weights == "mx4":
+        w = ops.mx4_quantize(w)
+        wv = ops.mx4_dequantize(w, F32).double()
+        got = ops.mx4_linear(x, w, bias, act=act, slope=slope)
+    else:
+        w = w.to(weights)
+        wv, got = w.double(), torch.empty((m, n), device="cuda")
+        d = N.LinearDesc(m, m, n, k, 1, 2, 0, 2, act, slope, 0, 0, 0)
+        size = N.lib().sm_linear_workspace_bytes(C.byref(d), 0, 0)
+        work = torch.empty(size, dtype=torch.uint8, device="cuda")
+        N.check(N.lib().sm_linear_fwd(C.byref(d), x.data_ptr(), None, w.data_ptr(), None, bias.data_ptr(), None, None, got.data_ptr(), work.data_ptr(), size, torch.cuda.current_stream().cuda_stream))
+    z, mag = x.double() @ wv.t() + bias.double(), x.double().abs() @ wv.abs().t()
+    inside(got, f(z), chain(3 * k) * mag + 2.0 ** -23 * z.abs() + 2.0 ** -126)
 
 
 @pytest.mark.parametrize("weights", [F16, BF16])
