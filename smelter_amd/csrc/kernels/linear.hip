@@ -108,7 +108,7 @@ template <class H> __global__ __launch_bounds__(256) void lin_parts_kernel(const
             for (int k = 4 * threadIdx.x; k < K && live; k += 1024) {
                 const floatx4 v = lin_load4(src, k, K);
 #pragma unroll
-                for (int q = 0; q < 4; q++) { const float f = v[q]; const unsigned b = __builtin_bit_cast(unsigned, f) & 0x7fffffffu; hi = hi > b ? hi : b; if (b) lo = lo < b ? lo : b; }
+                for (int q = 0; q < 4; q++) { const float f = v[q] /* (__builtin_bit_cast of a vector element takes the first) */; const unsigned b = __builtin_bit_cast(unsigned, f) & 0x7fffffffu; hi = hi > b ? hi : b; if (b) lo = lo < b ? lo : b; }
             }
 #pragma unroll
             for (int d = 1; d < 64; d <<= 1) { const unsigned a = __shfl_xor(hi, d), c = __shfl_xor(lo, d); hi = hi > a ? hi : a; lo = lo < c ? lo : c; }
